@@ -1,0 +1,874 @@
+// 8-bit StreamingLLM ring cache: write (quantise), attend, read back.
+//
+// Format.  One sequence b and key/value head h own R = sink + window rows of
+// DP codes (DP = head_dim rounded up to 64, 128 or 256; the columns behind
+// head_dim hold 0) for K and for V, and one pair of scale bytes (K, V) per
+// row.  Row r < sink holds position r, position p >= sink lives in row
+// sink + (p - sink) % window.  A row x is stored as codes c and byte e + 127,
+//   e = least integer with max|x| <= top * 2^e  (top = 448 e4m3, 127 int8),
+//   c = x * 2^-e rounded to the code type, ties to even,
+// so the scaling itself is exact, every code carries one rounding, and c * 2^e
+// is exact in fp32.  e >= -126; an all-zero row has e = 0.  A row with a NaN
+// or an infinity is stored as byte 255 with zero codes and reads as NaN.  A
+// code may round a value next to the 16-bit type's largest up past it: what
+// is read, and an attention's result, saturates there instead of overflowing.
+//
+// Every sequence has its own length L on the device, so a batch may be ragged
+// and a captured step advances when it is replayed.  The visible rows of the
+// query at position L - 1 are always rows [0, min(L, R)): before the ring is
+// full they are the positions in order, afterwards all of them are in the
+// window or sinks, and attention does not depend on the order of its keys.
+#include <cooperative_groups.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "quant_cache.cuh"
+#include "tc_prims.cuh"
+
+namespace sbfa {
+namespace {
+
+namespace cg = cooperative_groups;
+using tc::ex2;
+using tc::smem_u32;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kFull = 0xffffffffu;
+constexpr uint32_t kBadRow = 255;   // scale byte of a row with a NaN or an infinity
+
+// ---------------------------------------------------------------------------
+// codes and scales
+// ---------------------------------------------------------------------------
+
+// Scale byte of a row whose largest magnitude has the fp32 bits `amax`.
+template <int FMT>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+  if (amax >= 0x7f800000u) return kBadRow;
+  if (amax == 0) return 127;
+  // amax = f * 2^E, f in [1, 2); top = 1.75 * 2^8 or 1.984375 * 2^6
+  constexpr int kTopExp = FMT == SBFA_Q_E4M3 ? 8 : 6;
+  constexpr uint32_t kTopMant = FMT == SBFA_Q_E4M3 ? 0x600000u : 0x7e0000u;
+  const int e = (int)(amax >> 23) - kTopExp + ((amax & 0x7fffffu) > kTopMant ? 1 : 0);
+  return (uint32_t)max(e, 1);   // biased; subnormal amax gives e <= 1 as well
+}
+// 2^(byte - 127); NaN for a bad row.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == kBadRow ? 0x7fc00000u : byte << 23);
+}
+// 2^(127 - byte), the factor a row is multiplied by before rounding
+__device__ __forceinline__ float scale_inverse(uint32_t byte) {
+  return __uint_as_float((254u - byte) << 23);
+}
+
+// Four values (already scaled) to four codes.
+template <int FMT>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  if constexpr (FMT == SBFA_Q_E4M3) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+  } else {
+    // |x| <= 127 by the choice of the scale
+    const uint32_t x = (uint32_t)__float2int_rn(a) & 0xffu, y = (uint32_t)__float2int_rn(b) & 0xffu;
+    const uint32_t z = (uint32_t)__float2int_rn(c) & 0xffu, w = (uint32_t)__float2int_rn(d) & 0xffu;
+    return x | (y << 8) | (z << 16) | (w << 24);
+  }
+}
+// Codes 0, 1 (lo) and 2, 3 (hi) of a word as half pairs (exact).
+template <int FMT>
+__device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == SBFA_Q_E4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    // code + 128 in the low byte of a half with exponent 2^10 is 1024 + 128
+    // + code exactly; one subtraction leaves the code
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias);
+    __half2 hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+    lo = *reinterpret_cast<uint32_t*>(&ha);
+    hi = *reinterpret_cast<uint32_t*>(&hb);
+  }
+}
+
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w));
+}
+
+// x limited to T's finite range (NaN stays)
+template <typename T>
+__device__ __forceinline__ float saturated(float x) {
+  constexpr float top = std::is_same<T, __half>::value ? 65504.f : 3.38953138925153547590e38f;
+  return fabsf(x) > top ? copysignf(top, x) : x;
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+// A group of DP / 8 lanes takes one (head, token): 16 bytes of K and of V per
+// lane, the row maxima by shuffles, 8 code bytes back.  Bound by HBM: 4 D bytes
+// in, 2 D + 2 out per head and token.  The tokens of a head are adjacent, so
+// that their scale pairs fill whole sectors.  The last CTA of a sequence moves
+// its length on (a ticket per sequence, left at zero), which saves the launch of
+// a second kernel at the end of every decode step.
+constexpr int kAppThreads = 256;
+constexpr int kAppUnroll = 2;
+
+template <typename T, int FMT, int G>
+__global__ void __launch_bounds__(kAppThreads)
+    qcache_append_kernel(QCache c, int64_t* __restrict__ lengths, int32_t* __restrict__ tickets,
+                         const T* __restrict__ kn, const T* __restrict__ vn, Strides3 sk,
+                         Strides3 sv, const int64_t* __restrict__ counts, int64_t n_new) {
+  constexpr int DP = G * 8;
+  constexpr int kRows = kAppThreads / G;
+  const int b = blockIdx.y;
+  const int lane = threadIdx.x % G;
+  const int64_t len = max(lengths[b], (int64_t)0);
+  const int64_t cnt = counts ? min(max(counts[b], (int64_t)0), n_new) : n_new;
+  const int64_t end = len + cnt;
+  const int64_t items = n_new * c.heads;
+  const bool on = lane * 8 < c.d;
+  for (int64_t i0 = (int64_t)blockIdx.x * kRows * kAppUnroll; i0 < items;
+       i0 += (int64_t)gridDim.x * kRows * kAppUnroll) {
+    uint4 xk[kAppUnroll], xv[kAppUnroll];
+    int64_t dst[kAppUnroll];
+#pragma unroll
+    for (int u = 0; u < kAppUnroll; ++u) {
+      const int64_t i = i0 + u * kRows + threadIdx.x / G;
+      const int64_t h = i / n_new, t = i - h * n_new;
+      const int64_t p = len + t;
+      // padding, or a position that a later token of this call overwrites
+      const bool skip = i >= items || t >= cnt || (p >= c.sink && p < end - c.window);
+      xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
+      dst[u] = -1;
+      if (!skip) {
+        const int64_t row = p < c.sink ? p : c.sink + (p - c.sink) % c.window;
+        dst[u] = ((int64_t)b * c.heads + h) * c.rows + row;
+        if (on) {
+          xk[u] = __ldcs(reinterpret_cast<const uint4*>(kn + b * sk.b + h * sk.h + t * sk.n) + lane);
+          xv[u] = __ldcs(reinterpret_cast<const uint4*>(vn + b * sv.b + h * sv.h + t * sv.n) + lane);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAppUnroll; ++u) {
+      uint32_t bytes = 0;
+      uint2 codes[2];
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const uint4 w = part == 0 ? xk[u] : xv[u];
+        float2 f[4] = {unpack2<T>(w.x), unpack2<T>(w.y), unpack2<T>(w.z), unpack2<T>(w.w)};
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          m = max(m, max(__float_as_uint(f[j].x) & 0x7fffffffu,
+                         __float_as_uint(f[j].y) & 0x7fffffffu));
+#pragma unroll
+        for (int s = G / 2; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(kFull, m, s, G));
+        const uint32_t e = scale_byte<FMT>(m);
+        bytes |= e << (8 * part);
+        const float inv = e == kBadRow ? 0.f : scale_inverse(e);
+        if (e == kBadRow) {
+          codes[part] = make_uint2(0, 0);
+        } else {
+          codes[part].x = encode4<FMT>(f[0].x * inv, f[0].y * inv, f[1].x * inv, f[1].y * inv);
+          codes[part].y = encode4<FMT>(f[2].x * inv, f[2].y * inv, f[3].x * inv, f[3].y * inv);
+        }
+      }
+      if (dst[u] >= 0) {
+        reinterpret_cast<uint2*>(c.k + dst[u] * DP)[lane] = codes[0];
+        reinterpret_cast<uint2*>(c.v + dst[u] * DP)[lane] = codes[1];
+        if (lane == 0) c.scales[dst[u]] = (uint16_t)bytes;
+      }
+    }
+  }
+  // every CTA of this sequence has read its length before the last one writes it
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    if (gridDim.x == 1) {
+      lengths[b] = end;
+    } else {
+      __threadfence();
+      if (atomicAdd(&tickets[b], 1) == (int)gridDim.x - 1) {
+        tickets[b] = 0;
+        lengths[b] = end;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// read back
+// ---------------------------------------------------------------------------
+// Out row i of a sequence is its i-th kept position in order (sinks, then the
+// window from its oldest), rows behind the last one are zero with position -1.
+// A group of DP / 8 lanes per row as above; bound by HBM (2 D + 2 bytes in, 4 D
+// out per kept row and head).
+constexpr int kReadThreads = 256;
+constexpr int kReadUnroll = 4;
+
+template <typename T, int FMT>
+__device__ __forceinline__ uint4 values8(uint2 codes, float scale) {
+  uint32_t h[4];
+  decode4<FMT>(codes.x, h[0], h[1]);
+  decode4<FMT>(codes.y, h[2], h[3]);
+  uint32_t r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[j]));
+    r[j] = tc::pack2<T>(saturated<T>(f.x * scale), saturated<T>(f.y * scale));
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <typename T, int FMT, int G>
+__global__ void __launch_bounds__(kReadThreads)
+    qcache_read_kernel(QCache c, const int64_t* __restrict__ lengths, T* __restrict__ ko,
+                       T* __restrict__ vo, int64_t* __restrict__ positions) {
+  constexpr int DP = G * 8;
+  constexpr int kRows = kReadThreads / G;
+  const int b = blockIdx.y;
+  const int lane = threadIdx.x % G;
+  const int64_t len = max(lengths[b], (int64_t)0);
+  const int64_t items = c.rows * c.heads;
+  const bool on = lane * 8 < c.d;
+  for (int64_t i0 = (int64_t)blockIdx.x * kRows * kReadUnroll; i0 < items;
+       i0 += (int64_t)gridDim.x * kRows * kReadUnroll) {
+    uint2 xk[kReadUnroll], xv[kReadUnroll];
+    uint32_t sc[kReadUnroll];
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u) {
+      const int64_t i = i0 + u * kRows + threadIdx.x / G;
+      xk[u] = xv[u] = make_uint2(0, 0);
+      sc[u] = 0x7f7f;
+      if (i >= items) continue;
+      const int64_t h = i / c.rows, r = i - h * c.rows;
+      const bool kept = r < min(len, c.rows);
+      // position, and the ring row that holds it
+      const int64_t p = r < c.sink || len <= c.rows ? r : len - c.window + r - c.sink;
+      if (lane == 0 && h == 0) positions[b * c.rows + r] = kept ? p : -1;
+      if (!kept) continue;
+      const int64_t row = p < c.sink ? p : c.sink + (p - c.sink) % c.window;
+      const int64_t src = ((int64_t)b * c.heads + h) * c.rows + row;
+      xk[u] = __ldcs(reinterpret_cast<const uint2*>(c.k + src * DP) + lane);
+      xv[u] = __ldcs(reinterpret_cast<const uint2*>(c.v + src * DP) + lane);
+      sc[u] = c.scales[src];
+    }
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u) {
+      const int64_t i = i0 + u * kRows + threadIdx.x / G;
+      if (i >= items || !on) continue;
+      const int64_t dst = ((int64_t)b * items + i) * c.d + lane * 8;
+      __stcs(reinterpret_cast<uint4*>(ko + dst), values8<T, FMT>(xk[u], scale_value(sc[u] & 255u)));
+      __stcs(reinterpret_cast<uint4*>(vo + dst), values8<T, FMT>(xv[u], scale_value(sc[u] >> 8)));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// attend (one query position per sequence)
+// ---------------------------------------------------------------------------
+// O = softmax(scale q K^T) V over rows [0, min(L, R)).  Per key/value head the
+// rows are read once for 8 * NQ query heads of its group.  Bound by HBM: 2 D + 2
+// bytes per row against 8 * NQ * 4 D operations.
+//
+// Both products put the cache on the M side of mma.m16n8k16 (fp16 in, fp32 out)
+// and the query heads on the N side, which lets every lane load its operands
+// straight from global memory in 16-byte pieces, without shared memory:
+//   S^T = K Q^T: lane (g, c) = (lane / 4, lane % 4) holds bytes [16 c, 16 c + 16) of
+//     each 64-byte piece of rows g and g + 8; the order of the summed d does not
+//     matter as long as Q's fragment uses the same one;
+//   O^T = V^T P^T: lane (g, c) holds its DP / 8 bytes of rows 2c, 2c + 1, 2c + 8 and
+//     2c + 9; byte permutes pair two keys of one d, and the m16 tiles number the d's
+//     so that a lane's own columns are its rows g and g + 8.
+// P^T comes out of the score fragment with movmatrix.  Codes become fp16 exactly.
+//
+// Scales: a key's 2^ek multiplies its score in fp32.  A value row's 2^ev is folded
+// into the exponent of its weight: P' = 2^(x + ev - M), M a running bound of x + ev, so P'
+// is at most 2^kSlack and keeps fp16's 11 bits whatever the magnitudes of the rows, while
+// the row sum l = sum 2^(x - m) has its own per-lane maximum m (both in fp32); the result is
+// acc / l * 2^(M - m).  Q is scaled by a power of two into fp16's range, which is exact
+// for fp16 inputs and for bf16 down to 2^-38 of the row's largest element.
+//
+// A cluster of NS CTAs shares one unit (sequence, head, group of queries); its warps
+// take every (4 NS)-th step of KS rows, so that any length splits evenly without being
+// known to the host.  Warps merge through shared memory, CTAs through distributed
+// shared memory: no workspace and no second launch.
+constexpr int kAttWarps = 4;
+constexpr float kSlack = 4.f;
+
+template <int DP, int NQ>
+struct AttCfg {
+  static constexpr int kTiles = (DP == 256 || NQ == 2) ? 1 : 2;   // 16-row tiles per step
+  static constexpr int kRowsQ = 8 * NQ;
+  static constexpr int kCtas = DP == 256 ? 2 : 3;                 // aimed at per SM
+  // per warp: O [8 NQ][DP + 4]; M, m, l [8 NQ]
+  static constexpr int kPitch = DP + 4;
+  static constexpr size_t kBytes = (size_t)kAttWarps * kRowsQ * (kPitch + 3) * sizeof(float);
+};
+
+__device__ __forceinline__ uint4 ldg16(const uint8_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ldg8(const uint8_t* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
+               : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ldg2(const uint16_t* p) {
+  uint16_t r;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(r) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+template <typename T, int FMT, int DP, int NQ>
+__global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
+    qcache_attend_kernel(const T* __restrict__ q, QCache c, const int64_t* __restrict__ lengths,
+                         T* __restrict__ o, float* __restrict__ o32, float* __restrict__ lse,
+                         float scale_log2, int group, int chunks, int ns) {
+  using C = AttCfg<DP, NQ>;
+  constexpr int KT = C::kTiles, KS = 16 * KT;
+  constexpr int NCH = DP / 64;      // 16-byte pieces of a K row per lane
+  constexpr int VW = DP / 32;       // words of a V row per lane
+  extern __shared__ __align__(16) float att_smem[];
+  const int rank = blockIdx.x % ns;
+  const int64_t unit = blockIdx.x / ns;
+  const int64_t bh = unit / chunks;                       // (sequence, key/value head)
+  const int h0 = (int)(unit % chunks) * C::kRowsQ;        // first head of the group
+  const int nq = min(C::kRowsQ, group - h0);
+  const int b = (int)(bh / c.heads);
+  const int64_t qrow0 = bh * group + h0;                  // row of q, o, lse
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, cc = lane & 3;
+  const int64_t len = lengths[b];
+  const int n = (int)min(max(len, (int64_t)0), c.rows);
+
+  // Q fragments, column g of each n-tile, scaled into fp16's range
+  uint32_t qf[NQ][DP / 16][2];
+  float qs[NQ][2];   // softmax scale (base 2) over the two query columns of this lane
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    const int r = t * 8 + g;
+    uint32_t raw[NCH][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+      for (int hlf = 0; hlf < 2; ++hlf) {
+        const int col = j * 64 + cc * 16 + hlf * 8;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (r < nq && col < c.d)
+          w = __ldg(reinterpret_cast<const uint4*>(q + (qrow0 + r) * c.d + col));
+        raw[j][4 * hlf] = w.x;
+        raw[j][4 * hlf + 1] = w.y;
+        raw[j][4 * hlf + 2] = w.z;
+        raw[j][4 * hlf + 3] = w.w;
+      }
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = unpack2<T>(raw[j][i]);
+        m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+      }
+    m = max(m, __shfl_xor_sync(kFull, m, 1));
+    m = max(m, __shfl_xor_sync(kFull, m, 2));
+    // largest element to [2^14, 2^15); fp16 needs none of it (its own range)
+    int e = 0;
+    if (sizeof(T) == 2 && !std::is_same<T, __half>::value && m != 0 && m < 0x7f800000u)
+      e = max(-120, (int)(m >> 23) - 127 - 14);
+    const float f_in = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = unpack2<T>(raw[j][i]);
+        qf[t][j * 4 + (i >> 1)][i & 1] = tc::pack2<__half>(f.x * f_in, f.y * f_in);
+      }
+    const float f_out = __uint_as_float((uint32_t)(127 + e) << 23) * scale_log2;
+    qs[t][0] = __shfl_sync(kFull, f_out, (2 * cc) * 4);
+    qs[t][1] = __shfl_sync(kFull, f_out, (2 * cc + 1) * 4);
+  }
+
+  const uint8_t* kb = c.k + bh * c.rows * DP;
+  const uint8_t* vb = c.v + bh * c.rows * DP;
+  const uint16_t* sb = c.scales + bh * c.rows;
+  const int steps = (n + KS - 1) / KS;
+  const int stride = ns * kAttWarps;
+
+  uint4 kr[KT][2][NCH];
+  uint32_t vr[KT][4][VW];
+  uint32_t sc[KT][2], sc_next[KT][2];
+  auto load_k = [&](int s) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = min(s * KS + t * 16 + i * 8 + g, n - 1);
+        const uint8_t* p = kb + (int64_t)row * DP + cc * 16;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) kr[t][i][j] = ldg16(p + j * 64);
+        sc_next[t][i] = ldg2(sb + row);
+      }
+  };
+  auto load_v = [&](int s) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = min(s * KS + t * 16 + (i >> 1) * 8 + 2 * cc + (i & 1), n - 1);
+        const uint8_t* p = vb + (int64_t)row * DP;
+        if constexpr (DP == 64) {
+          const uint2 w = ldg8(p + g * 8);
+          vr[t][i][0] = w.x;
+          vr[t][i][1] = w.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < VW / 4; ++j) {
+            const uint4 w = ldg16(p + j * 128 + g * 16);
+            vr[t][i][4 * j] = w.x;
+            vr[t][i][4 * j + 1] = w.y;
+            vr[t][i][4 * j + 2] = w.z;
+            vr[t][i][4 * j + 3] = w.w;
+          }
+        }
+      }
+  };
+
+  float acc[NQ][2 * VW][4];
+  float M[NQ][2], m[NQ][2], l[NQ][2];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+#pragma unroll
+    for (int i = 0; i < 2 * VW; ++i) acc[t][i][0] = acc[t][i][1] = acc[t][i][2] = acc[t][i][3] = 0.f;
+    M[t][0] = M[t][1] = m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+  }
+
+  int s = rank * kAttWarps + warp;
+  if (s < steps) {
+    load_k(s);
+    load_v(s);
+  }
+  for (; s < steps; s += stride) {
+    const bool more = s + stride < steps;
+    // S^T, one 16-row tile of keys by 8 query columns each
+    float x[NQ][KT][4];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      sc[t][0] = sc_next[t][0];
+      sc[t][1] = sc_next[t][1];
+#pragma unroll
+      for (int u = 0; u < NQ; ++u) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        const uint32_t w0[4] = {kr[t][0][j].x, kr[t][0][j].y, kr[t][0][j].z, kr[t][0][j].w};
+        const uint32_t w1[4] = {kr[t][1][j].x, kr[t][1][j].y, kr[t][1][j].z, kr[t][1][j].w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t a0, a1, a2, a3;
+          decode4<FMT>(w0[w], a0, a2);
+          decode4<FMT>(w1[w], a1, a3);
+#pragma unroll
+          for (int u = 0; u < NQ; ++u)
+            mma_f16(x[u][t], a0, a1, a2, a3, qf[u][j * 4 + w][0], qf[u][j * 4 + w][1]);
+        }
+      }
+    }
+    if (more) load_k(s + stride);
+    // online softmax; element e of a tile is key g + 8 (e / 2), query 2 cc + e % 2
+    uint32_t pb[NQ][KT][2];
+#pragma unroll
+    for (int u = 0; u < NQ; ++u) {
+      float y[KT][4];
+      float mx[2] = {-INFINITY, -INFINITY}, my[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = s * KS + t * 16 + (e >> 1) * 8 + g;
+          const uint32_t sv = sc[t][e >> 1] >> 8;
+          const float ev = sv == kBadRow ? __uint_as_float(0x7fc00000u) : (float)((int)sv - 127);
+          const float xs = x[u][t][e] * (scale_value(sc[t][e >> 1] & 255u) * qs[u][e & 1]);
+          const bool in = key < n;
+          x[u][t][e] = in ? xs : -INFINITY;
+          y[t][e] = in ? xs + ev : -INFINITY;
+          mx[e & 1] = fmaxf(mx[e & 1], x[u][t][e]);
+          my[e & 1] = fmaxf(my[e & 1], y[t][e]);
+        }
+      bool grow = false;
+      float old[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // row sum: this lane's own keys against its own maximum
+        const float mn = fmaxf(m[u][i], mx[i]);
+        const float r = mn == -INFINITY ? 0.f : mn;
+        l[u][i] *= ex2(m[u][i] - r);
+        m[u][i] = mn;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+          l[u][i] += ex2(x[u][t][i] - r) + ex2(x[u][t][2 + i] - r);
+        // the accumulator's reference is shared by the warp's keys of a query
+        my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 4));
+        my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 8));
+        my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 16));
+        old[i] = M[u][i];
+        if (my[i] > M[u][i] + (M[u][i] == -INFINITY ? 0.f : kSlack)) {
+          M[u][i] = my[i];
+          grow = true;
+        }
+      }
+      if (__any_sync(kFull, grow)) {
+        float a[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) a[i] = old[i] == M[u][i] ? 1.f : ex2(old[i] - M[u][i]);
+#pragma unroll
+        for (int i = 0; i < 2 * VW; ++i) {
+          acc[u][i][0] *= a[0];
+          acc[u][i][1] *= a[1];
+          acc[u][i][2] *= a[0];
+          acc[u][i][3] *= a[1];
+        }
+      }
+      const float r0 = M[u][0] == -INFINITY ? 0.f : M[u][0];
+      const float r1 = M[u][1] == -INFINITY ? 0.f : M[u][1];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        pb[u][t][0] = movmatrix(tc::pack2<__half>(ex2(y[t][0] - r0), ex2(y[t][1] - r1)));
+        pb[u][t][1] = movmatrix(tc::pack2<__half>(ex2(y[t][2] - r0), ex2(y[t][3] - r1)));
+      }
+    }
+    // O^T += V^T P^T
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        uint32_t a[2][4];   // the word's four columns make two m16 tiles
+        decode4<FMT>(__byte_perm(vr[t][0][w], vr[t][1][w], 0x5140), a[0][0], a[0][1]);
+        decode4<FMT>(__byte_perm(vr[t][2][w], vr[t][3][w], 0x5140), a[0][2], a[0][3]);
+        decode4<FMT>(__byte_perm(vr[t][0][w], vr[t][1][w], 0x7362), a[1][0], a[1][1]);
+        decode4<FMT>(__byte_perm(vr[t][2][w], vr[t][3][w], 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+        for (int u = 0; u < NQ; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            mma_f16(acc[u][2 * w + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[u][t][0],
+                    pb[u][t][1]);
+      }
+    if (more) load_v(s + stride);
+  }
+
+  // ---- merge: lanes, then warps, then the CTAs of the cluster
+  float* so = att_smem;                                         // [warp][row][kPitch]
+  float* sM = so + kAttWarps * C::kRowsQ * C::kPitch;           // [warp][row] M, m, l
+  float* sm = sM + kAttWarps * C::kRowsQ;
+  float* sl = sm + kAttWarps * C::kRowsQ;
+#pragma unroll
+  for (int u = 0; u < NQ; ++u)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        const float m2 = __shfl_xor_sync(kFull, m[u][i], d);
+        const float l2 = __shfl_xor_sync(kFull, l[u][i], d);
+        const float mn = fmaxf(m[u][i], m2);
+        const float r = mn == -INFINITY ? 0.f : mn;
+        l[u][i] = l[u][i] * ex2(m[u][i] - r) + l2 * ex2(m2 - r);
+        m[u][i] = mn;
+      }
+      const int row = warp * C::kRowsQ + u * 8 + 2 * cc + i;
+      if (g == 0) {
+        sM[row] = M[u][i];
+        sm[row] = m[u][i];
+        sl[row] = l[u][i];
+      }
+      // lane g's columns: word w, bytes 2 t, 2 t + 1 (m16 tile t of the word)
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const int col = DP == 64 ? g * 8 + 4 * w : (w >> 2) * 128 + g * 16 + 4 * (w & 3);
+        *reinterpret_cast<float4*>(so + row * C::kPitch + col) =
+            make_float4(acc[u][2 * w][i], acc[u][2 * w][2 + i], acc[u][2 * w + 1][i],
+                        acc[u][2 * w + 1][2 + i]);
+      }
+    }
+  __syncthreads();
+  if (ns > 1) cg::this_cluster().sync();
+  // this CTA's share of the unit's rows, four columns per thread, over all warps of
+  // all CTAs: NaN results come through the sums, maxima ignore them
+  const int parts = kAttWarps * ns;
+  for (int idx = rank * (kAttWarps * 32) + threadIdx.x; idx < nq * (DP / 4);
+       idx += ns * kAttWarps * 32) {
+    const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
+    auto at = [&](float* p, int w) -> float* {
+      float* mine = p + (w % kAttWarps) * C::kRowsQ;
+      return ns > 1 ? cg::this_cluster().map_shared_rank(mine, w / kAttWarps) : mine;
+    };
+    float Mx = -INFINITY, mx = -INFINITY;
+    for (int w = 0; w < parts; ++w) {
+      Mx = fmaxf(Mx, at(sM, w)[row]);
+      mx = fmaxf(mx, at(sm, w)[row]);
+    }
+    const float rM = Mx == -INFINITY ? 0.f : Mx, rm = mx == -INFINITY ? 0.f : mx;
+    float L = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < parts; ++w) {
+      L += at(sl, w)[row] * ex2(at(sm, w)[row] - rm);
+      const float f = ex2(at(sM, w)[row] - rM);
+      float* mine = so + ((w % kAttWarps) * C::kRowsQ + row) * C::kPitch + col;
+      const float4 p = *reinterpret_cast<const float4*>(
+          ns > 1 ? cg::this_cluster().map_shared_rank(mine, w / kAttWarps) : mine);
+      a.x += p.x * f;
+      a.y += p.y * f;
+      a.z += p.z * f;
+      a.w += p.w * f;
+    }
+    const bool some = !(L == 0.f);
+    const float inv = some ? 1.f / L : 0.f;
+    const float back = ex2(rM - rm);
+    a.x = some ? saturated<T>(a.x * inv * back) : 0.f;
+    a.y = some ? saturated<T>(a.y * inv * back) : 0.f;
+    a.z = some ? saturated<T>(a.z * inv * back) : 0.f;
+    a.w = some ? saturated<T>(a.w * inv * back) : 0.f;
+    const int64_t out = qrow0 + row;
+    if (col < c.d) {
+      if (o32)
+        *reinterpret_cast<float4*>(o32 + out * c.d + col) = a;
+      else
+        *reinterpret_cast<uint2*>(o + out * c.d + col) =
+            make_uint2(tc::pack2<T>(a.x, a.y), tc::pack2<T>(a.z, a.w));
+    }
+    // a partial result marks an empty row by -inf, the public one by 0
+    if (col == 0 && lse)
+      lse[out] = some ? (mx + log2f(L)) * kLn2 : (o32 ? -INFINITY : 0.f);
+  }
+  if (ns > 1) cg::this_cluster().sync();   // peers may still read this CTA's memory
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+int padded_dim(int64_t d) {
+  if (d <= 0 || d > 256 || d % 8 != 0) return 0;
+  return d <= 64 ? 64 : d <= 128 ? 128 : 256;
+}
+
+int check_qcache(const void* k, const void* v, const void* scales, const void* lengths, int64_t B,
+                 int64_t H, int64_t D, int dtype, int fmt, int64_t sink, int64_t window) {
+  if (dtype != SBFA_F16 && dtype != SBFA_BF16)
+    return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: dtype must be float16 or bfloat16");
+  if (fmt != SBFA_Q_E4M3 && fmt != SBFA_Q_INT8)
+    return fail(SBFA_ERR_INVALID, "8-bit cache: unknown format code");
+  if (B <= 0 || H <= 0) return fail(SBFA_ERR_INVALID, "B and H must be positive");
+  if (B > 65535) return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: at most 65535 sequences");
+  if (padded_dim(D) == 0)
+    return fail(SBFA_ERR_UNSUPPORTED,
+                "8-bit cache: head_dim must be a multiple of 8 and at most 256");
+  if (sink < 0 || window < 0)
+    return fail(SBFA_ERR_INVALID, "sink_size and window_size must be non-negative");
+  if (sink + window <= 0 || sink + window >= (1ll << 30))
+    return fail(SBFA_ERR_INVALID, "sink_size + window_size must be in [1, 2^30)");
+  if (!k || !v || !scales || !lengths)
+    return fail(SBFA_ERR_INVALID, "8-bit cache: NULL cache pointer");
+  if (((uintptr_t)k | (uintptr_t)v) & 15u)
+    return fail(SBFA_ERR_INVALID, "8-bit cache: tensors must be 16-byte aligned");
+  return SBFA_OK;
+}
+
+QCache make_cache(void* k, void* v, void* scales, int64_t H, int64_t D, int64_t sink,
+                  int64_t window) {
+  return QCache{(uint8_t*)k, (uint8_t*)v, (uint16_t*)scales, H, sink + window, sink, window,
+                (int)D};
+}
+
+template <typename F>
+int by_format(int dtype, int fmt, int64_t D, F&& f) {
+  // f(type tag, format, padded dim) with the last two as integral constants
+  auto dims = [&](auto t, auto m) {
+    switch (padded_dim(D)) {
+      case 64: return f(t, m, std::integral_constant<int, 64>{});
+      case 128: return f(t, m, std::integral_constant<int, 128>{});
+      default: return f(t, m, std::integral_constant<int, 256>{});
+    }
+  };
+  auto fmts = [&](auto t) {
+    return fmt == SBFA_Q_E4M3 ? dims(t, std::integral_constant<int, SBFA_Q_E4M3>{})
+                              : dims(t, std::integral_constant<int, SBFA_Q_INT8>{});
+  };
+  return dtype == SBFA_BF16 ? fmts(__nv_bfloat16{}) : fmts(__half{});
+}
+
+// CTAs per unit of the attend kernel (a cluster, so a power of two up to 8).
+// More of them shorten a unit, which pays while there are SMs to fill.
+int attend_splits(int64_t units, int64_t rows, int slots) {
+  int ns = 1;
+  while (ns < 8 && units * ns * 2 <= slots && rows > (int64_t)ns * 128) ns *= 2;
+  return ns;
+}
+
+template <typename T, int FMT, int DP, int NQ>
+int launch_attend(const void* q, const QCache& c, const int64_t* lengths, void* o, float* o32,
+                  float* lse, int64_t B, int group, float scale, cudaStream_t s) {
+  using C = AttCfg<DP, NQ>;
+  const int chunks = (group + C::kRowsQ - 1) / C::kRowsQ;
+  const int64_t units = B * c.heads * chunks;
+  const int ns = attend_splits(units, c.rows, device_sm_count() * C::kCtas);
+  if (units * ns >= (1ll << 31))
+    return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many (sequence, head) units");
+  auto kern = qcache_attend_kernel<T, FMT, DP, NQ>;
+  if (C::kBytes > 48 * 1024)
+    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)C::kBytes),
+                            "cudaFuncSetAttribute(qcache_attend)"))
+      return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * ns));
+  cfg.blockDim = dim3(kAttWarps * 32);
+  cfg.dynamicSmemBytes = C::kBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)ns;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  LaunchScope ls("qcache_attend_kernel", s);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, (const T*)q, c, lengths, (T*)o, o32, lse,
+                                       scale * kLog2e, group, chunks, ns),
+                    "qcache_attend_kernel");
+}
+
+}  // namespace
+}  // namespace sbfa
+
+using namespace sbfa;
+
+extern "C" int64_t sbfa_qcache_row_bytes(int64_t head_dim) { return padded_dim(head_dim); }
+
+extern "C" int sbfa_qcache_append(void* k_codes, void* v_codes, void* scales, int64_t* lengths,
+                                  int32_t* tickets, const void* k_new, const void* v_new,
+                                  const int64_t* strides, const int64_t* counts, int64_t B,
+                                  int64_t H, int64_t head_dim, int dtype, int fmt, int64_t sink,
+                                  int64_t window, int64_t n_new, void* stream) {
+  if (int rc = check_qcache(k_codes, v_codes, scales, lengths, B, H, head_dim, dtype, fmt, sink,
+                            window))
+    return rc;
+  if (n_new < 0 || n_new >= (1ll << 31))
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_append: n_new must be in [0, 2^31)");
+  if (n_new == 0) return SBFA_OK;
+  if (!k_new || !v_new || !tickets)
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_append: NULL tensor pointer");
+  Strides3 st[2];
+  for (int i = 0; i < 2; ++i) {
+    st[i] = strides ? Strides3{strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}
+                    : Strides3{H * n_new * head_dim, n_new * head_dim, head_dim};
+    if (st[i].b < 0 || st[i].h < 0 || st[i].n < 0 || st[i].b % 8 || st[i].h % 8 || st[i].n % 8)
+      return fail(SBFA_ERR_INVALID, "sbfa_qcache_append: strides must be non-negative multiples "
+                                    "of 8 elements");
+  }
+  if (((uintptr_t)k_new | (uintptr_t)v_new) & 15u)
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_append: tensors must be 16-byte aligned");
+  const QCache c = make_cache(k_codes, v_codes, scales, H, head_dim, sink, window);
+  cudaStream_t s = (cudaStream_t)stream;
+  return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
+    using T = decltype(t);
+    constexpr int G = dp.value / 8;
+    const int64_t per = (int64_t)(kAppThreads / G) * kAppUnroll;
+    const dim3 grid((unsigned)std::min<int64_t>((n_new * H + per - 1) / per, 4096), (unsigned)B);
+    LaunchScope ls("qcache_append_kernel", s);
+    qcache_append_kernel<T, m.value, G><<<grid, kAppThreads, 0, s>>>(
+        c, lengths, tickets, (const T*)k_new, (const T*)v_new, st[0], st[1], counts, n_new);
+    return check_launch("qcache_append_kernel");
+  });
+}
+
+extern "C" int sbfa_qcache_read(const void* k_codes, const void* v_codes, const void* scales,
+                                const int64_t* lengths, void* k_out, void* v_out,
+                                int64_t* positions, int64_t B, int64_t H, int64_t head_dim,
+                                int dtype, int fmt, int64_t sink, int64_t window, void* stream) {
+  if (int rc = check_qcache(k_codes, v_codes, scales, lengths, B, H, head_dim, dtype, fmt, sink,
+                            window))
+    return rc;
+  if (!k_out || !v_out || !positions)
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_read: NULL tensor pointer");
+  if (((uintptr_t)k_out | (uintptr_t)v_out) & 15u)
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_read: tensors must be 16-byte aligned");
+  const QCache c = make_cache(const_cast<void*>(k_codes), const_cast<void*>(v_codes),
+                              const_cast<void*>(scales), H, head_dim, sink, window);
+  cudaStream_t s = (cudaStream_t)stream;
+  return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
+    using T = decltype(t);
+    constexpr int G = dp.value / 8;
+    const int64_t per = (int64_t)(kReadThreads / G) * kReadUnroll;
+    const dim3 grid((unsigned)std::min<int64_t>((c.rows * H + per - 1) / per, 65535),
+                    (unsigned)B);
+    LaunchScope ls("qcache_read_kernel", s);
+    qcache_read_kernel<T, m.value, G>
+        <<<grid, kReadThreads, 0, s>>>(c, lengths, (T*)k_out, (T*)v_out, positions);
+    return check_launch("qcache_read_kernel");
+  });
+}
+
+extern "C" int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
+                                  const void* scales, const int64_t* lengths, void* o,
+                                  float* o_partial, float* lse, int64_t B, int64_t H,
+                                  int64_t kv_heads, int64_t head_dim, int dtype, int fmt,
+                                  double softmax_scale, int64_t sink, int64_t window,
+                                  void* stream) {
+  if (kv_heads <= 0) kv_heads = H;
+  if (int rc = check_qcache(k_codes, v_codes, scales, lengths, B, kv_heads, head_dim, dtype, fmt,
+                            sink, window))
+    return rc;
+  if (H <= 0 || H % kv_heads != 0)
+    return fail(SBFA_ERR_INVALID, "the query head count must be a multiple of kv_heads");
+  if (!(softmax_scale > 0) || softmax_scale > 1e30)
+    return fail(SBFA_ERR_INVALID, "softmax_scale must be positive and finite");
+  if (!q || (!o && !o_partial) || (o_partial && !lse))
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_attend: NULL tensor pointer");
+  if (((uintptr_t)q | (uintptr_t)o | (uintptr_t)o_partial) & 15u)
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_attend: tensors must be 16-byte aligned");
+  const QCache c = make_cache(const_cast<void*>(k_codes), const_cast<void*>(v_codes),
+                              const_cast<void*>(scales), kv_heads, head_dim, sink, window);
+  cudaStream_t s = (cudaStream_t)stream;
+  const int64_t group = H / kv_heads;
+  if (group >= (1 << 20)) return fail(SBFA_ERR_UNSUPPORTED, "too many query heads");
+  return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
+    using T = decltype(t);
+    constexpr int DP = dp.value;
+    // 16 query columns halve the passes over a group of more than 8; at 256
+    // columns per row the second set of accumulators would not fit the registers
+    if constexpr (DP <= 128) {
+      if (group > 8)
+        return launch_attend<T, m.value, DP, 2>(q, c, lengths, o, o_partial, lse, B, (int)group,
+                                                (float)softmax_scale, s);
+    }
+    return launch_attend<T, m.value, DP, 1>(q, c, lengths, o, o_partial, lse, B, (int)group,
+                                            (float)softmax_scale, s);
+  });
+}

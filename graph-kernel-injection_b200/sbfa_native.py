@@ -10,6 +10,7 @@ There is no fallback: if the library is missing, :func:`lib` raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -21,6 +22,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsbfa.so")
 
 F16, BF16, F32, F64 = 0, 1, 2, 3
+Q_E4M3, Q_INT8 = 0, 1
 _DTYPE_CODE = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.float64: F64}
 
 _lib: Optional[ctypes.CDLL] = None
@@ -60,6 +62,16 @@ _SIGNATURES = {
                           _i64, _vp, _i64, _vp], _i32),
     "sbfa_ring_decode_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64], _i64),
     "sbfa_decode_supported": ([_i32, _i64], _i32),
+    "sbfa_qcache_row_bytes": ([_i64], _i64),
+    "sbfa_qcache_append": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32,
+                            _i32, _i64, _i64, _i64, _vp], _i32),
+    "sbfa_qcache_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32,
+                            _i32, _f64, _i64, _i64, _vp], _i32),
+    "sbfa_qcache_read": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i64,
+                          _i64, _vp], _i32),
+    "sbfa_prefix_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64,
+                            _i64, _i64, _i32, _f64, _vp, _i64, _vp], _i32),
+    "sbfa_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "sbfa_decode_noalloc": ([_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _f64, _i32,
                              _i64, _i64, _vp, _i64, _i64, _vp], _i32),
 }
@@ -109,6 +121,14 @@ def dtype_code(dt: torch.dtype) -> int:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def device_guard(device: torch.device):
+    """Makes ``device`` current for a launch; free when it already is."""
+    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

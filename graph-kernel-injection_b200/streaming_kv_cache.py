@@ -1,4 +1,6 @@
-"""StreamingLLM ring-buffer KV cache for the decode step.
+"""StreamingLLM ring-buffer KV caches for the decode step: :class:`StreamingKVCache`
+(16 or 32 bits, one length for the whole batch) and :class:`QuantizedStreamingKVCache`
+(8 bits, ragged batches, grouped key/value heads).
 
 No upstream counterpart: upstream decodes through its prefill kernel with
 ``N_Q = 1`` over the whole cache (``benchmark.py:799-804``), although the
@@ -9,16 +11,21 @@ StreamingLLM rule lets the query at position ``p`` see only positions
 Decoding over it gives the same attention as the block-sparse decode over a
 full-length cache (``block_sparse_attention`` with ``N_Q == 1``, causal,
 ``block_m = 1``), with ``(sink + window) / n_kv`` of the memory.
+
+Either cache's ``attend`` takes a :class:`shared_prefix.SharedPrefix`, tokens that
+every sequence of the batch has before its own and that are held once.
 """
 
 from __future__ import annotations
 
+import ctypes
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 import sbfa_native as native
+from shared_prefix import OWN_16, OWN_32, SharedPrefix, no_gradients, vector_readable
 
 
 class StreamingKVCache:
@@ -75,10 +82,11 @@ class StreamingKVCache:
         self.length += n
 
     def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
-               return_lse: bool = False):
+               return_lse: bool = False, prefix: Optional[SharedPrefix] = None):
         """Attention of the query at position ``length - 1`` ([B, H, 1, D])
         over the cached sink and window; returns O ([B, H, 1, D]) and, with
-        ``return_lse``, the natural-log LSE ([B, H, 1] fp32)."""
+        ``return_lse``, the natural-log LSE ([B, H, 1] fp32).  With ``prefix``
+        the query sees that shared prefix as well (float16 / bfloat16)."""
         if self.length == 0:
             raise RuntimeError("the cache is empty: append the query's own token first")
         q = self._check(q, 1, "q")
@@ -91,4 +99,176 @@ class StreamingKVCache:
                 self.batch, self.heads, self.head_dim, native.dtype_code(self.dtype), scale,
                 self.sink_size, self.window_size, self.length, self._ws.data_ptr(),
                 self._ws.numel(), native.stream_ptr(self.device)), "ring_decode")
+        if prefix is not None:
+            # o is rounded to its 16 bits before the merge rounds once more
+            o, lse = prefix.join(q, scale, o, lse, OWN_16)
         return (o, lse) if return_lse else o
+
+
+_FORMATS = {"e4m3": (native.Q_E4M3, torch.float8_e4m3fn), "int8": (native.Q_INT8, torch.int8)}
+
+
+class QuantizedStreamingKVCache:
+    """Per-layer 8-bit K/V ring cache of ``sink_size + window_size`` rows per
+    (sequence, head) on one CUDA device.
+
+    Rows are quantised as they are appended: 8-bit codes (``fmt`` ``"e4m3"`` or
+    ``"int8"``) and one power-of-two scale per row, the smallest that holds the
+    row's largest magnitude, so the scaling itself is exact.  Every sequence has its
+    own length, kept on the device in ``lengths`` (int64 [B]): batches may be
+    ragged, and ``append`` / ``attend`` can be captured in a CUDA graph whose
+    replays advance.  ``heads`` counts key/value heads; queries may have any
+    multiple of it.  ``dtype`` (float16 or bfloat16) is the type of new rows, queries
+    and outputs; ``head_dim`` is a multiple of 8, at most 256.
+
+    ``k``, ``v`` (codes [B, H, rows, D]), ``scales`` (uint8 [B, H, rows, 2]: ``e + 127``
+    of K's and of V's ``2 ** e``; 255 marks a row with a NaN or an infinity, which
+    reads as NaN) and ``lengths`` are the state: save them, and hand them to :meth:`load`.
+    No gradients.  Calls on one cache follow each other on one stream.
+    """
+
+    def __init__(self, batch: int, heads: int, head_dim: int, sink_size: int, window_size: int,
+                 dtype: torch.dtype = torch.bfloat16, fmt: str = "e4m3",
+                 device: str | torch.device = "cuda") -> None:
+        if min(batch, heads, head_dim) <= 0:
+            raise ValueError("batch, heads and head_dim must be positive")
+        if sink_size < 0 or window_size < 0 or sink_size + window_size <= 0:
+            raise ValueError("sink_size and window_size must be non-negative, not both zero")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype must be float16 or bfloat16, got {dtype}")
+        if fmt not in _FORMATS:
+            raise ValueError(f"fmt must be one of {sorted(_FORMATS)}, got {fmt!r}")
+        row_bytes = int(native.lib().sbfa_qcache_row_bytes(head_dim))
+        if row_bytes == 0:
+            raise ValueError(f"head_dim must be a multiple of 8 and at most 256, got {head_dim}")
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError("the cache must live on a CUDA device")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.batch, self.heads, self.head_dim = batch, heads, head_dim
+        self.sink_size, self.window_size = sink_size, window_size
+        self.dtype, self.fmt, self.device = dtype, fmt, dev
+        rows = sink_size + window_size
+        code, code_dtype = _FORMATS[fmt]
+        self._k = torch.zeros(batch, heads, rows, row_bytes, dtype=torch.uint8, device=dev)
+        self._v = torch.zeros_like(self._k)
+        self.k = self._k[..., :head_dim].view(code_dtype)
+        self.v = self._v[..., :head_dim].view(code_dtype)
+        self.scales = torch.zeros(batch, heads, rows, 2, dtype=torch.uint8, device=dev)
+        self.lengths = torch.zeros(batch, dtype=torch.int64, device=dev)
+        self._tickets = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self._codes = (native.dtype_code(dtype), code)
+        self._cache_ptrs = (self._k.data_ptr(), self._v.data_ptr(), self.scales.data_ptr(),
+                            self.lengths.data_ptr())
+
+    @property
+    def memory_bytes(self) -> int:
+        return 2 * self._k.numel() + self.scales.numel()
+
+    def _check(self, t: torch.Tensor, shape: Tuple[int, ...], name: str) -> None:
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+        if t.device != self.device or t.dtype != self.dtype:
+            raise ValueError(f"{name} must be {self.dtype} on {self.device}")
+        no_gradients(t)
+
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor,
+               counts: Optional[torch.Tensor] = None) -> None:
+        """Quantise and append the next ``t`` tokens of every sequence ([B, H, t, D],
+        views welcome).  ``counts`` (int64 [B] on the device, clamped to [0, t]) says how many
+        of them each sequence takes: the rest of a right-padded batch is not read."""
+        if k_new.dim() != 4:
+            raise ValueError(f"k_new must be [B, H, t, D], got {tuple(k_new.shape)}")
+        n = k_new.shape[2]
+        shape = (self.batch, self.heads, n, self.head_dim)
+        self._check(k_new, shape, "k_new")
+        self._check(v_new, shape, "v_new")
+        if counts is not None:
+            if (tuple(counts.shape) != (self.batch,) or counts.device != self.device
+                    or counts.dtype not in (torch.int64, torch.int32)):
+                raise ValueError(f"counts must be int64 [{self.batch}] on {self.device}")
+            counts = counts.to(torch.int64).contiguous()
+        if n == 0:
+            return
+        k_new, v_new = vector_readable(k_new), vector_readable(v_new)
+        strides = (ctypes.c_int64 * 6)(*k_new.stride()[:3], *v_new.stride()[:3])
+        k, v, scales, lengths = self._cache_ptrs
+        with native.device_guard(self.device):
+            native.check(native.lib().sbfa_qcache_append(
+                k, v, scales, lengths, self._tickets.data_ptr(), k_new.data_ptr(),
+                v_new.data_ptr(), strides, native.ptr(counts), self.batch, self.heads,
+                self.head_dim, *self._codes, self.sink_size, self.window_size, n,
+                native.stream_ptr(self.device)), "qcache_append")
+
+    def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
+               return_lse: bool = False, prefix: Optional[SharedPrefix] = None):
+        """Attention of each sequence's query at its last position ([B, Hq, 1, D], Hq a
+        multiple of ``heads``) over its cached rows; returns O ([B, Hq, 1, D]) and, with
+        ``return_lse``, the natural-log LSE ([B, Hq, 1] fp32).  A sequence that has no
+        token yet gives zeros.  With ``prefix`` every query sees that shared prefix as
+        well: the merged result is rounded once."""
+        if q.dim() != 4 or q.shape[1] == 0 or q.shape[1] % self.heads:
+            raise ValueError(f"q must be [B, Hq, 1, D] with Hq a multiple of {self.heads}, got "
+                             f"{tuple(q.shape)}")
+        hq = q.shape[1]
+        self._check(q, (self.batch, hq, 1, self.head_dim), "q")
+        scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+        o = torch.empty_like(q, dtype=torch.float32 if prefix is not None else None)
+        lse = None
+        if return_lse or prefix is not None:
+            lse = torch.empty(self.batch, hq, 1, dtype=torch.float32, device=self.device)
+        out, partial = (o.data_ptr(), None) if prefix is None else (None, o.data_ptr())
+        with native.device_guard(self.device):
+            native.check(native.lib().sbfa_qcache_attend(
+                q.data_ptr(), *self._cache_ptrs, out, partial, native.ptr(lse), self.batch, hq,
+                self.heads, self.head_dim, *self._codes, scale, self.sink_size,
+                self.window_size, native.stream_ptr(self.device)), "qcache_attend")
+        if prefix is not None:
+            o, lse = prefix.join(q, scale, o, lse, OWN_32)
+        return (o, lse) if return_lse else o
+
+    def read(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The kept rows as ``dtype`` values in order of position: K and V
+        ([B, H, rows, D], row i = the sequence's i-th kept position, zeros behind the
+        last) and those positions (int64 [B, rows], -1 behind the last)."""
+        rows = self.sink_size + self.window_size
+        k = torch.empty(self.batch, self.heads, rows, self.head_dim, dtype=self.dtype,
+                        device=self.device)
+        v = torch.empty_like(k)
+        positions = torch.empty(self.batch, rows, dtype=torch.int64, device=self.device)
+        with native.device_guard(self.device):
+            native.check(native.lib().sbfa_qcache_read(
+                *self._cache_ptrs, k.data_ptr(), v.data_ptr(), positions.data_ptr(), self.batch,
+                self.heads, self.head_dim, *self._codes, self.sink_size, self.window_size,
+                native.stream_ptr(self.device)), "qcache_read")
+        return k, v, positions
+
+    def load(self, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor,
+             lengths: torch.Tensor) -> None:
+        """Take over a saved state (the tensors ``k``, ``v``, ``scales``, ``lengths`` of a cache
+        of the same geometry and format).  Waits for the device to check the lengths."""
+        for t, mine, name in ((k, self.k, "k"), (v, self.v, "v"), (scales, self.scales, "scales"),
+                              (lengths, self.lengths, "lengths")):
+            if t.shape != mine.shape:
+                raise ValueError(f"{name} must have shape {tuple(mine.shape)}, got "
+                                 f"{tuple(t.shape)}")
+            if t.element_size() != mine.element_size() or (name in ("scales", "lengths")
+                                                           and t.dtype != mine.dtype):
+                raise ValueError(f"{name} must hold {mine.dtype}, got {t.dtype}")
+        if bool((lengths < 0).any()):
+            raise ValueError("lengths must not be negative")
+        self._k[..., :self.head_dim].copy_(k.view(torch.uint8))
+        self._v[..., :self.head_dim].copy_(v.view(torch.uint8))
+        self.scales.copy_(scales)
+        self.lengths.copy_(lengths)
+
+    def reset(self, sequences=None) -> None:
+        """Forget every sequence, or those that ``sequences`` (indices or a bool mask) names."""
+        if sequences is None:
+            self.lengths.zero_()
+        else:
+            self.lengths[sequences] = 0

@@ -49,6 +49,9 @@ enum sbfa_status {
 
 enum sbfa_dtype { SBFA_F16 = 0, SBFA_BF16 = 1, SBFA_F32 = 2, SBFA_F64 = 3 };
 
+/* Code types of the 8-bit ring cache. */
+enum sbfa_qformat { SBFA_Q_E4M3 = 0, SBFA_Q_INT8 = 1 };
+
 /* ABI version of this header (bumped on any signature change). */
 int sbfa_abi_version(void);
 
@@ -284,6 +287,96 @@ int sbfa_ring_decode(const void* q, const void* k_cache, const void* v_cache, vo
 /* Scratch bytes sbfa_ring_decode needs for this cache geometry (any seq_len). */
 int64_t sbfa_ring_decode_workspace_bytes(int64_t B, int64_t H, int64_t head_dim, int64_t sink,
                                          int64_t window);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit StreamingLLM ring cache (no upstream counterpart).  The ring of
+ * sbfa_ring_append with (a) rows quantised as they are written, (b) one
+ * length per sequence, on the device, so a batch may be ragged and a captured
+ * step moves on when it is replayed, and (c) kv_heads key/value heads shared by
+ * groups of query heads.
+ *
+ * Cache tensors, all contiguous, 16-byte aligned, owned by the caller:
+ *   k_codes, v_codes: 8-bit [B, kv_heads, sink + window, DP],
+ *     DP = sbfa_qcache_row_bytes(head_dim); the columns behind head_dim hold 0;
+ *   scales: uint8 [B, kv_heads, sink + window, 2], K's byte and V's;
+ *   lengths: int64 [B], tokens appended to each sequence;
+ *   tickets: int32 [B], zero before the first append and after each one.
+ * A row x is stored with e = the least integer >= -126 such that
+ * max|x| <= top * 2^e (top: 448 for SBFA_Q_E4M3, 127 for SBFA_Q_INT8; e = 0 for a
+ * row of zeros) as the byte e + 127 and the codes of x * 2^-e rounded to
+ * nearest, ties to even.  A row that holds a NaN or an infinity is stored as
+ * byte 255 and reads as NaN throughout.  Values that a code rounds up past the 16-bit
+ * type's largest saturate when they are read or attended to.
+ * dtype (of new rows, queries and outputs): SBFA_F16 or SBFA_BF16; head_dim a
+ * multiple of 8, at most 256.  Visible rows of a sequence: [0, min(length,
+ * sink + window)).
+ * ------------------------------------------------------------------------- */
+
+/* DP for this head_dim (64, 128 or 256), 0 when it is not supported. */
+int64_t sbfa_qcache_row_bytes(int64_t head_dim);
+
+/* Quantises the next tokens of every sequence into their ring rows and adds
+ * their number to lengths.  k_new, v_new: logical [B, kv_heads, n_new, head_dim];
+ * strides: (batch, head, row) element strides of k_new then v_new, non-negative
+ * multiples of 8, or NULL for contiguous tensors.  counts: int64[B] on the
+ * device, how many of the n_new tokens each sequence takes (clamped to [0,
+ * n_new]), or NULL for all; rows behind a count are not read.  Two appends to one cache
+ * must not run at the same time. */
+int sbfa_qcache_append(void* k_codes, void* v_codes, void* scales, int64_t* lengths,
+                       int32_t* tickets, const void* k_new, const void* v_new,
+                       const int64_t* strides, const int64_t* counts, int64_t B,
+                       int64_t kv_heads, int64_t head_dim, int dtype, int fmt, int64_t sink,
+                       int64_t window, int64_t n_new, void* stream);
+
+/* Attention of each sequence's query at its last position over its visible
+ * rows.  q: contiguous [B, H, head_dim], H a multiple of kv_heads (<= 0 means H);
+ * o: the same shape and dtype; lse (may be NULL): fp32 [B, H].  A sequence of
+ * length 0 gives O = 0 and LSE = 0.  With o_partial (fp32 [B, H, head_dim]) the
+ * result goes there unrounded instead of to o, and lse is -inf for an empty
+ * sequence: the form sbfa_prefix_attend merges.  softmax_scale > 0.  No workspace. */
+int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
+                       const void* scales, const int64_t* lengths, void* o, float* o_partial,
+                       float* lse, int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim,
+                       int dtype, int fmt, double softmax_scale, int64_t sink, int64_t window,
+                       void* stream);
+
+/* The kept rows as 16-bit values in order of position: out row i of a sequence
+ * is its i-th kept position (sinks, then the window from its oldest), positions[b, i] that
+ * position; rows behind the last are zero with position -1.  k_out, v_out:
+ * contiguous [B, kv_heads, sink + window, head_dim]; positions: int64 [B, sink + window]. */
+int sbfa_qcache_read(const void* k_codes, const void* v_codes, const void* scales,
+                     const int64_t* lengths, void* k_out, void* v_out, int64_t* positions,
+                     int64_t B, int64_t kv_heads, int64_t head_dim, int dtype, int fmt,
+                     int64_t sink, int64_t window, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention of a batch to a prefix that all its sequences share (no upstream
+ * counterpart).  Every query of every sequence sees all P prefix tokens, so the
+ * rows of the whole batch and of a group's query heads make one matrix per
+ * key/value head, and K and V of the prefix are read once for all of them.
+ * ------------------------------------------------------------------------- */
+
+/* q: logical [B, H, n_q, head_dim] (q_strides: batch, head, row, or NULL);
+ * k_prefix, v_prefix: contiguous [kv_heads, P, head_dim], fp16 or bf16 like q;
+ * head_dim a multiple of 8, at most 128; all 16-byte aligned, strides
+ * multiples of 8 elements; softmax_scale > 0.
+ * own: each query's attention over its sequence's own tokens, merged with the
+ * prefix's by their log-sum-exps: own_o contiguous [B, H, n_q, head_dim] and
+ * own_lse fp32 [B, H, n_q].  own_kind 0: none; 1: own_o has q's dtype and every
+ * row saw a key (sbfa_ring_decode, or sbfa_fwd with a causal window >= 1); 2:
+ * own_o is fp32 and own_lse = -inf marks a row that saw none (sbfa_qcache_attend's partial
+ * form).
+ * o: contiguous [B, H, n_q, head_dim]; lse: fp32 [B, H, n_q] or NULL.  ws:
+ * 16-byte aligned caller scratch of sbfa_prefix_workspace_bytes() bytes. */
+int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const void* k_prefix,
+                       const void* v_prefix, const void* own_o, const float* own_lse,
+                       int own_kind, void* o, float* lse, int64_t B, int64_t H,
+                       int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim, int dtype,
+                       double softmax_scale, void* ws, int64_t ws_bytes, void* stream);
+
+/* Scratch bytes sbfa_prefix_attend needs for this shape, 0 for a bad one. */
+int64_t sbfa_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q,
+                                    int64_t P, int64_t head_dim);
 
 /* sbfa_decode without any device allocation by anyone.  No counterpart in
  * the upstream project, which has no decode entry point at all.

@@ -1,0 +1,110 @@
+"""Refusals of the 8-bit ring cache and the shared prefix that need no GPU: the C entry points'
+argument checks (nothing is launched) and the Python classes' own."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import sbfa_native as native
+
+INVALID, UNSUPPORTED = 1, 2
+P = 4096   # a non-null, 16-byte aligned address that is never read
+
+
+def append(L, B=1, H=1, D=64, dtype=native.BF16, fmt=0, sink=4, window=8, n=1, k=P, new=P,
+           strides=None, tickets=P):
+    st = None if strides is None else (ctypes.c_int64 * 6)(*strides)
+    return L.sbfa_qcache_append(k, P, P, P, tickets, new, P, st, None, B, H, D, dtype, fmt, sink,
+                                window, n, None)
+
+
+@pytest.mark.parametrize("kw,rc,word", [
+    (dict(dtype=native.F32), UNSUPPORTED, "float16"), (dict(fmt=2), INVALID, "format"),
+    (dict(B=0), INVALID, "positive"), (dict(H=0), INVALID, "positive"),
+    (dict(B=65536), UNSUPPORTED, "65535"), (dict(D=0), UNSUPPORTED, "head_dim"),
+    (dict(D=60), UNSUPPORTED, "head_dim"), (dict(D=264), UNSUPPORTED, "head_dim"),
+    (dict(sink=-1), INVALID, "non-negative"), (dict(sink=0, window=0), INVALID, "2^30"),
+    (dict(window=1 << 30), INVALID, "2^30"), (dict(k=None), INVALID, "NULL"),
+    (dict(k=P + 8), INVALID, "aligned"), (dict(n=-1), INVALID, "n_new"),
+    (dict(new=None), INVALID, "NULL"), (dict(new=P + 2), INVALID, "aligned"),
+    (dict(tickets=None), INVALID, "NULL"),
+    (dict(strides=(64, 64, 60, 64, 64, 64)), INVALID, "strides"),
+    (dict(strides=(64, 64, 64, -64, 64, 64)), INVALID, "strides"),
+])
+def test_append_refuses(kw, rc, word):
+    assert append(native.lib(), **kw) == rc and word in native.last_error()
+
+
+def test_append_of_nothing_launches_nothing():
+    before = native.launch_count()
+    assert append(native.lib(), n=0, new=None) == 0 and native.launch_count() == before
+
+
+def attend(L, q=P, o=P, partial=None, lse=P, B=1, H=4, hkv=2, D=64, scale=0.1, fmt=1):
+    return L.sbfa_qcache_attend(q, P, P, P, P, o, partial, lse, B, H, hkv, D, native.F16, fmt,
+                                scale, 4, 8, None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(H=3), "multiple"), (dict(H=0), "multiple"), (dict(scale=0.0), "softmax_scale"),
+    (dict(scale=-1.0), "softmax_scale"), (dict(scale=float("nan")), "softmax_scale"),
+    (dict(scale=float("inf")), "softmax_scale"), (dict(q=None), "NULL"), (dict(o=None), "NULL"),
+    (dict(o=None, partial=P, lse=None), "NULL"), (dict(q=P + 8), "aligned"),
+    (dict(o=P + 4), "aligned"),
+])
+def test_attend_refuses(kw, word):
+    assert attend(native.lib(), **kw) == INVALID and word in native.last_error()
+
+
+def prefix(L, q=P, k=P, own=None, own_lse=None, kind=0, B=2, H=4, hkv=2, n=1, length=100, D=64,
+           dtype=native.F16, scale=0.1, ws=P, ws_bytes=1 << 40, strides=None):
+    st = None if strides is None else (ctypes.c_int64 * 3)(*strides)
+    return L.sbfa_prefix_attend(q, st, k, P, own, own_lse, kind, P, P, B, H, hkv, n, length, D,
+                                dtype, scale, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,rc,word", [
+    (dict(dtype=native.F32), UNSUPPORTED, "float16"), (dict(D=136), UNSUPPORTED, "head_dim"),
+    (dict(D=12), UNSUPPORTED, "head_dim"), (dict(H=3), INVALID, "multiple"),
+    (dict(length=0), INVALID, "positive"), (dict(n=0), INVALID, "positive"),
+    (dict(length=1 << 31), INVALID, "positive"), (dict(scale=0.0), INVALID, "softmax_scale"),
+    (dict(q=None), INVALID, "NULL"), (dict(kind=1), INVALID, "own"),
+    (dict(kind=3), INVALID, "own"), (dict(kind=2, own=P), INVALID, "own"),
+    (dict(k=P + 8), INVALID, "aligned"), (dict(ws=None), INVALID, "workspace"),
+    (dict(ws_bytes=16), INVALID, "workspace"), (dict(strides=(64, 64, 4)), INVALID, "strides"),
+    (dict(strides=(64, -8, 8)), INVALID, "strides"),
+])
+def test_prefix_refuses(kw, rc, word):
+    assert prefix(native.lib(), **kw) == rc and word in native.last_error()
+
+
+def test_sizes():
+    L = native.lib()
+    assert [L.sbfa_qcache_row_bytes(d) for d in (0, 8, 64, 72, 128, 136, 256, 264, 60)] == \
+        [0, 64, 64, 128, 128, 256, 256, 0, 0]
+    assert L.sbfa_prefix_workspace_bytes(2, 4, 2, 1, 100, 64) >= 2 * 4 * (64 * 4 + 8)
+    for bad in ((0, 4, 2, 1, 100, 64), (2, 4, 3, 1, 100, 64), (2, 4, 2, 1, 0, 64),
+                (2, 4, 2, 1, 100, 256)):
+        assert L.sbfa_prefix_workspace_bytes(*bad) == 0
+
+
+def test_python_refusals():
+    from shared_prefix import SharedPrefix
+    from streaming_kv_cache import QuantizedStreamingKVCache as Cache
+    for args, kw in (((0, 1, 64, 4, 8), {}), ((1, 1, 64, -1, 8), {}), ((1, 1, 64, 0, 0), {}),
+                     ((1, 1, 60, 4, 8), {}), ((1, 1, 512, 4, 8), {}),
+                     ((1, 1, 64, 4, 8), dict(dtype=torch.float32)),
+                     ((1, 1, 64, 4, 8), dict(fmt="e5m2")),
+                     ((1, 1, 64, 4, 8), dict(device="cpu"))):
+        with pytest.raises(ValueError):
+            Cache(*args, **kw)
+    k = torch.zeros(2, 10, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        SharedPrefix(k, k)
+    with pytest.raises(ValueError, match="empty"):
+        SharedPrefix(k[:, :0], k[:, :0])
+    with pytest.raises(ValueError, match="H_kv"):
+        SharedPrefix(k[0], k[0])
