@@ -115,12 +115,14 @@ __device__ __forceinline__ float saturated(float x) {
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
-// A group of DP / 8 lanes takes one (head, token): 16 bytes of K and of V per
-// lane, the row maxima by shuffles, 8 code bytes back.  Bound by HBM: 4 D bytes
-// in, 2 D + 2 out per head and token.  The tokens of a head are adjacent, so
-// that their scale pairs fill whole sectors.  The last CTA of a sequence moves
-// its length on (a ticket per sequence, left at zero), which saves the launch of
-// a second kernel at the end of every decode step.
+// A group of G = DP / 8 lanes takes one (head, token): 16 bytes of K and of V per
+// lane, the row maxima by shuffles, 8 code bytes back.  Bound by HBM: 4 D bytes in,
+// 2 D + 2 out per head and token.  A CTA covers 2^hs heads x kRows / 2^hs tokens at a
+// time (tokens adjacent, so that their scale pairs share sectors; several heads only
+// where a call has few tokens) and walks the tokens that survive the call: positions
+// that a later token of it overwrites are never visited.  The last CTA of a sequence moves its
+// length on (a ticket per sequence, left at zero), which saves a second launch in every
+// decode step.
 constexpr int kAppThreads = 256;
 constexpr int kAppUnroll = 2;
 
@@ -128,35 +130,43 @@ template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(kAppThreads)
     qcache_append_kernel(QCache c, int64_t* __restrict__ lengths, int32_t* __restrict__ tickets,
                          const T* __restrict__ kn, const T* __restrict__ vn, Strides3 sk,
-                         Strides3 sv, const int64_t* __restrict__ counts, int64_t n_new) {
+                         Strides3 sv, const int64_t* __restrict__ counts, int n_new,
+                         int head_blocks, int hs) {
   constexpr int DP = G * 8;
   constexpr int kRows = kAppThreads / G;
   const int b = blockIdx.y;
-  const int lane = threadIdx.x % G;
+  const int lane = threadIdx.x % G, slot = threadIdx.x / G;
+  const int tp = kRows >> hs;                                // tokens a CTA covers at a time
+  const int head = ((int)blockIdx.x % head_blocks << hs) + slot / tp;
+  const int chunk = (int)blockIdx.x / head_blocks, chunks = (int)gridDim.x / head_blocks;
   const int64_t len = max(lengths[b], (int64_t)0);
-  const int64_t cnt = counts ? min(max(counts[b], (int64_t)0), n_new) : n_new;
-  const int64_t end = len + cnt;
-  const int64_t items = n_new * c.heads;
-  const bool on = lane * 8 < c.d;
-  for (int64_t i0 = (int64_t)blockIdx.x * kRows * kAppUnroll; i0 < items;
-       i0 += (int64_t)gridDim.x * kRows * kAppUnroll) {
+  const int cnt = counts ? (int)min(max(counts[b], (int64_t)0), (int64_t)n_new) : n_new;
+  const int sink = (int)c.sink, window = (int)c.window;
+  // survivors: tokens [0, n_sink) into rows len + t, tokens [t_win, cnt) into the window
+  const int n_sink = (int)max((int64_t)0, min((int64_t)cnt, c.sink - len));
+  const int t_win = max(n_sink, cnt - window);
+  const int items = n_sink + cnt - t_win;
+  const int slot0 = cnt > t_win ? (int)((len + t_win - c.sink) % c.window) : 0;
+  const bool on = lane * 8 < c.d, real = head < (int)c.heads;
+  const T* ks = kn + b * sk.b + head * sk.h + lane * 8;
+  const T* vs = vn + b * sv.b + head * sv.h + lane * 8;
+  const int64_t row0 = ((int64_t)b * c.heads + head) * c.rows;
+  for (int j0 = chunk * tp * kAppUnroll; j0 < items; j0 += chunks * tp * kAppUnroll) {
     uint4 xk[kAppUnroll], xv[kAppUnroll];
-    int64_t dst[kAppUnroll];
+    int row[kAppUnroll];
 #pragma unroll
     for (int u = 0; u < kAppUnroll; ++u) {
-      const int64_t i = i0 + u * kRows + threadIdx.x / G;
-      const int64_t h = i / n_new, t = i - h * n_new;
-      const int64_t p = len + t;
-      // padding, or a position that a later token of this call overwrites
-      const bool skip = i >= items || t >= cnt || (p >= c.sink && p < end - c.window);
+      const int j = j0 + u * tp + slot % tp;
       xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
-      dst[u] = -1;
-      if (!skip) {
-        const int64_t row = p < c.sink ? p : c.sink + (p - c.sink) % c.window;
-        dst[u] = ((int64_t)b * c.heads + h) * c.rows + row;
+      row[u] = -1;
+      if (j < items && real) {
+        const int k = j - n_sink;
+        const int t = k < 0 ? j : t_win + k;
+        const int w = slot0 + k;                             // < 2 * window
+        row[u] = k < 0 ? (int)len + j : sink + (w >= window ? w - window : w);
         if (on) {
-          xk[u] = __ldcs(reinterpret_cast<const uint4*>(kn + b * sk.b + h * sk.h + t * sk.n) + lane);
-          xv[u] = __ldcs(reinterpret_cast<const uint4*>(vn + b * sv.b + h * sv.h + t * sv.n) + lane);
+          xk[u] = __ldcs(reinterpret_cast<const uint4*>(ks + t * sk.n));
+          xv[u] = __ldcs(reinterpret_cast<const uint4*>(vs + t * sv.n));
         }
       }
     }
@@ -177,18 +187,19 @@ __global__ void __launch_bounds__(kAppThreads)
         for (int s = G / 2; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(kFull, m, s, G));
         const uint32_t e = scale_byte<FMT>(m);
         bytes |= e << (8 * part);
-        const float inv = e == kBadRow ? 0.f : scale_inverse(e);
         if (e == kBadRow) {
           codes[part] = make_uint2(0, 0);
         } else {
+          const float inv = scale_inverse(e);
           codes[part].x = encode4<FMT>(f[0].x * inv, f[0].y * inv, f[1].x * inv, f[1].y * inv);
           codes[part].y = encode4<FMT>(f[2].x * inv, f[2].y * inv, f[3].x * inv, f[3].y * inv);
         }
       }
-      if (dst[u] >= 0) {
-        reinterpret_cast<uint2*>(c.k + dst[u] * DP)[lane] = codes[0];
-        reinterpret_cast<uint2*>(c.v + dst[u] * DP)[lane] = codes[1];
-        if (lane == 0) c.scales[dst[u]] = (uint16_t)bytes;
+      if (row[u] >= 0) {
+        const int64_t dst = row0 + row[u];
+        reinterpret_cast<uint2*>(c.k + dst * DP)[lane] = codes[0];
+        reinterpret_cast<uint2*>(c.v + dst * DP)[lane] = codes[1];
+        if (lane == 0) c.scales[dst] = (uint16_t)bytes;
       }
     }
   }
@@ -196,12 +207,12 @@ __global__ void __launch_bounds__(kAppThreads)
   __syncthreads();
   if (threadIdx.x == 0) {
     if (gridDim.x == 1) {
-      lengths[b] = end;
+      lengths[b] = len + cnt;
     } else {
       __threadfence();
       if (atomicAdd(&tickets[b], 1) == (int)gridDim.x - 1) {
         tickets[b] = 0;
-        lengths[b] = end;
+        lengths[b] = len + cnt;
       }
     }
   }
@@ -212,8 +223,8 @@ __global__ void __launch_bounds__(kAppThreads)
 // ---------------------------------------------------------------------------
 // Out row i of a sequence is its i-th kept position in order (sinks, then the
 // window from its oldest), rows behind the last one are zero with position -1.
-// A group of DP / 8 lanes per row as above; bound by HBM (2 D + 2 bytes in, 4 D
-// out per kept row and head).
+// A group of DP / 8 lanes per row as above, CTAs walk the rows of one head; bound by HBM
+// (2 D + 2 bytes in, 4 D out per kept row and head).
 constexpr int kReadThreads = 256;
 constexpr int kReadUnroll = 4;
 
@@ -234,43 +245,53 @@ __device__ __forceinline__ uint4 values8(uint2 codes, float scale) {
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(kReadThreads)
     qcache_read_kernel(QCache c, const int64_t* __restrict__ lengths, T* __restrict__ ko,
-                       T* __restrict__ vo, int64_t* __restrict__ positions) {
+                       T* __restrict__ vo, int64_t* __restrict__ positions, int head_blocks,
+                       int hs) {
   constexpr int DP = G * 8;
   constexpr int kRows = kReadThreads / G;
   const int b = blockIdx.y;
-  const int lane = threadIdx.x % G;
+  const int lane = threadIdx.x % G, slot = threadIdx.x / G;
+  const int tp = kRows >> hs;
+  const int head = ((int)blockIdx.x % head_blocks << hs) + slot / tp;
+  const int chunk = (int)blockIdx.x / head_blocks, chunks = (int)gridDim.x / head_blocks;
+  if (head >= (int)c.heads) return;
   const int64_t len = max(lengths[b], (int64_t)0);
-  const int64_t items = c.rows * c.heads;
+  const int rows = (int)c.rows, sink = (int)c.sink, window = (int)c.window;
+  const int kept = (int)min(len, c.rows);
+  // behind the sinks, out row i is position shift + i; the oldest of them is in slot0
+  const int64_t shift = len <= c.rows ? 0 : len - c.rows;
+  const int slot0 = window > 0 ? (int)(shift % c.window) : 0;
+  const int64_t row0 = ((int64_t)b * c.heads + head) * c.rows;
   const bool on = lane * 8 < c.d;
-  for (int64_t i0 = (int64_t)blockIdx.x * kRows * kReadUnroll; i0 < items;
-       i0 += (int64_t)gridDim.x * kRows * kReadUnroll) {
+  for (int i0 = chunk * tp * kReadUnroll + slot % tp; i0 < rows; i0 += chunks * tp * kReadUnroll) {
     uint2 xk[kReadUnroll], xv[kReadUnroll];
     uint32_t sc[kReadUnroll];
 #pragma unroll
     for (int u = 0; u < kReadUnroll; ++u) {
-      const int64_t i = i0 + u * kRows + threadIdx.x / G;
+      const int i = i0 + u * tp;
       xk[u] = xv[u] = make_uint2(0, 0);
       sc[u] = 0x7f7f;
-      if (i >= items) continue;
-      const int64_t h = i / c.rows, r = i - h * c.rows;
-      const bool kept = r < min(len, c.rows);
-      // position, and the ring row that holds it
-      const int64_t p = r < c.sink || len <= c.rows ? r : len - c.window + r - c.sink;
-      if (lane == 0 && h == 0) positions[b * c.rows + r] = kept ? p : -1;
-      if (!kept) continue;
-      const int64_t row = p < c.sink ? p : c.sink + (p - c.sink) % c.window;
-      const int64_t src = ((int64_t)b * c.heads + h) * c.rows + row;
-      xk[u] = __ldcs(reinterpret_cast<const uint2*>(c.k + src * DP) + lane);
-      xv[u] = __ldcs(reinterpret_cast<const uint2*>(c.v + src * DP) + lane);
-      sc[u] = c.scales[src];
+      if (i < kept) {
+        const int w = slot0 + i - sink;                      // < 2 * window
+        const int64_t src = row0 + (i < sink ? i : sink + (w >= window ? w - window : w));
+        xk[u] = __ldcs(reinterpret_cast<const uint2*>(c.k + src * DP) + lane);
+        xv[u] = __ldcs(reinterpret_cast<const uint2*>(c.v + src * DP) + lane);
+        sc[u] = c.scales[src];
+      }
     }
 #pragma unroll
     for (int u = 0; u < kReadUnroll; ++u) {
-      const int64_t i = i0 + u * kRows + threadIdx.x / G;
-      if (i >= items || !on) continue;
-      const int64_t dst = ((int64_t)b * items + i) * c.d + lane * 8;
-      __stcs(reinterpret_cast<uint4*>(ko + dst), values8<T, FMT>(xk[u], scale_value(sc[u] & 255u)));
-      __stcs(reinterpret_cast<uint4*>(vo + dst), values8<T, FMT>(xv[u], scale_value(sc[u] >> 8)));
+      const int i = i0 + u * tp;
+      if (i < rows) {
+        if (lane == 0 && head == 0)
+          positions[b * c.rows + i] = i >= kept ? -1 : i < sink ? i : shift + i;
+        if (on) {
+          const int64_t dst = (row0 + i) * c.d + lane * 8;
+          __stcs(reinterpret_cast<uint4*>(ko + dst),
+                 values8<T, FMT>(xk[u], scale_value(sc[u] & 255u)));
+          __stcs(reinterpret_cast<uint4*>(vo + dst), values8<T, FMT>(xv[u], scale_value(sc[u] >> 8)));
+        }
+      }
     }
   }
 }
@@ -724,6 +745,29 @@ int by_format(int dtype, int fmt, int64_t D, F&& f) {
   return dtype == SBFA_BF16 ? fmts(__nv_bfloat16{}) : fmts(__half{});
 }
 
+// Grid of the append and read kernels for `rows` rows of each head: 2^hs heads per CTA
+// where a head has fewer rows than a CTA takes at a time, else as many CTAs along a head as
+// keep every SM busy with about two rounds of resident CTAs.
+struct RowGrid {
+  dim3 grid;
+  int head_blocks, hs;
+};
+int row_grid(int64_t B, int64_t H, int64_t rows, int per_cta, int unroll, int resident,
+             RowGrid* g) {
+  int hs = 0;
+  while ((1 << (hs + 1)) <= per_cta && (1 << hs) < H && (per_cta >> (hs + 1)) >= rows) ++hs;
+  const int64_t blocks = (H + (1ll << hs) - 1) >> hs;
+  const int64_t step = (int64_t)(per_cta >> hs) * unroll;
+  const int64_t want = (int64_t)device_sm_count() * resident * 2;
+  const int64_t chunks = std::max<int64_t>(
+      1, std::min((rows + step - 1) / step, (want + B * blocks - 1) / (B * blocks)));
+  if (blocks * chunks >= (1ll << 31)) return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many heads");
+  g->grid = dim3((unsigned)(blocks * chunks), (unsigned)B);
+  g->head_blocks = (int)blocks;
+  g->hs = hs;
+  return SBFA_OK;
+}
+
 // CTAs per unit of the attend kernel (a cluster, so a power of two up to 8).
 // More of them shorten a unit, which pays while there are SMs to fill.
 int attend_splits(int64_t units, int64_t rows, int slots) {
@@ -799,11 +843,13 @@ extern "C" int sbfa_qcache_append(void* k_codes, void* v_codes, void* scales, in
   return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
     constexpr int G = dp.value / 8;
-    const int64_t per = (int64_t)(kAppThreads / G) * kAppUnroll;
-    const dim3 grid((unsigned)std::min<int64_t>((n_new * H + per - 1) / per, 4096), (unsigned)B);
+    RowGrid g;
+    if (int rc = row_grid(B, H, std::min(n_new, c.rows), kAppThreads / G, kAppUnroll, 5, &g))
+      return rc;
     LaunchScope ls("qcache_append_kernel", s);
-    qcache_append_kernel<T, m.value, G><<<grid, kAppThreads, 0, s>>>(
-        c, lengths, tickets, (const T*)k_new, (const T*)v_new, st[0], st[1], counts, n_new);
+    qcache_append_kernel<T, m.value, G><<<g.grid, kAppThreads, 0, s>>>(
+        c, lengths, tickets, (const T*)k_new, (const T*)v_new, st[0], st[1], counts, (int)n_new,
+        g.head_blocks, g.hs);
     return check_launch("qcache_append_kernel");
   });
 }
@@ -825,12 +871,11 @@ extern "C" int sbfa_qcache_read(const void* k_codes, const void* v_codes, const 
   return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
     constexpr int G = dp.value / 8;
-    const int64_t per = (int64_t)(kReadThreads / G) * kReadUnroll;
-    const dim3 grid((unsigned)std::min<int64_t>((c.rows * H + per - 1) / per, 65535),
-                    (unsigned)B);
+    RowGrid g;
+    if (int rc = row_grid(B, H, c.rows, kReadThreads / G, kReadUnroll, 4, &g)) return rc;
     LaunchScope ls("qcache_read_kernel", s);
-    qcache_read_kernel<T, m.value, G>
-        <<<grid, kReadThreads, 0, s>>>(c, lengths, (T*)k_out, (T*)v_out, positions);
+    qcache_read_kernel<T, m.value, G><<<g.grid, kReadThreads, 0, s>>>(
+        c, lengths, (T*)k_out, (T*)v_out, positions, g.head_blocks, g.hs);
     return check_launch("qcache_read_kernel");
   });
 }
