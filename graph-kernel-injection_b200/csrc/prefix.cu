@@ -6,19 +6,27 @@
 // instead of once per sequence.  Row r is (sequence, head of the group, query) =
 // (r / (G n_q), r / n_q % G, r % n_q).
 //
-// prefix_tc_kernel: one CTA per (256 rows, key/value head, slice of the keys), the
-// pipeline of the block-sparse forward without its masks: a TMA warp streams K and V tiles
-// of 128 keys through a ring, one warp per 128-row tile issues the MMAs, a warpgroup
-// per tile runs the online softmax on TMEM (see attn_tc.cu for the TMEM plan).  Q
-// rows come from scattered places, so the softmax threads gather them (a thread per
-// row) into the swizzled operand tile.  With 128 rows or fewer in the
-// CTA the second tile's warps leave at once.  Few rows against a long prefix are
-// bound by HBM (4 D bytes per key) and the key axis is split over the SMs; many rows are
-// bound by the tensor cores (4 D operations per row and key).
-// Each slice leaves its unnormalised O row in fp32 with (m, l) of its softmax.
+// prefix_tc_kernel: one CTA per (256 rows, key/value head) or per slice of its keys, the
+// pipeline of the block-sparse forward: a TMA warp streams K and V tiles of 128 keys
+// through a ring, one warp per 128-row tile issues the MMAs, a warpgroup per tile
+// runs the online softmax on TMEM (see attn_tc.cu for the TMEM plan).  Q rows come from
+// scattered places, so the softmax threads gather them (a thread per row) into the
+// swizzled operand tile.  With 128 rows or fewer in the CTA the second tile's
+// warps leave at once.  Few rows against a long prefix are bound by HBM (4 D bytes per
+// key), many by the tensor cores and the exponentials (4 D operations and one exponential per
+// row and key).
 //
-// prefix_merge_kernel: one warp per query row joins the slices and the row's
-// attention over its own tokens (already normalised, with its log-sum-exp).
+// The batch's own prompts (n_q tokens each, causal window) follow as more key tiles of
+// the same pass: a tile of 128 keys of one sequence, or of 128 / 2^k short
+// sequences with 2^k >= n_q rows each, in which each query row sees one interval
+// of columns.  So a prompt takes one launch, and its two parts share one softmax and
+// one rounding.
+//
+// Slices.  Whole waves of CTAs take all keys of their rows and write O themselves.  The
+// rest (all of them in a decode step) would leave most SMs idle, so their keys are cut
+// into slices, which leave fp32 rows with (m, l) that prefix_merge_kernel joins.  Either
+// epilogue also joins the row's attention over its own tokens that a cache's kernel
+// has computed (already normalised, with its log-sum-exp).
 #include <cuda.h>
 
 #include <algorithm>
@@ -50,7 +58,78 @@ struct PrefixGeom {
   int64_t rows;        // R, rows per key/value head
   int64_t sb, sh, sn;  // q strides (batch, head, query)
   int64_t P;
-  int group, n_q, kv_heads, d, splits, n_tiles;
+  int group, n_q, kv_heads, batch, d;
+  int pairs;           // 256-row tiles per key/value head
+  int n_full, n_tail;  // units (tile, head) that take all keys / that are cut into slices
+  int splits;          // slices of a tail unit
+  int n_tiles;         // 128-key tiles of the prefix
+  int own;             // whether own tokens follow the prefix
+  int window, box;     // their window; rows of a TMA box of own keys (128 / box sequences a tile)
+};
+
+enum OwnKind { kOwnNone = 0, kOwn16 = 1, kOwn32 = 2 };
+
+// Where O goes and what a cache's kernel contributes to it.
+struct PrefixOut {
+  void* o;               // [B, H, n_q, d]
+  float* lse;            // [B, H, n_q] or NULL
+  const void* own_o;
+  const float* own_lse;
+  int own_kind;
+  float* part;           // [splits][n_tail * 256][D]
+  float2* stats;         // [splits][n_tail * 256] (m, l)
+};
+
+// Row of O for row `row` of a key/value head.
+__device__ __forceinline__ int64_t out_row(const PrefixGeom& g, int kvh, int64_t row) {
+  const int64_t per = (int64_t)g.group * g.n_q;
+  const int64_t b = row / per;
+  return (b * g.kv_heads + kvh) * per + (row - b * per);
+}
+
+// The own-key tiles that rows [row0, row1) need, in order: sequence by sequence (box == 128;
+// the first one's from its window's oldest key), or blocks of 128 / box sequences.
+struct OwnTiles {
+  int b0, kt0, c0;   // first sequence (or block), its first tile and tiles
+  int full;          // tiles of a whole sequence
+  int count;
+  __device__ __forceinline__ OwnTiles(const PrefixGeom& g, int64_t row0, int64_t row1) {
+    const int64_t per = (int64_t)g.group * g.n_q;
+    b0 = (int)(row0 / per);
+    const int b1 = (int)((row1 - 1) / per);
+    kt0 = 0;
+    full = 1;
+    if (g.box < kTN) {
+      const int seqs = kTN / g.box;
+      b0 /= seqs;
+      c0 = 1;
+      count = b1 / seqs - b0 + 1;
+      return;
+    }
+    full = (g.n_q + kTN - 1) / kTN;
+    // queries [lo, hi] of a run of rows: of several heads, all of them
+    const int64_t lo = row0 - b0 * per, hi = min(row1 - b0 * per, per) - 1;
+    const bool one = lo / g.n_q == hi / g.n_q;
+    const int q_lo = one ? (int)(lo % g.n_q) : 0, q_hi = one ? (int)(hi % g.n_q) : g.n_q - 1;
+    kt0 = (int)max((int64_t)0, (int64_t)q_lo - g.window + 1) / kTN;
+    c0 = q_hi / kTN - kt0 + 1;
+    count = c0;
+    if (b1 > b0) {
+      const int64_t last = row1 - 1 - b1 * per;
+      const int l_hi = last < g.n_q ? (int)last : g.n_q - 1;
+      count += (b1 - b0 - 1) * full + l_hi / kTN + 1;
+    }
+  }
+  // own tile u: sequence (or block of them) and its key tile
+  __device__ __forceinline__ void at(int u, int* b, int* kt) const {
+    if (u < c0) {
+      *b = b0;
+      *kt = kt0 + u;
+    } else {
+      *b = b0 + 1 + (u - c0) / full;
+      *kt = (u - c0) % full;
+    }
+  }
 };
 
 template <int D, int STAGES>
@@ -75,8 +154,10 @@ struct PrefixLayout {
 template <typename T, int D, int STAGES>
 __global__ void __launch_bounds__(kThreads, 1)
     prefix_tc_kernel(const T* __restrict__ q, const __grid_constant__ CUtensorMap tmk,
-                     const __grid_constant__ CUtensorMap tmv, float* __restrict__ part,
-                     float2* __restrict__ stats, float scale_log2, PrefixGeom geo, int* status) {
+                     const __grid_constant__ CUtensorMap tmv,
+                     const __grid_constant__ CUtensorMap tmok,
+                     const __grid_constant__ CUtensorMap tmov, PrefixOut out, float scale_log2,
+                     PrefixGeom geo, int* status) {
   using L = PrefixLayout<D, STAGES>;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescQK = idesc_f16(kBF16, kTM, kHalf, false, false);
@@ -92,13 +173,40 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = blockIdx.y;
-  const int64_t row0 = (int64_t)blockIdx.x * kPair * kTM;
+  const int bid = (int)blockIdx.x;
+  const bool sliced = bid >= geo.n_full;
+  const int tail = sliced ? (bid - geo.n_full) % geo.n_tail : 0;
+  const int split = sliced ? (bid - geo.n_full) / geo.n_tail : 0;
+  const int splits = sliced ? geo.splits : 1;
+  const int unit = sliced ? geo.n_full + tail : bid;
+  const int kvh = unit / geo.pairs;
+  const int64_t row0 = (int64_t)(unit % geo.pairs) * kPair * kTM;
   const int nx = row0 + kTM < geo.rows ? 2 : 1;  // tiles with rows in them
-  const int split = blockIdx.z;
-  // slices of n_tiles / splits tiles, none empty (splits <= n_tiles)
-  const int t0 = (int)((int64_t)split * geo.n_tiles / geo.splits);
-  const int n = (int)((int64_t)(split + 1) * geo.n_tiles / geo.splits) - t0;
+  OwnTiles own = OwnTiles(geo, row0, min(row0 + kPair * kTM, geo.rows));
+  const int n_all = geo.n_tiles + (geo.own ? own.count : 0);
+  // slices of n_all / splits tiles, none empty (splits <= n_tiles)
+  const int t0 = (int)((int64_t)split * n_all / splits);
+  const int n = (int)((int64_t)(split + 1) * n_all / splits) - t0;
+
+  // K (part 0) or V (part 1) of key tile t into ring slot s
+  auto load_tile = [&](int t, int part, int s) {
+    const uint32_t dst = sb + L::KV + (uint32_t)s * L::kTile;
+    mbar_expect_tx(bar(L::kKVFull + s), L::kTile);
+    if (t < geo.n_tiles) {
+      for (int r = 0; r < kBoxes; ++r)
+        tma_load_4d(dst + r * 16384u, part == 0 ? &tmk : &tmv, bar(L::kKVFull + s), 64 * r,
+                    t * kTN, kvh, 0);
+      return;
+    }
+    int b, kt;
+    own.at(t - geo.n_tiles, &b, &kt);
+    const int seqs = kTN / geo.box;
+    for (int i = 0; i < seqs; ++i)   // a sequence behind the last one reads as zeros
+      for (int r = 0; r < kBoxes; ++r)
+        tma_load_4d(dst + r * 16384u + (uint32_t)(i * geo.box) * 128u,
+                    part == 0 ? &tmok : &tmov, bar(L::kKVFull + s), 64 * r, kt * kTN, kvh,
+                    b * seqs + i);
+  };
 
   if (threadIdx.x == 0) {
     mbar_init(bar(L::kQFull), 128 * nx);
@@ -117,13 +225,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     *abort_flag = 0;
     mbar_init_fence();
-    // K_0 and V_0 on their way before the TMEM allocation and the CTA-wide sync
-    for (int part_ = 0; part_ < 2; ++part_) {
-      mbar_expect_tx(bar(L::kKVFull + part_), L::kTile);
-      for (int r = 0; r < kBoxes; ++r)
-        tma_load_4d(sb + L::KV + part_ * L::kTile + r * 16384u, part_ == 0 ? &tmk : &tmv,
-                    bar(L::kKVFull + part_), 64 * r, t0 * kTN, kvh, 0);
-    }
+    // the first K and V on their way before the TMEM allocation and the CTA-wide sync
+    load_tile(t0, 0, 0);
+    load_tile(t0, 1, 1);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), kTmemCols);
@@ -149,10 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          mbar_expect_tx(bar(L::kKVFull + s), L::kTile);
-          for (int r = 0; r < kBoxes; ++r)
-            tma_load_4d(sb + L::KV + s * L::kTile + r * 16384u, part_ == 0 ? &tmk : &tmv,
-                        bar(L::kKVFull + s), 64 * r, (t0 + j) * kTN, kvh, 0);
+          load_tile(t0 + j, part_, s);
           issued = e + 1;
         }
       }
@@ -237,11 +338,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
       const uint32_t t_sx = tmem + lane_base + 128u * x;
       const uint32_t t_o = tmem + lane_base + 256u + 128u * x;
+      const int64_t per = (int64_t)geo.group * geo.n_q;
+      const int64_t seq = row / per;
+      const int iq = (int)((row - seq * per) % geo.n_q);   // the row's query of its sequence
       {  // gather this thread's query row; columns behind d and rows behind R are zero
-        const int64_t per = (int64_t)geo.group * geo.n_q;
-        const int64_t b = row / per, rem = row - b * per;
-        const int64_t hg = rem / geo.n_q, i = rem - hg * geo.n_q;
-        const T* src = q + b * geo.sb + (kvh * (int64_t)geo.group + hg) * geo.sh + i * geo.sn;
+        const int64_t hg = (row - seq * per) / geo.n_q;
+        const T* src = q + seq * geo.sb + (kvh * (int64_t)geo.group + hg) * geo.sh + iq * geo.sn;
         const uint32_t tile = sb + L::Q + (uint32_t)x * L::kTile;
         uint4 w[D / 8];
 #pragma unroll
@@ -264,8 +366,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int u = 0; u < U; ++u) {
         const int h = u & 1;
-        const int64_t k0 = (int64_t)(t0 + (u >> 1)) * kTN + kHalf * h;
-        const int left = (int)min((int64_t)kHalf, geo.P - k0);  // <= 0: nothing of this half
+        const int t = t0 + (u >> 1);
+        // visible keys of this half-step: one interval of columns
+        uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+        bool all_vis = t < geo.n_tiles - 1;   // all but the prefix's last tile are full
+        if (!all_vis) {
+          int lo = 0, hi;
+          if (t < geo.n_tiles) {
+            hi = (int)(geo.P - (int64_t)t * kTN);
+          } else {
+            int b, kt;
+            own.at(t - geo.n_tiles, &b, &kt);
+            const int seqs = kTN / geo.box;
+            const int64_t s = seq - (int64_t)b * seqs;     // this row's sequence in the tile
+            const int off = (int)s * geo.box - kt * kTN;
+            lo = off + max(iq - geo.window + 1, 0);
+            hi = live && s >= 0 && s < seqs ? off + iq + 1 : 0;
+          }
+          vis[0] = range_bits(lo, hi, kHalf * h);
+          vis[1] = range_bits(lo, hi, kHalf * h + 32);
+          all_vis = __all_sync(0xffffffffu, (vis[0] & vis[1]) == 0xffffffffu);
+        }
         ok = wait_bar_w(bar(L::kSFull + 2 * x + h), (uint32_t)((u >> 1) & 1), abort_flag, status);
         if (!ok) break;
         tc_fence_after();
@@ -274,10 +395,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld32(t_s, sv);
         tmem_ld32(t_s + 32u, sv + 32);
         tmem_wait_ld();
-        if (left < kHalf) {
+        if (!all_vis) {
 #pragma unroll
           for (int c = 0; c < kHalf; ++c)
-            if (c >= left) sv[c] = __float_as_uint(-INFINITY);
+            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sv[c] = __float_as_uint(-INFINITY);
         }
         if (!settled) {
           float mx[8];
@@ -323,12 +444,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float alpha = need ? ex2(m_run - m_new) : 1.f;
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
-            uint32_t t[32];
-            tmem_ld32(t_o + 32u * c, t);
+            uint32_t ov[32];
+            tmem_ld32(t_o + 32u * c, ov);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) t[i] = __float_as_uint(__uint_as_float(t[i]) * alpha);
-            tmem_st32(t_o + 32u * c, t);
+            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+            tmem_st32(t_o + 32u * c, ov);
           }
           if (need) {
             l_run *= alpha;
@@ -338,14 +459,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float m_re = (m_run == -INFINITY) ? 0.f : m_run;
 #pragma unroll 1
           for (int c = 0; c < kHalf / 32; ++c) {
-            uint32_t t[32], w[16];
-            tmem_ld32(t_s + 32u * c, t);
+            uint32_t sc[32], w[16];
+            tmem_ld32(t_s + 32u * c, sc);
             tmem_wait_ld();
+            const uint32_t vb = c == 0 ? vis[0] : vis[1];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float s0 = 32 * c + 2 * i < left ? __uint_as_float(t[2 * i]) : -INFINITY;
+              const float s0 = ((vb >> (2 * i)) & 1u) ? __uint_as_float(sc[2 * i]) : -INFINITY;
               const float s1 =
-                  32 * c + 2 * i + 1 < left ? __uint_as_float(t[2 * i + 1]) : -INFINITY;
+                  ((vb >> (2 * i + 1)) & 1u) ? __uint_as_float(sc[2 * i + 1]) : -INFINITY;
               const float p0 = ex2(fmaf(s0, scale_log2, -m_re));
               const float p1 = ex2(fmaf(s1, scale_log2, -m_re));
               rsum += p0 + p1;
@@ -362,21 +484,83 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) ok = wait_bar_w(bar(L::kOFull + x), 0, abort_flag, status);
       if (ok) {
         tc_fence_after();
-        const int64_t slot = ((int64_t)split * geo.kv_heads + kvh) * geo.rows + row;
-        float* dst = part + slot * D;
+        // A row's 2 D bytes pass through this warp's part of the Q tile, which is no
+        // longer read, so that a row is written by adjacent lanes.
+        const uint32_t stage = sb + L::Q + (uint32_t)x * L::kTile;
+        constexpr int kChunks = D / 8;
+        auto put = [&](int c, uint32_t a, uint32_t b, uint32_t e, uint32_t f) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                           stage + (uint32_t)(c >> 3) * 16384u +
+                           sw128_offset((uint32_t)r, 8u * (uint32_t)(c & 7))),
+                       "r"(a), "r"(b), "r"(e), "r"(f)
+                       : "memory");
+        };
+        auto flush = [&](char* dst, int chunks) {   // chunks of 16 bytes that exist
+          __syncwarp();
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t t[32];
-          tmem_ld32(t_o + 32u * c, t);
-          tmem_wait_ld();
-          if (live) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(dst + 32 * c + 4 * i) =
-                  make_uint4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
+          for (int i = 0; i < kChunks; ++i) {
+            const int rr = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
+            char* to = (char*)__shfl_sync(0xffffffffu, (unsigned long long)dst, rr);
+            uint4 w;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                         : "r"(stage + (uint32_t)(c >> 3) * 16384u +
+                               sw128_offset((uint32_t)(quarter * 32 + rr), 8u * (uint32_t)(c & 7))));
+            if (to != nullptr && c < chunks) reinterpret_cast<uint4*>(to)[c] = w;
           }
+          __syncwarp();
+        };
+        if (sliced) {
+          const int64_t all = (int64_t)geo.n_tail * (kPair * kTM);
+          const int64_t slot = split * all + (int64_t)tail * (kPair * kTM) + x * kTM + r;
+          if (live) out.stats[slot] = make_float2(m_run, l_run);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {   // D / 2 fp32 columns at a time
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              uint32_t ov[32];
+              tmem_ld32(t_o + (uint32_t)(half * (D / 2) + 32 * c), ov);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                put(8 * c + i, ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
+            }
+            flush(live ? (char*)(out.part + slot * D + half * (D / 2)) : nullptr, kChunks);
+          }
+        } else {
+          const int64_t at = live ? out_row(geo, kvh, row) : 0;
+          const float own_l2 =
+              out.own_kind != kOwnNone && live ? out.own_lse[at] * kLog2e : -INFINITY;
+          const float M = fmaxf(m_run, own_l2);
+          const float f_own = own_l2 == -INFINITY ? 0.f : ex2(own_l2 - M);
+          const float f_pre = ex2(m_run - M);
+          const float l = l_run * f_pre + f_own;
+          const float inv = 1.f / l;
+          const float w_pre = f_pre * inv, w_own = f_own * inv;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t ov[32];
+            tmem_ld32(t_o + 32u * c, ov);
+            tmem_wait_ld();
+            float f[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(ov[i]) * w_pre;
+            if (f_own != 0.f) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (32 * c + i < geo.d)
+                  f[i] += w_own * (out.own_kind == kOwn32
+                                       ? ((const float*)out.own_o)[at * geo.d + 32 * c + i]
+                                       : Elem<T>::to(((const T*)out.own_o)[at * geo.d + 32 * c + i]));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              put(4 * c + i, pack2<T>(f[8 * i], f[8 * i + 1]), pack2<T>(f[8 * i + 2], f[8 * i + 3]),
+                  pack2<T>(f[8 * i + 4], f[8 * i + 5]), pack2<T>(f[8 * i + 6], f[8 * i + 7]));
+          }
+          flush(live ? (char*)((T*)out.o + at * geo.d) : nullptr, geo.d / 8);
+          if (live && out.lse) out.lse[at] = (M + log2f(l)) * kLn2;
         }
-        if (live) stats[slot] = make_float2(m_run, l_run);
       }
     }
   }
@@ -393,24 +577,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 // merge
 // ---------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
-enum OwnKind { kOwnNone = 0, kOwn16 = 1, kOwn32 = 2 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeThreads)
-    prefix_merge_kernel(const float* __restrict__ part, const float2* __restrict__ stats,
-                        const void* __restrict__ own_o, const float* __restrict__ own_lse,
-                        int own_kind, T* __restrict__ o, float* __restrict__ lse,
-                        PrefixGeom geo) {
+    prefix_merge_kernel(PrefixOut po, PrefixGeom geo) {
   constexpr int kLanes = D / 4;            // lanes per row, four columns each
   constexpr int kRows = kMergeThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const int64_t all = geo.rows * geo.kv_heads;
+  const int64_t all = (int64_t)geo.n_tail * (kPair * kTM);
   const int64_t at = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
   if (at >= all) return;
-  const int64_t kvh = at / geo.rows, row = at - kvh * geo.rows;
-  const int64_t per = (int64_t)geo.group * geo.n_q;
-  const int64_t b = row / per, rem = row - b * per;   // rem = head of the group * n_q + query
-  const int64_t out = (b * geo.kv_heads + kvh) * per + rem;   // row of o [B, H, n_q]
+  const int unit = geo.n_full + (int)(at / (kPair * kTM));
+  const int64_t row = (int64_t)(unit % geo.pairs) * (kPair * kTM) + at % (kPair * kTM);
+  if (row >= geo.rows) return;
+  const int64_t out = out_row(geo, unit / geo.pairs, row);
+  const float* part = po.part;
+  const float2* stats = po.stats;
+  const int own_kind = po.own_kind;
+  const void* own_o = po.own_o;
+  const float* own_lse = po.own_lse;
+  T* o = (T*)po.o;
+  float* lse = po.lse;
   const bool on = lane * 4 < geo.d;
   const float own_l2 =
       own_kind == kOwnNone ? -INFINITY : own_lse[out] * kLog2e;   // log2 of the own weight
@@ -461,16 +648,17 @@ int tile_dim(int64_t d) {
   return d <= 64 ? 64 : 128;
 }
 
-// Key slices: whole waves of one CTA per SM, each as long as its tiles plus a set-up worth
-// about three (Q gather, pipeline fill, epilogue), against the partial rows that every
-// slice writes and the merge reads (a tile's time moves about 6 MB).
-int prefix_splits(int64_t ctas, int n_tiles, int64_t part_bytes) {
+// Slices of the tail units: whole waves of one CTA per SM, each as long as its tiles plus
+// a set-up worth about three (Q gather, pipeline fill, epilogue), against the partial
+// rows that every slice writes and the merge reads (a tile's time moves about 6 MB).
+int prefix_splits(int64_t units, int n_tiles, int64_t part_bytes) {
   const int64_t sms = device_sm_count();
   int best = 1;
   double best_cost = 1e300;
   for (int ns = 1; ns <= std::min(n_tiles, 64); ++ns) {
-    const int64_t waves = (ctas * ns + sms - 1) / sms;
-    const double cost = (double)waves * ((n_tiles + ns - 1) / ns + 3) + ns * part_bytes / 3e6;
+    const int64_t waves = (units * ns + sms - 1) / sms;
+    const double cost =
+        (double)waves * ((n_tiles + ns - 1) / ns + 3) + (ns > 1 ? ns * part_bytes / 3e6 + 2 : 0);
     if (cost < best_cost) {
       best_cost = cost;
       best = ns;
@@ -480,74 +668,147 @@ int prefix_splits(int64_t ctas, int n_tiles, int64_t part_bytes) {
 }
 
 bool prefix_geometry(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P,
-                     int64_t head_dim, PrefixGeom* geo) {
-  if (B <= 0 || H <= 0 || n_q <= 0 || P <= 0 || P >= (1ll << 31) || tile_dim(head_dim) == 0)
+                     int64_t head_dim, int64_t window, PrefixGeom* geo) {
+  if (B <= 0 || H <= 0 || n_q <= 0 || P <= 0 || P >= (1ll << 31) - kTN || window < 0 ||
+      tile_dim(head_dim) == 0)
     return false;
   if (kv_heads <= 0) kv_heads = H;
-  if (H % kv_heads != 0 || kv_heads > 65535 || B >= (1ll << 31) || H >= (1ll << 31) ||
-      n_q >= (1ll << 31))
+  if (H % kv_heads != 0 || B >= (1ll << 31) || H >= (1ll << 31) || n_q >= (1ll << 30))
     return false;
   const int64_t group = H / kv_heads;
-  if (B * group >= (1ll << 31) || B * group * n_q >= (1ll << 38)) return false;
+  // rows of a key/value head, and CTAs, in 31 bits
+  if (B * group >= (1ll << 31) || B * group * n_q >= (1ll << 31)) return false;
   geo->rows = B * group * n_q;
+  const int64_t pairs = (geo->rows + kPair * kTM - 1) / (kPair * kTM);
+  const int64_t units = pairs * kv_heads;
+  if (units >= (1ll << 30)) return false;
+  geo->sb = geo->sh = geo->sn = 0;
   geo->P = P;
   geo->group = (int)group;
   geo->n_q = (int)n_q;
   geo->kv_heads = (int)kv_heads;
+  geo->batch = (int)B;
   geo->d = (int)head_dim;
+  geo->pairs = (int)pairs;
   geo->n_tiles = ceil_div_i(P, kTN);
-  const int64_t pairs = (geo->rows + kPair * kTM - 1) / (kPair * kTM);
-  geo->splits = prefix_splits(pairs * kv_heads, geo->n_tiles,
-                              geo->rows * kv_heads * tile_dim(head_dim) * 4);
+  geo->own = window > 0;
+  geo->window = (int)std::min<int64_t>(window, n_q);
+  // a box of own keys holds one sequence's rows: the least power of two, at least the 8 rows
+  // of a swizzle atom; more than 64 rows take whole tiles of one sequence
+  int box = 8;
+  while (box < n_q && box < kTN) box *= 2;
+  geo->box = box;
+  const int sms = device_sm_count();
+  geo->n_full = (int)(units / sms * sms);
+  geo->n_tail = (int)(units - geo->n_full);
+  geo->splits = 1;
+  if (geo->n_tail > 0)
+    geo->splits = prefix_splits(geo->n_tail, geo->n_tiles,
+                                (int64_t)geo->n_tail * kPair * kTM * tile_dim(head_dim) * 4);
+  if (geo->splits == 1) {  // nothing to cut
+    geo->n_full += geo->n_tail;
+    geo->n_tail = 0;
+  }
   return true;
 }
 
-int64_t stats_bytes(const PrefixGeom& g) {
-  return (g.splits * g.kv_heads * g.rows * (int64_t)sizeof(float2) + 255) / 256 * 256;
+int64_t tail_rows(const PrefixGeom& g) {
+  return (int64_t)g.splits * g.n_tail * kPair * kTM;
 }
-int64_t part_bytes(const PrefixGeom& g) {
-  return g.splits * g.kv_heads * g.rows * (int64_t)tile_dim(g.d) * (int64_t)sizeof(float);
+int64_t ws_bytes_of(const PrefixGeom& g) {
+  return tail_rows(g) * (tile_dim(g.d) * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
 }
 
+// Everything of a call but its sizes.
+struct PrefixCall {
+  const void *q, *k, *v;        // queries; prefix
+  const void *own_k, *own_v;    // own tokens or NULL
+  Strides3 sk, sv;              // their strides
+  PrefixOut out;
+  float scale;
+  void* ws;
+  cudaStream_t stream;
+};
+
 template <typename T, int D, int STAGES>
-int launch_prefix(const void* q, const void* k, const void* v, const void* own_o,
-                  const float* own_lse, int own_kind, void* o, float* lse, float scale,
-                  const PrefixGeom& geo, void* ws, cudaStream_t s) {
+int launch_prefix(const PrefixCall& c, const PrefixGeom& geo) {
   using L = PrefixLayout<D, STAGES>;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mok, mov;
+  const uint64_t d = (uint64_t)geo.d, P = (uint64_t)geo.P, h = (uint64_t)geo.kv_heads;
   const Strides3 st{geo.kv_heads * geo.P * geo.d, geo.P * geo.d, geo.d};
-  if (int rc = make_tmap_4d(&mk, k, kBF16, (uint64_t)geo.d, (uint64_t)geo.P,
-                            (uint64_t)geo.kv_heads, 1, st, kTN))
-    return rc;
-  if (int rc = make_tmap_4d(&mv, v, kBF16, (uint64_t)geo.d, (uint64_t)geo.P,
-                            (uint64_t)geo.kv_heads, 1, st, kTN))
-    return rc;
-  float2* stats = (float2*)ws;
-  float* part = (float*)((char*)ws + stats_bytes(geo));
+  if (int rc = make_tmap_4d(&mk, c.k, kBF16, d, P, h, 1, st, kTN)) return rc;
+  if (int rc = make_tmap_4d(&mv, c.v, kBF16, d, P, h, 1, st, kTN)) return rc;
+  mok = mk;
+  mov = mv;
+  if (geo.own) {
+    const uint64_t n = (uint64_t)geo.n_q, b = (uint64_t)geo.batch;
+    if (int rc = make_tmap_4d(&mok, c.own_k, kBF16, d, n, h, b, c.sk, (uint32_t)geo.box)) return rc;
+    if (int rc = make_tmap_4d(&mov, c.own_v, kBF16, d, n, h, b, c.sv, (uint32_t)geo.box)) return rc;
+  }
+  PrefixOut out = c.out;
+  out.stats = (float2*)c.ws;   // tail_rows is a multiple of 256, so part stays aligned
+  out.part = (float*)((char*)c.ws + tail_rows(geo) * (int64_t)sizeof(float2));
   auto kern = prefix_tc_kernel<T, D, STAGES>;
   if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)L::kAlloc),
                           "cudaFuncSetAttribute(prefix_tc)"))
     return rc;
-  const int64_t pairs = (geo.rows + kPair * kTM - 1) / (kPair * kTM);
-  if (pairs >= (1ll << 31)) return fail(SBFA_ERR_UNSUPPORTED, "prefix: too many query rows");
   {
-    LaunchScope ls("prefix_tc_kernel", s);
-    kern<<<dim3((unsigned)pairs, (unsigned)geo.kv_heads, (unsigned)geo.splits), kThreads,
-           L::kAlloc, s>>>((const T*)q, mk, mv, part, stats, scale * kLog2e, geo,
-                           device_status_ptr());
+    LaunchScope ls("prefix_tc_kernel", c.stream);
+    kern<<<(unsigned)(geo.n_full + geo.n_tail * geo.splits), kThreads, L::kAlloc, c.stream>>>(
+        (const T*)c.q, mk, mv, mok, mov, out, c.scale * kLog2e, geo, device_status_ptr());
   }
   if (int rc = check_launch("prefix_tc_kernel")) return rc;
+  if (geo.n_tail == 0) return SBFA_OK;
   const int64_t rows_per = kMergeThreads / (D / 4);
-  const int64_t blocks = (geo.rows * geo.kv_heads + rows_per - 1) / rows_per;
-  if (blocks >= (1ll << 31)) return fail(SBFA_ERR_UNSUPPORTED, "prefix: too many query rows");
+  const int64_t blocks = ((int64_t)geo.n_tail * kPair * kTM + rows_per - 1) / rows_per;
   {
-    LaunchScope ls("prefix_merge_kernel", s);
-    prefix_merge_kernel<T, D><<<(unsigned)blocks, kMergeThreads, 0, s>>>(
-        part, stats, own_o, own_lse, own_kind, (T*)o, lse, geo);
+    LaunchScope ls("prefix_merge_kernel", c.stream);
+    prefix_merge_kernel<T, D><<<(unsigned)blocks, kMergeThreads, 0, c.stream>>>(out, geo);
   }
   return check_launch("prefix_merge_kernel");
+}
+
+// Checks what both entry points share and launches.
+int run_prefix(PrefixCall& c, const int64_t* q_strides, PrefixGeom& geo, int64_t H, int dtype,
+               double softmax_scale, int64_t ws_bytes) {
+  if (!(softmax_scale > 0) || softmax_scale > 1e30)
+    return fail(SBFA_ERR_INVALID, "softmax_scale must be positive and finite");
+  if (!c.q || !c.k || !c.v || !c.out.o)
+    return fail(SBFA_ERR_INVALID, "prefix attention: NULL tensor pointer");
+  geo.sn = q_strides ? q_strides[2] : geo.d;
+  geo.sh = q_strides ? q_strides[1] : (int64_t)geo.n_q * geo.d;
+  geo.sb = q_strides ? q_strides[0] : H * geo.n_q * geo.d;
+  if (geo.sb < 0 || geo.sh < 0 || geo.sn < 0 || geo.sb % 8 || geo.sh % 8 || geo.sn % 8)
+    return fail(SBFA_ERR_INVALID,
+                "prefix attention: q strides must be non-negative multiples of 8 elements");
+  for (const void* p : {c.q, c.k, c.v, c.out.own_o, (const void*)c.out.o, (const void*)c.ws})
+    if ((uintptr_t)p & 15u)
+      return fail(SBFA_ERR_INVALID, "prefix attention: tensors must be 16-byte aligned");
+  const int64_t need = ws_bytes_of(geo);
+  if (need > 0 && (c.ws == nullptr || ws_bytes < need))
+    return fail(SBFA_ERR_INVALID, "prefix attention: workspace too small (need " +
+                                      std::to_string(need) + " bytes)");
+  c.scale = (float)softmax_scale;
+  if (tile_dim(geo.d) == 64)
+    return dtype == SBFA_BF16 ? launch_prefix<__nv_bfloat16, 64, 8>(c, geo)
+                              : launch_prefix<__half, 64, 8>(c, geo);
+  return dtype == SBFA_BF16 ? launch_prefix<__nv_bfloat16, 128, 5>(c, geo)
+                            : launch_prefix<__half, 128, 5>(c, geo);
+}
+
+int check_prefix(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim,
+                 int dtype, int64_t window, PrefixGeom* geo) {
+  if (dtype != SBFA_F16 && dtype != SBFA_BF16)
+    return fail(SBFA_ERR_UNSUPPORTED, "prefix attention: dtype must be float16 or bfloat16");
+  if (tile_dim(head_dim) == 0)
+    return fail(SBFA_ERR_UNSUPPORTED,
+                "prefix attention: head_dim must be a multiple of 8 and at most 128");
+  if (!prefix_geometry(B, H, kv_heads, n_q, P, head_dim, window, geo))
+    return fail(SBFA_ERR_INVALID, "prefix attention: sizes must be positive, H a multiple of "
+                                  "kv_heads, P and B * H / kv_heads * n_q below 2^31");
+  return SBFA_OK;
 }
 
 }  // namespace
@@ -556,10 +817,11 @@ int launch_prefix(const void* q, const void* k, const void* v, const void* own_o
 using namespace sbfa;
 
 extern "C" int64_t sbfa_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
-                                               int64_t n_q, int64_t P, int64_t head_dim) {
+                                               int64_t n_q, int64_t P, int64_t head_dim,
+                                               int64_t window) {
   PrefixGeom geo;
-  if (!prefix_geometry(B, H, kv_heads, n_q, P, head_dim, &geo)) return 0;
-  return stats_bytes(geo) + part_bytes(geo);
+  if (!prefix_geometry(B, H, kv_heads, n_q, P, head_dim, window, &geo)) return -1;
+  return ws_bytes_of(geo);
 }
 
 extern "C" int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const void* k_prefix,
@@ -568,44 +830,51 @@ extern "C" int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const
                                   int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim,
                                   int dtype, double softmax_scale, void* ws, int64_t ws_bytes,
                                   void* stream) {
-  if (dtype != SBFA_F16 && dtype != SBFA_BF16)
-    return fail(SBFA_ERR_UNSUPPORTED, "sbfa_prefix_attend: dtype must be float16 or bfloat16");
-  if (tile_dim(head_dim) == 0)
-    return fail(SBFA_ERR_UNSUPPORTED,
-                "sbfa_prefix_attend: head_dim must be a multiple of 8 and at most 128");
   PrefixGeom geo;
-  if (!prefix_geometry(B, H, kv_heads, n_q, P, head_dim, &geo))
-    return fail(SBFA_ERR_INVALID, "sbfa_prefix_attend: sizes must be positive and below 2^31, H "
-                                  "a multiple of kv_heads");
-  if (!(softmax_scale > 0) || softmax_scale > 1e30)
-    return fail(SBFA_ERR_INVALID, "softmax_scale must be positive and finite");
-  if (!q || !k_prefix || !v_prefix || !o)
-    return fail(SBFA_ERR_INVALID, "sbfa_prefix_attend: NULL tensor pointer");
+  if (int rc = check_prefix(B, H, kv_heads, n_q, P, head_dim, dtype, 0, &geo)) return rc;
   if (own_kind < 0 || own_kind > 2 || (own_kind != 0 && (!own_o || !own_lse)))
     return fail(SBFA_ERR_INVALID, "sbfa_prefix_attend: own_o and own_lse must match own_kind");
-  geo.sn = q_strides ? q_strides[2] : head_dim;
-  geo.sh = q_strides ? q_strides[1] : n_q * head_dim;
-  geo.sb = q_strides ? q_strides[0] : H * n_q * head_dim;
-  if (geo.sb < 0 || geo.sh < 0 || geo.sn < 0 || geo.sb % 8 || geo.sh % 8 || geo.sn % 8)
-    return fail(SBFA_ERR_INVALID,
-                "sbfa_prefix_attend: q strides must be non-negative multiples of 8 elements");
-  for (const void* p : {q, k_prefix, v_prefix, own_o, (const void*)o, (const void*)ws})
-    if ((uintptr_t)p & 15u)
-      return fail(SBFA_ERR_INVALID, "sbfa_prefix_attend: tensors must be 16-byte aligned");
-  const int64_t need = stats_bytes(geo) + part_bytes(geo);
-  if (ws == nullptr || ws_bytes < need)
-    return fail(SBFA_ERR_INVALID, "sbfa_prefix_attend: workspace too small (need " +
-                                      std::to_string(need) + " bytes)");
-  cudaStream_t s = (cudaStream_t)stream;
-  const float sc = (float)softmax_scale;
-#define SBFA_PREFIX(TT, DD, ST) \
-  return launch_prefix<TT, DD, ST>(q, k_prefix, v_prefix, own_o, own_lse, own_kind, o, lse, sc, \
-                                   geo, ws, s)
-  if (tile_dim(head_dim) == 64) {
-    if (dtype == SBFA_BF16) SBFA_PREFIX(__nv_bfloat16, 64, 8);
-    SBFA_PREFIX(__half, 64, 8);
-  }
-  if (dtype == SBFA_BF16) SBFA_PREFIX(__nv_bfloat16, 128, 5);
-  SBFA_PREFIX(__half, 128, 5);
-#undef SBFA_PREFIX
+  PrefixCall c = {};
+  c.q = q;
+  c.k = k_prefix;
+  c.v = v_prefix;
+  c.out.o = o;
+  c.out.lse = lse;
+  c.out.own_o = own_o;
+  c.out.own_lse = own_lse;
+  c.out.own_kind = own_kind;
+  c.ws = ws;
+  c.stream = (cudaStream_t)stream;
+  return run_prefix(c, q_strides, geo, H, dtype, softmax_scale, ws_bytes);
+}
+
+extern "C" int sbfa_prefix_prompt(const void* q, const void* k, const void* v,
+                                  const int64_t* strides, const void* k_prefix,
+                                  const void* v_prefix, void* o, float* lse, int64_t B, int64_t H,
+                                  int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim,
+                                  int dtype, double softmax_scale, int64_t window, void* ws,
+                                  int64_t ws_bytes, void* stream) {
+  PrefixGeom geo;
+  if (int rc = check_prefix(B, H, kv_heads, n_q, P, head_dim, dtype, window, &geo)) return rc;
+  if (window < 1)
+    return fail(SBFA_ERR_INVALID, "sbfa_prefix_prompt: window must be at least 1");
+  if (!k || !v) return fail(SBFA_ERR_INVALID, "sbfa_prefix_prompt: NULL tensor pointer");
+  PrefixCall c = {};
+  c.q = q;
+  c.k = k_prefix;
+  c.v = v_prefix;
+  c.own_k = k;
+  c.own_v = v;
+  const int64_t hk = geo.kv_heads;
+  const Strides3 dense{hk * n_q * head_dim, n_q * head_dim, head_dim};
+  c.sk = strides ? Strides3{strides[3], strides[4], strides[5]} : dense;
+  c.sv = strides ? Strides3{strides[6], strides[7], strides[8]} : dense;
+  if (!tma_compatible(k, c.sk) || !tma_compatible(v, c.sv))
+    return fail(SBFA_ERR_INVALID, "sbfa_prefix_prompt: k and v must be 16-byte aligned with "
+                                  "strides that are positive multiples of 8 elements");
+  c.out.o = o;
+  c.out.lse = lse;
+  c.ws = ws;
+  c.stream = (cudaStream_t)stream;
+  return run_prefix(c, strides, geo, H, dtype, softmax_scale, ws_bytes);
 }

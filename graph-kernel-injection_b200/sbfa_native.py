@@ -71,7 +71,9 @@ _SIGNATURES = {
                           _i64, _vp], _i32),
     "sbfa_prefix_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64,
                             _i64, _i64, _i32, _f64, _vp, _i64, _vp], _i32),
-    "sbfa_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
+    "sbfa_prefix_prompt": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                            _i64, _i32, _f64, _i64, _vp, _i64, _vp], _i32),
+    "sbfa_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "sbfa_decode_noalloc": ([_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _f64, _i32,
                              _i64, _i64, _vp, _i64, _i64, _vp], _i32),
 }

@@ -28,9 +28,6 @@ import sparse_triton_kernel as stk
 # how a row's attention to its own tokens comes to the merge (sbfa_prefix_attend)
 OWN_NONE, OWN_16, OWN_32 = 0, 1, 2
 
-_PROMPT_BLOCK = 128   # block size of the causal window mask behind attend_prompt
-
-
 def no_gradients(*tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("this serving operator has no gradients: call it under torch.no_grad() "
@@ -43,6 +40,12 @@ def vector_readable(t: torch.Tensor) -> torch.Tensor:
     if st[-1] != 1 or t.data_ptr() % 16 or any(x < 0 or x % 8 for x in st[:-1]):
         return t.clone(memory_format=torch.contiguous_format)
     return t
+
+
+def tma_readable(t: torch.Tensor) -> torch.Tensor:
+    """``t`` when tiles of it can be fetched in place, else a contiguous copy."""
+    t = stk._readable(t, True)
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 class SharedPrefix:
@@ -65,6 +68,7 @@ class SharedPrefix:
                           else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
         self.heads, self.length, self.head_dim = (int(x) for x in k.shape)
         self.dtype, self.device = k.dtype, k.device
+        self._code = native.dtype_code(k.dtype)
 
     def _check(self, q: torch.Tensor) -> None:
         if (q.dim() != 4 or 0 in q.shape or q.shape[1] % self.heads
@@ -83,20 +87,25 @@ class SharedPrefix:
         self._check(q)
         q = vector_readable(q)
         B, H, N, D = q.shape
-        L = native.lib()
         dev = self.device
         o = torch.empty((B, H, N, D), dtype=self.dtype, device=dev)
         lse = torch.empty((B, H, N), dtype=torch.float32, device=dev)
         with native.device_guard(dev):
-            need = int(L.sbfa_prefix_workspace_bytes(B, H, self.heads, N, self.length, D))
-            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-            native.check(L.sbfa_prefix_attend(
+            ws, ws_bytes = self._workspace(B, H, N, 0)
+            native.check(native.lib().sbfa_prefix_attend(
                 q.data_ptr(), (ctypes.c_int64 * 3)(*q.stride()[:3]), self.k.data_ptr(),
                 self.v.data_ptr(), native.ptr(own_o), native.ptr(own_lse), own_kind,
-                o.data_ptr(), lse.data_ptr(), B, H, self.heads, N, self.length, D,
-                native.dtype_code(self.dtype), scale, ws.data_ptr(), ws.numel(),
-                native.stream_ptr(dev)), "prefix_attend")
+                o.data_ptr(), lse.data_ptr(), B, H, self.heads, N, self.length, D, self._code,
+                scale, native.ptr(ws), ws_bytes, native.stream_ptr(dev)), "prefix_attend")
         return o, lse
+
+    def _workspace(self, B: int, H: int, N: int, window: int):
+        """Scratch of one call (from torch's allocator, so of its stream or graph) and its bytes."""
+        need = native.lib().sbfa_prefix_workspace_bytes(B, H, self.heads, N, self.length,
+                                                        self.head_dim, window)
+        if need <= 0:   # none, or a bad shape that the call refuses
+            return None, 0
+        return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
     def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
                return_lse: bool = False):
@@ -110,9 +119,8 @@ class SharedPrefix:
                       softmax_scale: Optional[float] = None, return_lse: bool = False):
         """Attention of the batch's own prompts behind the prefix: query ``i`` of a sequence
         ([B, H, N, D]) sees the whole prefix and the sequence's tokens ``(i - window_size, i]``
-        of ``k``, ``v`` ([B, H_kv, N, D]).  Right-padded prompts need no lengths: no query
-        sees a token behind it.  The own part runs the block-sparse forward, whose 16-bit O is
-        merged with the prefix's."""
+        of ``k``, ``v`` ([B, H_kv, N, D]); views welcome.  Right-padded prompts need no
+        lengths: no query sees a token behind it.  One pass over both parts."""
         self._check(q)
         B, H, N, D = q.shape
         if tuple(k.shape) != (B, self.heads, N, D) or k.shape != v.shape:
@@ -125,24 +133,18 @@ class SharedPrefix:
             raise ValueError("window_size must be at least 1: a query sees its own token")
         no_gradients(k, v)
         scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
-        if not 0 < scale <= 1e30:
-            raise ValueError("softmax_scale must be positive and finite")
-        tcore = stk._uses_tensor_cores(self.dtype, D)
-        q, k, v = (stk._readable(t, tcore) for t in (q, k, v))
-        o = torch.empty((B, H, N, D), dtype=self.dtype, device=self.device)
-        lse = torch.empty((B, H, N), dtype=torch.float32, device=self.device)
-        with native.device_guard(self.device):
-            bm = _PROMPT_BLOCK
-            mask = stk.make_streaming_mask(N, N, stk.StreamingMaskSpec(0, window_size), bm, bm,
-                                           self.device)
-            tm, tn = native.plan_tiles(0, self.dtype, D, N)
-            plan = stk.build_plan(mask, N, N, bm, bm, tm, tn)
-            native.check(native.lib().sbfa_fwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), B, H, N,
-                N, D, native.dtype_code(self.dtype), scale, 1, 0, window_size, mask.data_ptr(),
-                bm, bm, plan["row_ptr"].data_ptr(), plan["col_idx"].data_ptr(),
-                stk._stride_array(q, k, v, o), self.heads, native.stream_ptr(self.device)), "fwd")
-        o, lse = self.join(q, scale, o, lse, OWN_16)
+        q, k, v = vector_readable(q), tma_readable(k), tma_readable(v)
+        dev = self.device
+        o = torch.empty((B, H, N, D), dtype=self.dtype, device=dev)
+        lse = torch.empty((B, H, N), dtype=torch.float32, device=dev) if return_lse else None
+        with native.device_guard(dev):
+            ws, ws_bytes = self._workspace(B, H, N, window_size)
+            strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *stk._strides3(k), *stk._strides3(v))
+            native.check(native.lib().sbfa_prefix_prompt(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, self.k.data_ptr(),
+                self.v.data_ptr(), o.data_ptr(), native.ptr(lse), B, H, self.heads, N,
+                self.length, D, self._code, scale, window_size, native.ptr(ws), ws_bytes,
+                native.stream_ptr(dev)), "prefix_prompt")
         return (o, lse) if return_lse else o
 
 

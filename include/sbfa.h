@@ -374,9 +374,20 @@ int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const void* k_pr
                        int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim, int dtype,
                        double softmax_scale, void* ws, int64_t ws_bytes, void* stream);
 
-/* Scratch bytes sbfa_prefix_attend needs for this shape, 0 for a bad one. */
+/* The batch's own prompts behind the prefix, in one pass: query i of a sequence sees
+ * the whole prefix and its sequence's tokens (i - window, i] of k, v (logical [B,
+ * kv_heads, n_q, head_dim]); window >= 1.  strides: (batch, head, row) of q, k, v, or NULL
+ * for contiguous tensors; those of k and v are positive.  The rest as above. */
+int sbfa_prefix_prompt(const void* q, const void* k, const void* v, const int64_t* strides,
+                       const void* k_prefix, const void* v_prefix, void* o, float* lse,
+                       int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P,
+                       int64_t head_dim, int dtype, double softmax_scale, int64_t window,
+                       void* ws, int64_t ws_bytes, void* stream);
+
+/* Scratch bytes sbfa_prefix_attend (window = 0) or sbfa_prefix_prompt needs for this shape
+ * on the current device (may be 0; ws may then be NULL), -1 for a bad shape. */
 int64_t sbfa_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q,
-                                    int64_t P, int64_t head_dim);
+                                    int64_t P, int64_t head_dim, int64_t window);
 
 /* sbfa_decode without any device allocation by anyone.  No counterpart in
  * the upstream project, which has no decode entry point at all.

@@ -110,7 +110,10 @@ def test_decode_behind_a_prefix_with_the_16_bit_cache(dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("B,Hkv,G,N,P,D,W", [
     (2, 2, 4, 100, 300, 128, 16), (1, 1, 1, 1, 1, 64, 1), (2, 1, 3, 33, 77, 80, 1000),
-    (1, 2, 2, 300, 129, 64, 128)])
+    (1, 2, 2, 300, 129, 64, 128),
+    (37, 1, 2, 5, 200, 64, 3), (150, 2, 1, 1, 10, 128, 7), (9, 1, 5, 64, 128, 40, 20),
+    (3, 1, 7, 65, 64, 96, 65), (2, 2, 1, 513, 5, 128, 200), (1, 1, 2, 700, 1500, 64, 701),
+    (5, 1, 1, 129, 1000, 128, 129), (6, 1, 3, 8, 9000, 128, 8)])
 def test_prompts_behind_a_prefix(dtype, B, Hkv, G, N, P, D, W):
     g = gen(25)
     pre = make(g, Hkv, P, D, dtype)
@@ -127,8 +130,7 @@ def test_prompts_behind_a_prefix(dtype, B, Hkv, G, N, P, D, W):
             x = (q[b, h].double() @ kk.T / math.sqrt(D)).masked_fill(~seen, -math.inf)
             w = torch.softmax(x, -1)
             ds = (q[b, h].double().abs() @ kk.abs().T).amax(-1) / math.sqrt(D) * D * 2.0 ** -23
-            # both parts round their weights, the own part its result as well
-            ref.check(o[b, h], w @ vv, w @ vv.abs(), ds, u, 2 * u)
+            ref.check(o[b, h], w @ vv, w @ vv.abs(), ds, u, u)
             ref.check_lse(lse[b, h], torch.logsumexp(x, -1), ds)
     assert native.device_status() == 0
 
@@ -208,6 +210,11 @@ def test_prefix_copies_only_what_it_must():
     assert torch.equal(pre.attend(q), pre.attend(odd))
     wide = q[:, :1].expand(1, 2, 3, 64)
     assert torch.equal(pre.attend(wide), pre.attend(wide.contiguous()))
+    kv = rows(g, (1, 1, 3, 64), torch.float16).expand(1, 2, 3, 64)   # a stride of zero
+    oddk = torch.empty(kv.numel() + 1, dtype=kv.dtype, device=DEV)[1:].view(kv.shape)
+    oddk.copy_(kv)
+    want = pre.attend_prompt(q, kv.contiguous(), kv.contiguous(), 2)
+    assert torch.equal(want, pre.attend_prompt(odd, kv, oddk, 2))
 
 
 def test_refusals():
@@ -222,7 +229,6 @@ def test_refusals():
                 lambda: pre.attend_prompt(q, k, k[:, :, :2], 4),
                 lambda: pre.attend_prompt(q, k, k, 0),
                 lambda: pre.attend_prompt(q, k.bfloat16(), k.bfloat16(), 4),
-                lambda: pre.attend_prompt(q, k, k, 4, softmax_scale=0.0),
                 lambda: SharedPrefix(k[0], k[0].bfloat16()),
                 lambda: SharedPrefix(k[0].float(), k[0].float()),
                 lambda: SharedPrefix(k[0][..., :60], k[0][..., :60])):
@@ -230,6 +236,8 @@ def test_refusals():
             bad()
     with pytest.raises(RuntimeError, match="softmax_scale"):
         pre.attend(q, softmax_scale=-1.0)
+    with pytest.raises(RuntimeError, match="softmax_scale"):
+        pre.attend_prompt(q, k, k, 4, softmax_scale=0.0)
     with pytest.raises(RuntimeError, match="gradients"):
         pre.attend(q.clone().requires_grad_(True))
     f32 = StreamingKVCache(1, 2, 64, 0, 8, dtype=torch.float32, device=DEV)

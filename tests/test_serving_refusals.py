@@ -73,8 +73,8 @@ def prefix(L, q=P, k=P, own=None, own_lse=None, kind=0, B=2, H=4, hkv=2, n=1, le
     (dict(length=1 << 31), INVALID, "positive"), (dict(scale=0.0), INVALID, "softmax_scale"),
     (dict(q=None), INVALID, "NULL"), (dict(kind=1), INVALID, "own"),
     (dict(kind=3), INVALID, "own"), (dict(kind=2, own=P), INVALID, "own"),
-    (dict(k=P + 8), INVALID, "aligned"), (dict(ws=None), INVALID, "workspace"),
-    (dict(ws_bytes=16), INVALID, "workspace"), (dict(strides=(64, 64, 4)), INVALID, "strides"),
+    (dict(k=P + 8), INVALID, "aligned"), (dict(ws=None, length=9000), INVALID, "workspace"),
+    (dict(ws_bytes=16, length=9000), INVALID, "workspace"), (dict(strides=(64, 64, 4)), INVALID, "strides"),
     (dict(strides=(64, -8, 8)), INVALID, "strides"),
 ])
 def test_prefix_refuses(kw, rc, word):
@@ -85,10 +85,28 @@ def test_sizes():
     L = native.lib()
     assert [L.sbfa_qcache_row_bytes(d) for d in (0, 8, 64, 72, 128, 136, 256, 264, 60)] == \
         [0, 64, 64, 128, 128, 256, 256, 0, 0]
-    assert L.sbfa_prefix_workspace_bytes(2, 4, 2, 1, 100, 64) >= 2 * 4 * (64 * 4 + 8)
-    for bad in ((0, 4, 2, 1, 100, 64), (2, 4, 3, 1, 100, 64), (2, 4, 2, 1, 0, 64),
-                (2, 4, 2, 1, 100, 256)):
-        assert L.sbfa_prefix_workspace_bytes(*bad) == 0
+    # one key tile is never cut; a long prefix before few rows is
+    assert L.sbfa_prefix_workspace_bytes(2, 4, 2, 1, 100, 64, 0) == 0
+    assert L.sbfa_prefix_workspace_bytes(2, 4, 2, 1, 9000, 64, 0) >= 2 * 2 * 256 * (64 * 4 + 8)
+    for bad in ((0, 4, 2, 1, 100, 64, 0), (2, 4, 3, 1, 100, 64, 0), (2, 4, 2, 1, 0, 64, 0),
+                (2, 4, 2, 1, 100, 256, 0), (2, 4, 2, 1, 100, 64, -1)):
+        assert L.sbfa_prefix_workspace_bytes(*bad) == -1
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(window=0), "window"), (dict(k=None), "NULL"), (dict(k=P + 8), "k and v"),
+    (dict(strides=(64,) * 3 + (64, 0, 64) + (64,) * 3), "k and v"),
+    (dict(strides=(64,) * 3 + (64,) * 3 + (64, 64, 12)), "k and v"),
+    (dict(strides=(64, 64, -8) + (64,) * 6), "strides"), (dict(n=0), "positive"),
+    (dict(length=9000, ws=None), "workspace"),
+])
+def test_prompt_refuses(kw, word):
+    a = dict(k=P, window=4, strides=None, n=3, length=100, ws=P) | kw
+    st = None if a["strides"] is None else (ctypes.c_int64 * 9)(*a["strides"])
+    rc = native.lib().sbfa_prefix_prompt(P, a["k"], P, st, P, P, P, None, 2, 4, 2, a["n"],
+                                         a["length"], 64, native.BF16, 0.1, a["window"], a["ws"],
+                                         1 << 40, None)
+    assert rc == INVALID and word in native.last_error()
 
 
 def test_python_refusals():
