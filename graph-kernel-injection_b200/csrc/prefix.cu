@@ -32,11 +32,10 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "quant_cache.cuh"
 #include "tc_attn_common.cuh"
 
 namespace sbfa {
-
-int device_sm_count();
 
 namespace {
 
@@ -55,9 +54,9 @@ constexpr float kRescaleLog2 = 8.0f;
 constexpr uint32_t kTmemCols = 512;
 
 struct PrefixGeom {
-  int64_t rows;        // R, rows per key/value head
   int64_t sb, sh, sn;  // q strides (batch, head, query)
-  int64_t P;
+  int rows;            // R, rows per key/value head (below 2^31 - 256)
+  int P;
   int group, n_q, kv_heads, batch, d;
   int pairs;           // 256-row tiles per key/value head
   int n_full, n_tail;  // units (tile, head) that take all keys / that are cut into slices
@@ -67,6 +66,8 @@ struct PrefixGeom {
   int window, box;     // their window; rows of a TMA box of own keys (128 / box sequences a tile)
 };
 
+// How a row's attention to its own tokens comes from a cache's kernel: O of the output type (every
+// row saw a key), or fp32 with LSE -inf for a row that saw none.
 enum OwnKind { kOwnNone = 0, kOwn16 = 1, kOwn32 = 2 };
 
 // Where O goes and what a cache's kernel contributes to it.
@@ -81,10 +82,10 @@ struct PrefixOut {
 };
 
 // Row of O for row `row` of a key/value head.
-__device__ __forceinline__ int64_t out_row(const PrefixGeom& g, int kvh, int64_t row) {
-  const int64_t per = (int64_t)g.group * g.n_q;
-  const int64_t b = row / per;
-  return (b * g.kv_heads + kvh) * per + (row - b * per);
+__device__ __forceinline__ int64_t out_row(const PrefixGeom& g, int kvh, int row) {
+  const int per = g.group * g.n_q;
+  const int b = row / per;
+  return ((int64_t)b * g.kv_heads + kvh) * per + (row - b * per);
 }
 
 // The own-key tiles that rows [row0, row1) need, in order: sequence by sequence (box == 128;
@@ -93,12 +94,13 @@ struct OwnTiles {
   int b0, kt0, c0;   // first sequence (or block), its first tile and tiles
   int full;          // tiles of a whole sequence
   int count;
-  __device__ __forceinline__ OwnTiles(const PrefixGeom& g, int64_t row0, int64_t row1) {
-    const int64_t per = (int64_t)g.group * g.n_q;
-    b0 = (int)(row0 / per);
-    const int b1 = (int)((row1 - 1) / per);
-    kt0 = 0;
+  __device__ __forceinline__ OwnTiles(const PrefixGeom& g, int row0, int row1) {
+    b0 = kt0 = c0 = count = 0;
     full = 1;
+    if (!g.own) return;
+    const int per = g.group * g.n_q;
+    b0 = row0 / per;
+    const int b1 = (row1 - 1) / per;
     if (g.box < kTN) {
       const int seqs = kTN / g.box;
       b0 /= seqs;
@@ -107,17 +109,16 @@ struct OwnTiles {
       return;
     }
     full = (g.n_q + kTN - 1) / kTN;
-    // queries [lo, hi] of a run of rows: of several heads, all of them
-    const int64_t lo = row0 - b0 * per, hi = min(row1 - b0 * per, per) - 1;
+    // queries [q_lo, q_hi] of a run of rows: of several heads, all of them
+    const int lo = row0 - b0 * per, hi = min(row1 - b0 * per, per) - 1;
     const bool one = lo / g.n_q == hi / g.n_q;
-    const int q_lo = one ? (int)(lo % g.n_q) : 0, q_hi = one ? (int)(hi % g.n_q) : g.n_q - 1;
-    kt0 = (int)max((int64_t)0, (int64_t)q_lo - g.window + 1) / kTN;
+    const int q_lo = one ? lo % g.n_q : 0, q_hi = one ? hi % g.n_q : g.n_q - 1;
+    kt0 = max(0, q_lo - g.window + 1) / kTN;
     c0 = q_hi / kTN - kt0 + 1;
     count = c0;
     if (b1 > b0) {
-      const int64_t last = row1 - 1 - b1 * per;
-      const int l_hi = last < g.n_q ? (int)last : g.n_q - 1;
-      count += (b1 - b0 - 1) * full + l_hi / kTN + 1;
+      const int last = row1 - 1 - b1 * per;
+      count += (b1 - b0 - 1) * full + (last < g.n_q ? last : g.n_q - 1) / kTN + 1;
     }
   }
   // own tile u: sequence (or block of them) and its key tile
@@ -180,9 +181,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int splits = sliced ? geo.splits : 1;
   const int unit = sliced ? geo.n_full + tail : bid;
   const int kvh = unit / geo.pairs;
-  const int64_t row0 = (int64_t)(unit % geo.pairs) * kPair * kTM;
+  const int row0 = unit % geo.pairs * (kPair * kTM);
   const int nx = row0 + kTM < geo.rows ? 2 : 1;  // tiles with rows in them
-  OwnTiles own = OwnTiles(geo, row0, min(row0 + kPair * kTM, geo.rows));
+  const OwnTiles own(geo, row0, min(row0 + kPair * kTM, geo.rows));
   const int n_all = geo.n_tiles + (geo.own ? own.count : 0);
   // slices of n_all / splits tiles, none empty (splits <= n_tiles)
   const int t0 = (int)((int64_t)split * n_all / splits);
@@ -333,30 +334,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (x < nx) {
       const int quarter = warp & 3;
       const int r = quarter * 32 + lane;
-      const int64_t row = row0 + x * kTM + r;
+      const int row = row0 + x * kTM + r;
       const bool live = row < geo.rows;
       const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
       const uint32_t t_sx = tmem + lane_base + 128u * x;
       const uint32_t t_o = tmem + lane_base + 256u + 128u * x;
-      const int64_t per = (int64_t)geo.group * geo.n_q;
-      const int64_t seq = row / per;
-      const int iq = (int)((row - seq * per) % geo.n_q);   // the row's query of its sequence
-      {  // gather this thread's query row; columns behind d and rows behind R are zero
-        const int64_t hg = (row - seq * per) / geo.n_q;
-        const T* src = q + seq * geo.sb + (kvh * (int64_t)geo.group + hg) * geo.sh + iq * geo.sn;
+      const int per = geo.group * geo.n_q;
+      const int seq = row / per;
+      const int hg = (row - seq * per) / geo.n_q;
+      const int iq = row - seq * per - hg * geo.n_q;   // the row's query of its sequence
+      {  // gather this warp's query rows, D / 8 lanes a row; columns behind d and rows behind
+         // R are zero.  (A row per lane would touch 32 lines with every load: 1.5 us more.)
+        const T* mine = live ? q + seq * geo.sb + ((int64_t)kvh * geo.group + hg) * geo.sh +
+                                   iq * geo.sn
+                             : nullptr;
         const uint32_t tile = sb + L::Q + (uint32_t)x * L::kTile;
-        uint4 w[D / 8];
+        constexpr int kChunks = D / 8;
+        uint4 w[kChunks];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          w[c] = live && 8 * c < geo.d ? __ldg(reinterpret_cast<const uint4*>(src) + c)
-                                       : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kChunks; ++i) {
+          const int rr = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
+          const T* src = (const T*)__shfl_sync(0xffffffffu, (unsigned long long)mine, rr);
+          w[i] = src != nullptr && 8 * c < geo.d ? __ldg(reinterpret_cast<const uint4*>(src) + c)
+                                                 : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c)
+        for (int i = 0; i < kChunks; ++i) {
+          const int rr = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
                            tile + (uint32_t)(c >> 3) * 16384u +
-                           sw128_offset((uint32_t)r, 8u * (uint32_t)(c & 7))),
-                       "r"(w[c].x), "r"(w[c].y), "r"(w[c].z), "r"(w[c].w)
+                           sw128_offset((uint32_t)(quarter * 32 + rr), 8u * (uint32_t)(c & 7))),
+                       "r"(w[i].x), "r"(w[i].y), "r"(w[i].z), "r"(w[i].w)
                        : "memory");
+        }
         fence_proxy_async_smem();
         mbar_arrive(bar(L::kQFull));
       }
@@ -373,13 +383,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!all_vis) {
           int lo = 0, hi;
           if (t < geo.n_tiles) {
-            hi = (int)(geo.P - (int64_t)t * kTN);
+            hi = geo.P - t * kTN;
           } else {
             int b, kt;
             own.at(t - geo.n_tiles, &b, &kt);
             const int seqs = kTN / geo.box;
-            const int64_t s = seq - (int64_t)b * seqs;     // this row's sequence in the tile
-            const int off = (int)s * geo.box - kt * kTN;
+            const int s = seq - b * seqs;                  // this row's sequence in the tile
+            const int off = s * geo.box - kt * kTN;
             lo = off + max(iq - geo.window + 1, 0);
             hi = live && s >= 0 && s < seqs ? off + iq + 1 : 0;
           }
@@ -482,6 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(bar(L::kPFull + 2 * x + h));
       }
       if (ok) ok = wait_bar_w(bar(L::kOFull + x), 0, abort_flag, status);
+      griddep_wait();   // the cache's kernel before this one, if any
       if (ok) {
         tc_fence_after();
         // A row's 2 D bytes pass through this warp's part of the Q tile, which is no
@@ -565,6 +576,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  // complete only after the kernel before this one, so that the merge, which waits for this
+  // one, sees both
+  griddep_wait();
+  griddep_launch();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -586,57 +601,68 @@ __global__ void __launch_bounds__(kMergeThreads)
   const int lane = threadIdx.x % kLanes;
   const int64_t all = (int64_t)geo.n_tail * (kPair * kTM);
   const int64_t at = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
-  if (at >= all) return;
   const int unit = geo.n_full + (int)(at / (kPair * kTM));
-  const int64_t row = (int64_t)(unit % geo.pairs) * (kPair * kTM) + at % (kPair * kTM);
-  if (row >= geo.rows) return;
-  const int64_t out = out_row(geo, unit / geo.pairs, row);
-  const float* part = po.part;
-  const float2* stats = po.stats;
-  const int own_kind = po.own_kind;
-  const void* own_o = po.own_o;
-  const float* own_lse = po.own_lse;
-  T* o = (T*)po.o;
-  float* lse = po.lse;
+  const int row = unit % geo.pairs * (kPair * kTM) + (int)(at % (kPair * kTM));
+  griddep_wait();
+  const bool live = at < all && row < geo.rows;   // uniform over a row's lanes
+  const int64_t out = live ? out_row(geo, unit / geo.pairs, row) : 0;
   const bool on = lane * 4 < geo.d;
-  const float own_l2 =
-      own_kind == kOwnNone ? -INFINITY : own_lse[out] * kLog2e;   // log2 of the own weight
+  const float own_l2 = live && po.own_kind != kOwnNone ? po.own_lse[out] * kLog2e : -INFINITY;
+  // every slice's m and l at once, a lane each (at most 64 slices, 16 or 32 lanes)
+  float2 st[64 / kLanes];
   float M = own_l2;
-  for (int s = 0; s < geo.splits; ++s) M = fmaxf(M, stats[s * all + at].x);
+#pragma unroll
+  for (int i = 0; i < 64 / kLanes; ++i) {
+    const int s = i * kLanes + lane;
+    st[i] = live && s < geo.splits ? po.stats[s * all + at] : make_float2(-INFINITY, 0.f);
+    M = fmaxf(M, st[i].x);
+  }
+#pragma unroll
+  for (int d = kLanes / 2; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
   const float ref = M == -INFINITY ? 0.f : M;
   float l = 0.f;
+  float w[64 / kLanes];
+#pragma unroll
+  for (int i = 0; i < 64 / kLanes; ++i) {
+    w[i] = ex2(st[i].x - ref);
+    l += st[i].y * w[i];
+  }
+#pragma unroll
+  for (int d = kLanes / 2; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  const float f_own = own_l2 == -INFINITY ? 0.f : ex2(own_l2 - ref);
+  l += f_own;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < geo.splits; ++s) {
-    const float2 st = stats[s * all + at];
-    const float f = ex2(st.x - ref);
-    const float4 p = *reinterpret_cast<const float4*>(part + (s * all + at) * D + lane * 4);
-    l += st.y * f;
+  const float* src = po.part + (live ? at : 0) * D + lane * 4;
+  auto add = [&](float4 p, float f) {
     a.x += p.x * f;
     a.y += p.y * f;
     a.z += p.z * f;
     a.w += p.w * f;
-  }
-  if (own_kind != kOwnNone && on && own_l2 != -INFINITY) {
-    const float f = ex2(own_l2 - ref);
+  };
+#pragma unroll
+  for (int i = 0; i < 64 / kLanes; ++i)
+#pragma unroll 8
+    for (int j = 0; j < kLanes; ++j) {
+      if (i * kLanes + j >= geo.splits) break;
+      add(*reinterpret_cast<const float4*>(src + (i * kLanes + j) * all * D),
+          __shfl_sync(0xffffffffu, w[i], j, kLanes));
+    }
+  if (!live || !on) return;
+  if (f_own != 0.f) {
     float4 p;
-    if (own_kind == kOwn32) {
-      p = *reinterpret_cast<const float4*>((const float*)own_o + out * geo.d + lane * 4);
+    if (po.own_kind == kOwn32) {
+      p = *reinterpret_cast<const float4*>((const float*)po.own_o + out * geo.d + lane * 4);
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>((const T*)own_o + out * geo.d + lane * 4);
-      const T* e = reinterpret_cast<const T*>(&w);
+      const uint2 x = *reinterpret_cast<const uint2*>((const T*)po.own_o + out * geo.d + lane * 4);
+      const T* e = reinterpret_cast<const T*>(&x);
       p = make_float4(Elem<T>::to(e[0]), Elem<T>::to(e[1]), Elem<T>::to(e[2]), Elem<T>::to(e[3]));
     }
-    l += f;
-    a.x += p.x * f;
-    a.y += p.y * f;
-    a.z += p.z * f;
-    a.w += p.w * f;
+    add(p, f_own);
   }
-  if (!on) return;
   const float inv = 1.f / l;
-  *reinterpret_cast<uint2*>(o + out * geo.d + lane * 4) =
+  *reinterpret_cast<uint2*>((T*)po.o + out * geo.d + lane * 4) =
       make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-  if (lane == 0 && lse) lse[out] = (ref + log2f(l)) * kLn2;
+  if (lane == 0 && po.lse) po.lse[out] = (ref + log2f(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------
@@ -677,13 +703,13 @@ bool prefix_geometry(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_
     return false;
   const int64_t group = H / kv_heads;
   // rows of a key/value head, and CTAs, in 31 bits
-  if (B * group >= (1ll << 31) || B * group * n_q >= (1ll << 31)) return false;
-  geo->rows = B * group * n_q;
-  const int64_t pairs = (geo->rows + kPair * kTM - 1) / (kPair * kTM);
+  if (B * group >= (1ll << 31) || B * group * n_q >= (1ll << 31) - 512) return false;
+  geo->rows = (int)(B * group * n_q);
+  const int64_t pairs = ((int64_t)geo->rows + kPair * kTM - 1) / (kPair * kTM);
   const int64_t units = pairs * kv_heads;
   if (units >= (1ll << 30)) return false;
   geo->sb = geo->sh = geo->sn = 0;
-  geo->P = P;
+  geo->P = (int)P;
   geo->group = (int)group;
   geo->n_q = (int)n_q;
   geo->kv_heads = (int)kv_heads;
@@ -727,8 +753,27 @@ struct PrefixCall {
   PrefixOut out;
   float scale;
   void* ws;
+  bool chained;                 // the kernel before this one is the cache's attend kernel
   cudaStream_t stream;
 };
+
+// A launch whose kernel may start before the kernel ahead of it in the stream has ended (and
+// waits for it itself).
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kern)(P...), unsigned grid, unsigned block, size_t smem,
+                         cudaStream_t s, bool early, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
 
 template <typename T, int D, int STAGES>
 int launch_prefix(const PrefixCall& c, const PrefixGeom& geo) {
@@ -736,7 +781,8 @@ int launch_prefix(const PrefixCall& c, const PrefixGeom& geo) {
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   CUtensorMap mk, mv, mok, mov;
   const uint64_t d = (uint64_t)geo.d, P = (uint64_t)geo.P, h = (uint64_t)geo.kv_heads;
-  const Strides3 st{geo.kv_heads * geo.P * geo.d, geo.P * geo.d, geo.d};
+  const int64_t head = (int64_t)geo.P * geo.d;
+  const Strides3 st{geo.kv_heads * head, head, geo.d};
   if (int rc = make_tmap_4d(&mk, c.k, kBF16, d, P, h, 1, st, kTN)) return rc;
   if (int rc = make_tmap_4d(&mv, c.v, kBF16, d, P, h, 1, st, kTN)) return rc;
   mok = mk;
@@ -750,28 +796,33 @@ int launch_prefix(const PrefixCall& c, const PrefixGeom& geo) {
   out.stats = (float2*)c.ws;   // tail_rows is a multiple of 256, so part stays aligned
   out.part = (float*)((char*)c.ws + tail_rows(geo) * (int64_t)sizeof(float2));
   auto kern = prefix_tc_kernel<T, D, STAGES>;
-  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = once_per_device(ready, [&] {
+        return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)L::kAlloc),
-                          "cudaFuncSetAttribute(prefix_tc)"))
+                          "cudaFuncSetAttribute(prefix_tc)");
+      }))
     return rc;
   {
     LaunchScope ls("prefix_tc_kernel", c.stream);
-    kern<<<(unsigned)(geo.n_full + geo.n_tail * geo.splits), kThreads, L::kAlloc, c.stream>>>(
-        (const T*)c.q, mk, mv, mok, mov, out, c.scale * kLog2e, geo, device_status_ptr());
+    if (int rc = check_cuda(
+            launch_early(kern, (unsigned)(geo.n_full + geo.n_tail * geo.splits), kThreads,
+                         L::kAlloc, c.stream, c.chained, (const T*)c.q, mk, mv, mok, mov, out,
+                         c.scale * kLog2e, geo, device_status_ptr()),
+            "prefix_tc_kernel"))
+      return rc;
   }
-  if (int rc = check_launch("prefix_tc_kernel")) return rc;
   if (geo.n_tail == 0) return SBFA_OK;
   const int64_t rows_per = kMergeThreads / (D / 4);
   const int64_t blocks = ((int64_t)geo.n_tail * kPair * kTM + rows_per - 1) / rows_per;
-  {
-    LaunchScope ls("prefix_merge_kernel", c.stream);
-    prefix_merge_kernel<T, D><<<(unsigned)blocks, kMergeThreads, 0, c.stream>>>(out, geo);
-  }
-  return check_launch("prefix_merge_kernel");
+  LaunchScope ls("prefix_merge_kernel", c.stream);
+  return check_cuda(launch_early(prefix_merge_kernel<T, D>, (unsigned)blocks, kMergeThreads, 0,
+                                 c.stream, true, out, geo),
+                    "prefix_merge_kernel");
 }
 
-// Checks what both entry points share and launches.
-int run_prefix(PrefixCall& c, const int64_t* q_strides, PrefixGeom& geo, int64_t H, int dtype,
+// Checks what the entry points share; launches behind it.
+int check_call(PrefixCall& c, const int64_t* q_strides, PrefixGeom& geo, int64_t H,
                double softmax_scale, int64_t ws_bytes) {
   if (!(softmax_scale > 0) || softmax_scale > 1e30)
     return fail(SBFA_ERR_INVALID, "softmax_scale must be positive and finite");
@@ -791,6 +842,10 @@ int run_prefix(PrefixCall& c, const int64_t* q_strides, PrefixGeom& geo, int64_t
     return fail(SBFA_ERR_INVALID, "prefix attention: workspace too small (need " +
                                       std::to_string(need) + " bytes)");
   c.scale = (float)softmax_scale;
+  return SBFA_OK;
+}
+
+int launch_call(const PrefixCall& c, const PrefixGeom& geo, int dtype) {
   if (tile_dim(geo.d) == 64)
     return dtype == SBFA_BF16 ? launch_prefix<__nv_bfloat16, 64, 8>(c, geo)
                               : launch_prefix<__half, 64, 8>(c, geo);
@@ -811,6 +866,10 @@ int check_prefix(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P,
   return SBFA_OK;
 }
 
+int64_t own_bytes(int64_t B, int64_t H, int64_t d) {
+  return (B * H * (d + 1) * (int64_t)sizeof(float) + 255) / 256 * 256;
+}
+
 }  // namespace
 }  // namespace sbfa
 
@@ -826,14 +885,14 @@ extern "C" int64_t sbfa_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_
 
 extern "C" int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const void* k_prefix,
                                   const void* v_prefix, const void* own_o, const float* own_lse,
-                                  int own_kind, void* o, float* lse, int64_t B, int64_t H,
-                                  int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim,
-                                  int dtype, double softmax_scale, void* ws, int64_t ws_bytes,
+                                  void* o, float* lse, int64_t B, int64_t H, int64_t kv_heads,
+                                  int64_t n_q, int64_t P, int64_t head_dim, int dtype,
+                                  double softmax_scale, void* ws, int64_t ws_bytes,
                                   void* stream) {
   PrefixGeom geo;
   if (int rc = check_prefix(B, H, kv_heads, n_q, P, head_dim, dtype, 0, &geo)) return rc;
-  if (own_kind < 0 || own_kind > 2 || (own_kind != 0 && (!own_o || !own_lse)))
-    return fail(SBFA_ERR_INVALID, "sbfa_prefix_attend: own_o and own_lse must match own_kind");
+  if ((own_o == nullptr) != (own_lse == nullptr))
+    return fail(SBFA_ERR_INVALID, "sbfa_prefix_attend: own_o and own_lse come together");
   PrefixCall c = {};
   c.q = q;
   c.k = k_prefix;
@@ -842,10 +901,55 @@ extern "C" int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const
   c.out.lse = lse;
   c.out.own_o = own_o;
   c.out.own_lse = own_lse;
-  c.out.own_kind = own_kind;
+  c.out.own_kind = own_o ? kOwn16 : kOwnNone;
   c.ws = ws;
   c.stream = (cudaStream_t)stream;
-  return run_prefix(c, q_strides, geo, H, dtype, softmax_scale, ws_bytes);
+  if (int rc = check_call(c, q_strides, geo, H, softmax_scale, ws_bytes)) return rc;
+  return launch_call(c, geo, dtype);
+}
+
+extern "C" int64_t sbfa_qcache_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
+                                                      int64_t P, int64_t head_dim) {
+  PrefixGeom geo;
+  if (!prefix_geometry(B, H, kv_heads, 1, P, head_dim, 0, &geo)) return -1;
+  return ws_bytes_of(geo) + own_bytes(B, H, head_dim);
+}
+
+extern "C" int sbfa_qcache_prefix_attend(
+    const void* q, const void* k_codes, const void* v_codes, const void* scales,
+    const int64_t* lengths, const void* k_prefix, const void* v_prefix, void* o, float* lse,
+    int64_t B, int64_t H, int64_t kv_heads, int64_t P, int64_t head_dim, int dtype, int fmt,
+    double softmax_scale, int64_t sink, int64_t window, void* ws, int64_t ws_bytes,
+    void* stream) {
+  PrefixGeom geo;
+  if (int rc = check_prefix(B, H, kv_heads, 1, P, head_dim, dtype, 0, &geo)) return rc;
+  const int64_t own = own_bytes(B, H, head_dim);
+  if (ws == nullptr || ws_bytes < own + ws_bytes_of(geo))
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: workspace too small (need " +
+                                      std::to_string(own + ws_bytes_of(geo)) + " bytes)");
+  // the cache's own result in fp32 [B, H, d] and its LSE [B, H], then the prefix's scratch
+  float* own_o = (float*)ws;
+  float* own_lse = own_o + B * H * head_dim;
+  const QAttend a{q, k_codes, v_codes, scales, lengths, nullptr, own_o, own_lse, B, H,
+                  geo.kv_heads, head_dim, dtype, fmt, softmax_scale, sink, window,
+                  (cudaStream_t)stream};
+  PrefixCall c = {};
+  c.q = q;
+  c.k = k_prefix;
+  c.v = v_prefix;
+  c.out.o = o;
+  c.out.lse = lse;
+  c.out.own_o = own_o;
+  c.out.own_lse = own_lse;
+  c.out.own_kind = kOwn32;
+  c.ws = (char*)ws + own;
+  c.chained = true;
+  c.stream = (cudaStream_t)stream;
+  // all checks before the first launch
+  if (int rc = qcache_attend_check(a)) return rc;
+  if (int rc = check_call(c, nullptr, geo, H, softmax_scale, ws_bytes - own)) return rc;
+  if (int rc = qcache_attend_launch(a)) return rc;
+  return launch_call(c, geo, dtype);
 }
 
 extern "C" int sbfa_prefix_prompt(const void* q, const void* k, const void* v,
@@ -876,5 +980,6 @@ extern "C" int sbfa_prefix_prompt(const void* q, const void* k, const void* v,
   c.out.lse = lse;
   c.ws = ws;
   c.stream = (cudaStream_t)stream;
-  return run_prefix(c, strides, geo, H, dtype, softmax_scale, ws_bytes);
+  if (int rc = check_call(c, strides, geo, H, softmax_scale, ws_bytes)) return rc;
+  return launch_call(c, geo, dtype);
 }

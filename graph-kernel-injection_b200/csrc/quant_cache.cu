@@ -333,9 +333,10 @@ struct AttCfg {
   static constexpr int kTiles = (DP == 256 || NQ == 2) ? 1 : 2;   // 16-row tiles per step
   static constexpr int kRowsQ = 8 * NQ;
   static constexpr int kCtas = DP == 256 ? 2 : 3;                 // aimed at per SM
-  // per warp: O [8 NQ][DP + 4]; M, m, l [8 NQ]
+  // per warp: O [8 NQ][DP + 4]; M, m, l [8 NQ]; the CTA's M, m, l
   static constexpr int kPitch = DP + 4;
-  static constexpr size_t kBytes = (size_t)kAttWarps * kRowsQ * (kPitch + 3) * sizeof(float);
+  static constexpr size_t kBytes =
+      ((size_t)kAttWarps * kRowsQ * (kPitch + 3) + 3 * kRowsQ) * sizeof(float);
 };
 
 __device__ __forceinline__ uint4 ldg16(const uint8_t* p) {
@@ -378,6 +379,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
   constexpr int NCH = DP / 64;      // 16-byte pieces of a K row per lane
   constexpr int VW = DP / 32;       // words of a V row per lane
   extern __shared__ __align__(16) float att_smem[];
+  tc::griddep_launch();   // a shared prefix's kernel reads nothing of ours before its own wait
   const int rank = blockIdx.x % ns;
   const int64_t unit = blockIdx.x / ns;
   const int64_t bh = unit / chunks;                       // (sequence, key/value head)
@@ -639,43 +641,40 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
       }
     }
   __syncthreads();
-  if (ns > 1) cg::this_cluster().sync();
-  // this CTA's share of the unit's rows, four columns per thread, over all warps of
-  // all CTAs: NaN results come through the sums, maxima ignore them
-  const int parts = kAttWarps * ns;
-  for (int idx = rank * (kAttWarps * 32) + threadIdx.x; idx < nq * (DP / 4);
-       idx += ns * kAttWarps * 32) {
-    const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
-    auto at = [&](float* p, int w) -> float* {
-      float* mine = p + (w % kAttWarps) * C::kRowsQ;
-      return ns > 1 ? cg::this_cluster().map_shared_rank(mine, w / kAttWarps) : mine;
-    };
-    float Mx = -INFINITY, mx = -INFINITY;
+  // the CTA's warps into warp 0's place (each thread its own four columns of a row); maxima
+  // ignore NaN, which comes through the sums
+  float* cM = sl + kAttWarps * C::kRowsQ;   // [row] M, m, l of the CTA
+  float* cm = cM + C::kRowsQ;
+  float* cl = cm + C::kRowsQ;
+  auto join = [&](int parts, int row, auto&& stat, auto&& vec, float& Mx, float& mx, float& L,
+                  float4& a) {
+    Mx = mx = -INFINITY;
     for (int w = 0; w < parts; ++w) {
-      Mx = fmaxf(Mx, at(sM, w)[row]);
-      mx = fmaxf(mx, at(sm, w)[row]);
+      Mx = fmaxf(Mx, *stat(0, w));
+      mx = fmaxf(mx, *stat(1, w));
     }
     const float rM = Mx == -INFINITY ? 0.f : Mx, rm = mx == -INFINITY ? 0.f : mx;
-    float L = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    L = 0.f;
+    a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int w = 0; w < parts; ++w) {
-      L += at(sl, w)[row] * ex2(at(sm, w)[row] - rm);
-      const float f = ex2(at(sM, w)[row] - rM);
-      float* mine = so + ((w % kAttWarps) * C::kRowsQ + row) * C::kPitch + col;
-      const float4 p = *reinterpret_cast<const float4*>(
-          ns > 1 ? cg::this_cluster().map_shared_rank(mine, w / kAttWarps) : mine);
+      L += *stat(2, w) * ex2(*stat(1, w) - rm);
+      const float f = ex2(*stat(0, w) - rM);
+      const float4 p = *vec(w);
       a.x += p.x * f;
       a.y += p.y * f;
       a.z += p.z * f;
       a.w += p.w * f;
     }
+  };
+  // O and LSE of a row's four columns
+  auto write = [&](int row, int col, float Mx, float mx, float L, float4 a) {
     const bool some = !(L == 0.f);
-    const float inv = some ? 1.f / L : 0.f;
-    const float back = ex2(rM - rm);
-    a.x = some ? saturated<T>(a.x * inv * back) : 0.f;
-    a.y = some ? saturated<T>(a.y * inv * back) : 0.f;
-    a.z = some ? saturated<T>(a.z * inv * back) : 0.f;
-    a.w = some ? saturated<T>(a.w * inv * back) : 0.f;
+    const float f = some ? 1.f / L : 0.f;
+    const float back = ex2((Mx == -INFINITY ? 0.f : Mx) - (mx == -INFINITY ? 0.f : mx));
+    a.x = some ? saturated<T>(a.x * f * back) : 0.f;
+    a.y = some ? saturated<T>(a.y * f * back) : 0.f;
+    a.z = some ? saturated<T>(a.z * f * back) : 0.f;
+    a.w = some ? saturated<T>(a.w * f * back) : 0.f;
     const int64_t out = qrow0 + row;
     if (col < c.d) {
       if (o32)
@@ -685,10 +684,47 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
             make_uint2(tc::pack2<T>(a.x, a.y), tc::pack2<T>(a.z, a.w));
     }
     // a partial result marks an empty row by -inf, the public one by 0
-    if (col == 0 && lse)
-      lse[out] = some ? (mx + log2f(L)) * kLn2 : (o32 ? -INFINITY : 0.f);
+    if (col == 0 && lse) lse[out] = some ? (mx + log2f(L)) * kLn2 : (o32 ? -INFINITY : 0.f);
+  };
+  for (int idx = threadIdx.x; idx < nq * (DP / 4); idx += kAttWarps * 32) {
+    const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
+    float* mine = so + row * C::kPitch + col;
+    float Mx, mx, L;
+    float4 a;
+    join(kAttWarps, row,
+         [&](int k, int w) { return sM + (k * kAttWarps + w) * C::kRowsQ + row; },
+         [&](int w) { return reinterpret_cast<float4*>(mine + w * C::kRowsQ * C::kPitch); }, Mx,
+         mx, L, a);
+    if (ns == 1) {
+      write(row, col, Mx, mx, L, a);
+    } else {
+      *reinterpret_cast<float4*>(mine) = a;
+      if (col == 0) {
+        cM[row] = Mx;
+        cm[row] = mx;
+        cl[row] = L;
+      }
+    }
   }
-  if (ns > 1) cg::this_cluster().sync();   // peers may still read this CTA's memory
+  if (ns == 1) return;
+  // the CTAs of the cluster: each takes its share of the rows' columns from all of them
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int idx = rank * (kAttWarps * 32) + threadIdx.x; idx < nq * (DP / 4);
+       idx += ns * kAttWarps * 32) {
+    const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
+    float Mx, mx, L;
+    float4 a;
+    join(ns, row,
+         [&](int k, int w) { return cluster.map_shared_rank(cM + k * C::kRowsQ + row, w); },
+         [&](int w) {
+           return reinterpret_cast<float4*>(
+               cluster.map_shared_rank(so + row * C::kPitch + col, w));
+         },
+         Mx, mx, L, a);
+    write(row, col, Mx, mx, L, a);
+  }
+  cluster.sync();   // peers may still read this CTA's memory
 }
 
 // ---------------------------------------------------------------------------
@@ -786,10 +822,14 @@ int launch_attend(const void* q, const QCache& c, const int64_t* lengths, void* 
   if (units * ns >= (1ll << 31))
     return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many (sequence, head) units");
   auto kern = qcache_attend_kernel<T, FMT, DP, NQ>;
+  static std::atomic<uint64_t> ready{0};
   if (C::kBytes > 48 * 1024)
-    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)C::kBytes),
-                            "cudaFuncSetAttribute(qcache_attend)"))
+    if (int rc = once_per_device(ready, [&] {
+          return check_cuda(
+              cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)C::kBytes),
+              "cudaFuncSetAttribute(qcache_attend)");
+        }))
       return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * ns));
@@ -880,40 +920,51 @@ extern "C" int sbfa_qcache_read(const void* k_codes, const void* v_codes, const 
   });
 }
 
-extern "C" int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
-                                  const void* scales, const int64_t* lengths, void* o,
-                                  float* o_partial, float* lse, int64_t B, int64_t H,
-                                  int64_t kv_heads, int64_t head_dim, int dtype, int fmt,
-                                  double softmax_scale, int64_t sink, int64_t window,
-                                  void* stream) {
-  if (kv_heads <= 0) kv_heads = H;
-  if (int rc = check_qcache(k_codes, v_codes, scales, lengths, B, kv_heads, head_dim, dtype, fmt,
-                            sink, window))
+namespace sbfa {
+int qcache_attend_check(const QAttend& a) {
+  if (int rc = check_qcache(a.k, a.v, a.scales, a.lengths, a.B, a.kv_heads, a.d, a.dtype, a.fmt,
+                            a.sink, a.window))
     return rc;
-  if (H <= 0 || H % kv_heads != 0)
+  if (a.H <= 0 || a.H % a.kv_heads != 0)
     return fail(SBFA_ERR_INVALID, "the query head count must be a multiple of kv_heads");
-  if (!(softmax_scale > 0) || softmax_scale > 1e30)
+  if (a.H / a.kv_heads >= (1 << 20)) return fail(SBFA_ERR_UNSUPPORTED, "too many query heads");
+  if (!(a.scale > 0) || a.scale > 1e30)
     return fail(SBFA_ERR_INVALID, "softmax_scale must be positive and finite");
-  if (!q || (!o && !o_partial) || (o_partial && !lse))
-    return fail(SBFA_ERR_INVALID, "sbfa_qcache_attend: NULL tensor pointer");
-  if (((uintptr_t)q | (uintptr_t)o | (uintptr_t)o_partial) & 15u)
-    return fail(SBFA_ERR_INVALID, "sbfa_qcache_attend: tensors must be 16-byte aligned");
-  const QCache c = make_cache(const_cast<void*>(k_codes), const_cast<void*>(v_codes),
-                              const_cast<void*>(scales), kv_heads, head_dim, sink, window);
-  cudaStream_t s = (cudaStream_t)stream;
-  const int64_t group = H / kv_heads;
-  if (group >= (1 << 20)) return fail(SBFA_ERR_UNSUPPORTED, "too many query heads");
-  return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
+  if (!a.q || (!a.o && !a.o32))
+    return fail(SBFA_ERR_INVALID, "8-bit cache: NULL query or output pointer");
+  if (((uintptr_t)a.q | (uintptr_t)a.o | (uintptr_t)a.o32) & 15u)
+    return fail(SBFA_ERR_INVALID, "8-bit cache: tensors must be 16-byte aligned");
+  return SBFA_OK;
+}
+
+int qcache_attend_launch(const QAttend& a) {
+  const QCache c = make_cache(const_cast<void*>(a.k), const_cast<void*>(a.v),
+                              const_cast<void*>(a.scales), a.kv_heads, a.d, a.sink, a.window);
+  const int group = (int)(a.H / a.kv_heads);
+  return by_format(a.dtype, a.fmt, a.d, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
     constexpr int DP = dp.value;
     // 16 query columns halve the passes over a group of more than 8; at 256
     // columns per row the second set of accumulators would not fit the registers
     if constexpr (DP <= 128) {
       if (group > 8)
-        return launch_attend<T, m.value, DP, 2>(q, c, lengths, o, o_partial, lse, B, (int)group,
-                                                (float)softmax_scale, s);
+        return launch_attend<T, m.value, DP, 2>(a.q, c, a.lengths, a.o, a.o32, a.lse, a.B, group,
+                                                (float)a.scale, a.stream);
     }
-    return launch_attend<T, m.value, DP, 1>(q, c, lengths, o, o_partial, lse, B, (int)group,
-                                            (float)softmax_scale, s);
+    return launch_attend<T, m.value, DP, 1>(a.q, c, a.lengths, a.o, a.o32, a.lse, a.B, group,
+                                            (float)a.scale, a.stream);
   });
+}
+}  // namespace sbfa
+
+extern "C" int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
+                                  const void* scales, const int64_t* lengths, void* o, float* lse,
+                                  int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim,
+                                  int dtype, int fmt, double softmax_scale, int64_t sink,
+                                  int64_t window, void* stream) {
+  const QAttend a{q,  k_codes,  v_codes,  scales, lengths, o,    nullptr, lse, B, H,
+                  kv_heads <= 0 ? H : kv_heads, head_dim, dtype, fmt, softmax_scale, sink, window,
+                  (cudaStream_t)stream};
+  if (int rc = qcache_attend_check(a)) return rc;
+  return qcache_attend_launch(a);
 }

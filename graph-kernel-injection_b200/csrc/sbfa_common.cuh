@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "sbfa.h"
@@ -192,6 +193,19 @@ __device__ __forceinline__ int32_t plan_entry(const int32_t* list, int e, int n_
 inline int ceil_div_i(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 __device__ __forceinline__ int ceil_div_dev(int a, int b) {
   return (int)(((int64_t)a + b - 1) / b);
+}
+
+// Whether a kernel's one-time set-up on the current device is still to be done; `done` is
+// that kernel's own bit per device (devices behind the 64th are set up every time).
+template <typename F>
+int once_per_device(std::atomic<uint64_t>& done, F&& set_up) {
+  int dev = 0;
+  if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return SBFA_OK;
+  if (int rc = set_up()) return rc;
+  done.fetch_or(bit, std::memory_order_release);
+  return SBFA_OK;
 }
 
 // Wraps one kernel launch: counts it, and when timing is enabled

@@ -135,6 +135,17 @@ __device__ __forceinline__ bool named_bar_and(int id, int nthreads, bool pred) {
   return r != 0;
 }
 
+// Programmatic dependent launch: the next kernel of the stream, if it was launched with the
+// programmatic attribute, may start once every CTA has called `launch`; `wait` returns when the
+// kernels before this one have completed and their writes are visible (at once for a
+// kernel launched without the attribute).
+__device__ __forceinline__ void griddep_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void griddep_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Per-warpgroup register budget changes (all 4 warps of a warpgroup execute
 // them).  The sum over the CTA must stay within what it was launched with.
 template <int N>

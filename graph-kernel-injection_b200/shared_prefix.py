@@ -17,16 +17,14 @@ sequence's own tokens follow it under the causal window rule.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
-from typing import Optional, Tuple
+from typing import Dict, Optional, Tuple
 
 import torch
 
 import sbfa_native as native
 import sparse_triton_kernel as stk
-
-# how a row's attention to its own tokens comes to the merge (sbfa_prefix_attend)
-OWN_NONE, OWN_16, OWN_32 = 0, 1, 2
 
 def no_gradients(*tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
@@ -40,6 +38,12 @@ def vector_readable(t: torch.Tensor) -> torch.Tensor:
     if st[-1] != 1 or t.data_ptr() % 16 or any(x < 0 or x % 8 for x in st[:-1]):
         return t.clone(memory_format=torch.contiguous_format)
     return t
+
+
+@functools.lru_cache(maxsize=256)
+def stride_array(strides: Tuple[int, ...]):
+    """A host array of these element strides for the C ABI, which only reads it."""
+    return (ctypes.c_int64 * len(strides))(*strides)
 
 
 def tma_readable(t: torch.Tensor) -> torch.Tensor:
@@ -69,6 +73,7 @@ class SharedPrefix:
         self.heads, self.length, self.head_dim = (int(x) for x in k.shape)
         self.dtype, self.device = k.dtype, k.device
         self._code = native.dtype_code(k.dtype)
+        self._scratch: Dict[tuple, int] = {}   # scratch bytes by a call's sizes
 
     def _check(self, q: torch.Tensor) -> None:
         if (q.dim() != 4 or 0 in q.shape or q.shape[1] % self.heads
@@ -80,39 +85,73 @@ class SharedPrefix:
         no_gradients(q)
 
     def join(self, q: torch.Tensor, scale: float, own_o: Optional[torch.Tensor],
-             own_lse: Optional[torch.Tensor], own_kind: int) -> Tuple[torch.Tensor, torch.Tensor]:
+             own_lse: Optional[torch.Tensor],
+             return_lse: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         """Attention of ``q`` ([B, H, N, D]) to the prefix, merged with its attention to its
-        sequence's own tokens (``own_o``, ``own_lse`` in the form ``own_kind``, see
-        ``sbfa_prefix_attend``): O and the natural-log LSE over both."""
+        sequence's own tokens where ``own_o``, ``own_lse`` give it (every query saw a
+        token there): O and, with ``return_lse``, the natural-log LSE over both."""
         self._check(q)
         q = vector_readable(q)
         B, H, N, D = q.shape
         dev = self.device
         o = torch.empty((B, H, N, D), dtype=self.dtype, device=dev)
-        lse = torch.empty((B, H, N), dtype=torch.float32, device=dev)
+        lse = torch.empty((B, H, N), dtype=torch.float32, device=dev) if return_lse else None
         with native.device_guard(dev):
             ws, ws_bytes = self._workspace(B, H, N, 0)
             native.check(native.lib().sbfa_prefix_attend(
-                q.data_ptr(), (ctypes.c_int64 * 3)(*q.stride()[:3]), self.k.data_ptr(),
-                self.v.data_ptr(), native.ptr(own_o), native.ptr(own_lse), own_kind,
-                o.data_ptr(), lse.data_ptr(), B, H, self.heads, N, self.length, D, self._code,
+                q.data_ptr(), stride_array(q.stride()[:3]), self.k.data_ptr(),
+                self.v.data_ptr(), native.ptr(own_o), native.ptr(own_lse),
+                o.data_ptr(), native.ptr(lse), B, H, self.heads, N, self.length, D, self._code,
                 scale, native.ptr(ws), ws_bytes, native.stream_ptr(dev)), "prefix_attend")
         return o, lse
 
     def _workspace(self, B: int, H: int, N: int, window: int):
         """Scratch of one call (from torch's allocator, so of its stream or graph) and its bytes."""
-        need = native.lib().sbfa_prefix_workspace_bytes(B, H, self.heads, N, self.length,
-                                                        self.head_dim, window)
+        need = self._scratch.get((B, H, N, window))
+        if need is None:
+            need = self._remember((B, H, N, window), native.lib().sbfa_prefix_workspace_bytes(
+                B, H, self.heads, N, self.length, self.head_dim, window))
         if need <= 0:   # none, or a bad shape that the call refuses
             return None, 0
         return torch.empty(need, dtype=torch.uint8, device=self.device), need
+
+    def _remember(self, sizes: tuple, need: int) -> int:
+        if len(self._scratch) >= 256:
+            self._scratch.clear()
+        self._scratch[sizes] = need
+        return need
+
+    def attend_cached(self, cache, q: torch.Tensor, scale: float, return_lse: bool):
+        """A decode step of a ``QuantizedStreamingKVCache`` behind this prefix (``q`` checked by the
+        cache)."""
+        if (cache.heads != self.heads or cache.head_dim != self.head_dim
+                or cache.dtype != self.dtype or cache.device != self.device):
+            raise ValueError(f"the prefix has {self.heads} heads of {self.head_dim} {self.dtype} on "
+                             f"{self.device}, the cache {cache.heads} of {cache.head_dim} "
+                             f"{cache.dtype} on {cache.device}")
+        B, H = q.shape[:2]
+        dev = self.device
+        o = torch.empty_like(q)
+        lse = torch.empty((B, H, 1), dtype=torch.float32, device=dev) if return_lse else None
+        with native.device_guard(dev):
+            need = self._scratch.get((B, H))
+            if need is None:
+                need = self._remember((B, H), native.lib().sbfa_qcache_prefix_workspace_bytes(
+                    B, H, self.heads, self.length, self.head_dim))
+            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+            native.check(native.lib().sbfa_qcache_prefix_attend(
+                q.data_ptr(), *cache._cache_ptrs, self.k.data_ptr(), self.v.data_ptr(),
+                o.data_ptr(), native.ptr(lse), B, H, self.heads, self.length, self.head_dim,
+                *cache._codes, scale, cache.sink_size, cache.window_size, ws.data_ptr(), need,
+                native.stream_ptr(dev)), "qcache_prefix_attend")
+        return (o, lse) if return_lse else o
 
     def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
                return_lse: bool = False):
         """Attention of every query ([B, H, N, D]) to the whole prefix and nothing else:
         O ([B, H, N, D]) and, with ``return_lse``, the natural-log LSE ([B, H, N] fp32)."""
         scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
-        o, lse = self.join(q, scale, None, None, OWN_NONE)
+        o, lse = self.join(q, scale, None, None, return_lse)
         return (o, lse) if return_lse else o
 
     def attend_prompt(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window_size: int,
@@ -139,7 +178,7 @@ class SharedPrefix:
         lse = torch.empty((B, H, N), dtype=torch.float32, device=dev) if return_lse else None
         with native.device_guard(dev):
             ws, ws_bytes = self._workspace(B, H, N, window_size)
-            strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *stk._strides3(k), *stk._strides3(v))
+            strides = stride_array((*q.stride()[:3], *stk._strides3(k), *stk._strides3(v)))
             native.check(native.lib().sbfa_prefix_prompt(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, self.k.data_ptr(),
                 self.v.data_ptr(), o.data_ptr(), native.ptr(lse), B, H, self.heads, N,

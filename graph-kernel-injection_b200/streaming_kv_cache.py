@@ -18,14 +18,13 @@ every sequence of the batch has before its own and that are held once.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Tuple
 
 import torch
 
 import sbfa_native as native
-from shared_prefix import OWN_16, OWN_32, SharedPrefix, no_gradients, vector_readable
+from shared_prefix import SharedPrefix, no_gradients, stride_array, vector_readable
 
 
 class StreamingKVCache:
@@ -101,7 +100,7 @@ class StreamingKVCache:
                 self._ws.numel(), native.stream_ptr(self.device)), "ring_decode")
         if prefix is not None:
             # o is rounded to its 16 bits before the merge rounds once more
-            o, lse = prefix.join(q, scale, o, lse, OWN_16)
+            o, lse = prefix.join(q, scale, o, lse, return_lse)
         return (o, lse) if return_lse else o
 
 
@@ -167,7 +166,7 @@ class QuantizedStreamingKVCache:
         return 2 * self._k.numel() + self.scales.numel()
 
     def _check(self, t: torch.Tensor, shape: Tuple[int, ...], name: str) -> None:
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
         if t.device != self.device or t.dtype != self.dtype:
             raise ValueError(f"{name} must be {self.dtype} on {self.device}")
@@ -192,7 +191,7 @@ class QuantizedStreamingKVCache:
         if n == 0:
             return
         k_new, v_new = vector_readable(k_new), vector_readable(v_new)
-        strides = (ctypes.c_int64 * 6)(*k_new.stride()[:3], *v_new.stride()[:3])
+        strides = stride_array(k_new.stride()[:3] + v_new.stride()[:3])
         k, v, scales, lengths = self._cache_ptrs
         with native.device_guard(self.device):
             native.check(native.lib().sbfa_qcache_append(
@@ -217,18 +216,16 @@ class QuantizedStreamingKVCache:
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-        o = torch.empty_like(q, dtype=torch.float32 if prefix is not None else None)
-        lse = None
-        if return_lse or prefix is not None:
-            lse = torch.empty(self.batch, hq, 1, dtype=torch.float32, device=self.device)
-        out, partial = (o.data_ptr(), None) if prefix is None else (None, o.data_ptr())
+        if prefix is not None:
+            return prefix.attend_cached(self, q, scale, return_lse)
+        o = torch.empty_like(q)
+        lse = (torch.empty(self.batch, hq, 1, dtype=torch.float32, device=self.device)
+               if return_lse else None)
         with native.device_guard(self.device):
             native.check(native.lib().sbfa_qcache_attend(
-                q.data_ptr(), *self._cache_ptrs, out, partial, native.ptr(lse), self.batch, hq,
+                q.data_ptr(), *self._cache_ptrs, o.data_ptr(), native.ptr(lse), self.batch, hq,
                 self.heads, self.head_dim, *self._codes, scale, self.sink_size,
                 self.window_size, native.stream_ptr(self.device)), "qcache_attend")
-        if prefix is not None:
-            o, lse = prefix.join(q, scale, o, lse, OWN_32)
         return (o, lse) if return_lse else o
 
     def read(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

@@ -331,13 +331,11 @@ int sbfa_qcache_append(void* k_codes, void* v_codes, void* scales, int64_t* leng
 /* Attention of each sequence's query at its last position over its visible
  * rows.  q: contiguous [B, H, head_dim], H a multiple of kv_heads (<= 0 means H);
  * o: the same shape and dtype; lse (may be NULL): fp32 [B, H].  A sequence of
- * length 0 gives O = 0 and LSE = 0.  With o_partial (fp32 [B, H, head_dim]) the
- * result goes there unrounded instead of to o, and lse is -inf for an empty
- * sequence: the form sbfa_prefix_attend merges.  softmax_scale > 0.  No workspace. */
+ * length 0 gives O = 0 and LSE = 0.  softmax_scale > 0.  No workspace. */
 int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
-                       const void* scales, const int64_t* lengths, void* o, float* o_partial,
-                       float* lse, int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim,
-                       int dtype, int fmt, double softmax_scale, int64_t sink, int64_t window,
+                       const void* scales, const int64_t* lengths, void* o, float* lse,
+                       int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim, int dtype,
+                       int fmt, double softmax_scale, int64_t sink, int64_t window,
                        void* stream);
 
 /* The kept rows as 16-bit values in order of position: out row i of a sequence
@@ -360,19 +358,32 @@ int sbfa_qcache_read(const void* k_codes, const void* v_codes, const void* scale
  * k_prefix, v_prefix: contiguous [kv_heads, P, head_dim], fp16 or bf16 like q;
  * head_dim a multiple of 8, at most 128; all 16-byte aligned, strides
  * multiples of 8 elements; softmax_scale > 0.
- * own: each query's attention over its sequence's own tokens, merged with the
- * prefix's by their log-sum-exps: own_o contiguous [B, H, n_q, head_dim] and
- * own_lse fp32 [B, H, n_q].  own_kind 0: none; 1: own_o has q's dtype and every
- * row saw a key (sbfa_ring_decode, or sbfa_fwd with a causal window >= 1); 2:
- * own_o is fp32 and own_lse = -inf marks a row that saw none (sbfa_qcache_attend's partial
- * form).
+ * own_o, own_lse (both or neither): each query's attention over its sequence's own
+ * tokens, merged with the prefix's by their log-sum-exps: contiguous [B, H, n_q,
+ * head_dim] of q's dtype and fp32 [B, H, n_q], from sbfa_ring_decode or another call in
+ * which every row saw a key.
  * o: contiguous [B, H, n_q, head_dim]; lse: fp32 [B, H, n_q] or NULL.  ws:
  * 16-byte aligned caller scratch of sbfa_prefix_workspace_bytes() bytes. */
 int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const void* k_prefix,
-                       const void* v_prefix, const void* own_o, const float* own_lse,
-                       int own_kind, void* o, float* lse, int64_t B, int64_t H,
-                       int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim, int dtype,
-                       double softmax_scale, void* ws, int64_t ws_bytes, void* stream);
+                       const void* v_prefix, const void* own_o, const float* own_lse, void* o,
+                       float* lse, int64_t B, int64_t H, int64_t kv_heads, int64_t n_q,
+                       int64_t P, int64_t head_dim, int dtype, double softmax_scale, void* ws,
+                       int64_t ws_bytes, void* stream);
+
+/* A decode step over an 8-bit cache behind a shared prefix: sbfa_qcache_attend and
+ * sbfa_prefix_attend (n_q = 1, head_dim <= 128) with one rounding at the end and their
+ * launches overlapped.  A sequence of length 0 sees the prefix alone.  ws:
+ * sbfa_qcache_prefix_workspace_bytes() bytes. */
+int sbfa_qcache_prefix_attend(const void* q, const void* k_codes, const void* v_codes,
+                              const void* scales, const int64_t* lengths, const void* k_prefix,
+                              const void* v_prefix, void* o, float* lse, int64_t B, int64_t H,
+                              int64_t kv_heads, int64_t P, int64_t head_dim, int dtype, int fmt,
+                              double softmax_scale, int64_t sink, int64_t window, void* ws,
+                              int64_t ws_bytes, void* stream);
+
+/* Scratch bytes sbfa_qcache_prefix_attend needs on the current device, -1 for a bad shape. */
+int64_t sbfa_qcache_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t P,
+                                           int64_t head_dim);
 
 /* The batch's own prompts behind the prefix, in one pass: query i of a sequence sees
  * the whole prefix and its sequence's tokens (i - window, i] of k, v (logical [B,

@@ -240,6 +240,12 @@ def test_refusals():
         pre.attend_prompt(q, k, k, 4, softmax_scale=0.0)
     with pytest.raises(RuntimeError, match="gradients"):
         pre.attend(q.clone().requires_grad_(True))
+    c = filled(g, 2, 2, 64, 0, 8, torch.bfloat16, "int8", [3, 4])
+    with pytest.raises(ValueError, match="the cache"):
+        c.attend(q[:, :, :1].bfloat16(), prefix=pre)
+    c = filled(g, 2, 1, 64, 0, 8, torch.float16, "int8", [3, 4])
+    with pytest.raises(ValueError, match="the cache"):
+        c.attend(q[:, :, :1], prefix=pre)
     f32 = StreamingKVCache(1, 2, 64, 0, 8, dtype=torch.float32, device=DEV)
     f32.append(torch.zeros(1, 2, 1, 64, device=DEV), torch.zeros(1, 2, 1, 64, device=DEV))
     with pytest.raises(ValueError, match="q must be"):

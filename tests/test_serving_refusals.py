@@ -43,26 +43,26 @@ def test_append_of_nothing_launches_nothing():
     assert append(native.lib(), n=0, new=None) == 0 and native.launch_count() == before
 
 
-def attend(L, q=P, o=P, partial=None, lse=P, B=1, H=4, hkv=2, D=64, scale=0.1, fmt=1):
-    return L.sbfa_qcache_attend(q, P, P, P, P, o, partial, lse, B, H, hkv, D, native.F16, fmt,
-                                scale, 4, 8, None)
+def attend(L, q=P, o=P, lse=P, B=1, H=4, hkv=2, D=64, scale=0.1, fmt=1):
+    return L.sbfa_qcache_attend(q, P, P, P, P, o, lse, B, H, hkv, D, native.F16, fmt, scale, 4, 8,
+                                None)
 
 
 @pytest.mark.parametrize("kw,word", [
     (dict(H=3), "multiple"), (dict(H=0), "multiple"), (dict(scale=0.0), "softmax_scale"),
     (dict(scale=-1.0), "softmax_scale"), (dict(scale=float("nan")), "softmax_scale"),
     (dict(scale=float("inf")), "softmax_scale"), (dict(q=None), "NULL"), (dict(o=None), "NULL"),
-    (dict(o=None, partial=P, lse=None), "NULL"), (dict(q=P + 8), "aligned"),
+    (dict(q=P + 8), "aligned"),
     (dict(o=P + 4), "aligned"),
 ])
 def test_attend_refuses(kw, word):
     assert attend(native.lib(), **kw) == INVALID and word in native.last_error()
 
 
-def prefix(L, q=P, k=P, own=None, own_lse=None, kind=0, B=2, H=4, hkv=2, n=1, length=100, D=64,
+def prefix(L, q=P, k=P, own=None, own_lse=None, B=2, H=4, hkv=2, n=1, length=100, D=64,
            dtype=native.F16, scale=0.1, ws=P, ws_bytes=1 << 40, strides=None):
     st = None if strides is None else (ctypes.c_int64 * 3)(*strides)
-    return L.sbfa_prefix_attend(q, st, k, P, own, own_lse, kind, P, P, B, H, hkv, n, length, D,
+    return L.sbfa_prefix_attend(q, st, k, P, own, own_lse, P, P, B, H, hkv, n, length, D,
                                 dtype, scale, ws, ws_bytes, None)
 
 
@@ -71,14 +71,30 @@ def prefix(L, q=P, k=P, own=None, own_lse=None, kind=0, B=2, H=4, hkv=2, n=1, le
     (dict(D=12), UNSUPPORTED, "head_dim"), (dict(H=3), INVALID, "multiple"),
     (dict(length=0), INVALID, "positive"), (dict(n=0), INVALID, "positive"),
     (dict(length=1 << 31), INVALID, "positive"), (dict(scale=0.0), INVALID, "softmax_scale"),
-    (dict(q=None), INVALID, "NULL"), (dict(kind=1), INVALID, "own"),
-    (dict(kind=3), INVALID, "own"), (dict(kind=2, own=P), INVALID, "own"),
+    (dict(q=None), INVALID, "NULL"), (dict(own=P), INVALID, "own"),
+    (dict(own_lse=P), INVALID, "own"),
     (dict(k=P + 8), INVALID, "aligned"), (dict(ws=None, length=9000), INVALID, "workspace"),
     (dict(ws_bytes=16, length=9000), INVALID, "workspace"), (dict(strides=(64, 64, 4)), INVALID, "strides"),
     (dict(strides=(64, -8, 8)), INVALID, "strides"),
 ])
 def test_prefix_refuses(kw, rc, word):
     assert prefix(native.lib(), **kw) == rc and word in native.last_error()
+
+
+@pytest.mark.parametrize("kw,rc,word", [
+    (dict(D=136), UNSUPPORTED, "head_dim"), (dict(dtype=native.F32), UNSUPPORTED, "float16"),
+    (dict(fmt=7), INVALID, "format"), (dict(H=3), INVALID, "multiple"),
+    (dict(length=0), INVALID, "positive"), (dict(ws=None), INVALID, "workspace"),
+    (dict(ws_bytes=256), INVALID, "workspace"), (dict(k=None), INVALID, "NULL"),
+    (dict(q=P + 8), INVALID, "aligned"), (dict(scale=0.0), INVALID, "softmax_scale"),
+])
+def test_decode_behind_a_prefix_refuses(kw, rc, word):
+    a = dict(q=P, k=P, H=4, length=100, D=64, dtype=native.F16, fmt=0, scale=0.1, ws=P,
+             ws_bytes=1 << 40) | kw
+    got = native.lib().sbfa_qcache_prefix_attend(
+        a["q"], P, P, P, P, a["k"], P, P, None, 2, a["H"], 2, a["length"], a["D"], a["dtype"],
+        a["fmt"], a["scale"], 4, 8, a["ws"], a["ws_bytes"], None)
+    assert got == rc and word in native.last_error()
 
 
 def test_sizes():
@@ -91,6 +107,8 @@ def test_sizes():
     for bad in ((0, 4, 2, 1, 100, 64, 0), (2, 4, 3, 1, 100, 64, 0), (2, 4, 2, 1, 0, 64, 0),
                 (2, 4, 2, 1, 100, 256, 0), (2, 4, 2, 1, 100, 64, -1)):
         assert L.sbfa_prefix_workspace_bytes(*bad) == -1
+    assert L.sbfa_qcache_prefix_workspace_bytes(2, 4, 2, 100, 64) >= 2 * 4 * 65 * 4
+    assert L.sbfa_qcache_prefix_workspace_bytes(2, 3, 2, 100, 64) == -1
 
 
 @pytest.mark.parametrize("kw,word", [
