@@ -757,24 +757,6 @@ struct PrefixCall {
   cudaStream_t stream;
 };
 
-// A launch whose kernel may start before the kernel ahead of it in the stream has ended (and
-// waits for it itself).
-template <typename... P, typename... A>
-cudaError_t launch_early(void (*kern)(P...), unsigned grid, unsigned block, size_t smem,
-                         cudaStream_t s, bool early, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = early ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
-}
-
 template <typename T, int D, int STAGES>
 int launch_prefix(const PrefixCall& c, const PrefixGeom& geo) {
   using L = PrefixLayout<D, STAGES>;
@@ -866,8 +848,9 @@ int check_prefix(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P,
   return SBFA_OK;
 }
 
+int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 int64_t own_bytes(int64_t B, int64_t H, int64_t d) {
-  return (B * H * (d + 1) * (int64_t)sizeof(float) + 255) / 256 * 256;
+  return align256(B * H * (d + 1) * (int64_t)sizeof(float));
 }
 
 }  // namespace
@@ -909,10 +892,14 @@ extern "C" int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const
 }
 
 extern "C" int64_t sbfa_qcache_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
-                                                      int64_t P, int64_t head_dim) {
+                                                      int64_t P, int64_t head_dim, int64_t sink,
+                                                      int64_t window) {
+  const int64_t rows = sink + window;
   PrefixGeom geo;
   if (!prefix_geometry(B, H, kv_heads, 1, P, head_dim, 0, &geo)) return -1;
-  return ws_bytes_of(geo) + own_bytes(B, H, head_dim);
+  const int64_t cache = qcache_attend_ws_bytes(B, H, geo.kv_heads, head_dim, rows);
+  if (cache < 0) return -1;
+  return ws_bytes_of(geo) + own_bytes(B, H, head_dim) + align256(cache);
 }
 
 extern "C" int sbfa_qcache_prefix_attend(
@@ -923,16 +910,19 @@ extern "C" int sbfa_qcache_prefix_attend(
     void* stream) {
   PrefixGeom geo;
   if (int rc = check_prefix(B, H, kv_heads, 1, P, head_dim, dtype, 0, &geo)) return rc;
-  const int64_t own = own_bytes(B, H, head_dim);
-  if (ws == nullptr || ws_bytes < own + ws_bytes_of(geo))
+  const int64_t need =
+      sbfa_qcache_prefix_workspace_bytes(B, H, kv_heads, P, head_dim, sink, window);
+  if (need < 0) return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: bad sizes");
+  if (ws == nullptr || ws_bytes < need)
     return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: workspace too small (need " +
-                                      std::to_string(own + ws_bytes_of(geo)) + " bytes)");
-  // the cache's own result in fp32 [B, H, d] and its LSE [B, H], then the prefix's scratch
+                                      std::to_string(need) + " bytes)");
+  // the cache's own result in fp32 [B, H, d] and its LSE [B, H], the prefix's scratch, the cache's
+  const int64_t own = own_bytes(B, H, head_dim), pre = ws_bytes_of(geo);
   float* own_o = (float*)ws;
   float* own_lse = own_o + B * H * head_dim;
   const QAttend a{q, k_codes, v_codes, scales, lengths, nullptr, own_o, own_lse, B, H,
                   geo.kv_heads, head_dim, dtype, fmt, softmax_scale, sink, window,
-                  (cudaStream_t)stream};
+                  (char*)ws + own + pre, need - own - pre, (cudaStream_t)stream};
   PrefixCall c = {};
   c.q = q;
   c.k = k_prefix;
@@ -947,7 +937,7 @@ extern "C" int sbfa_qcache_prefix_attend(
   c.stream = (cudaStream_t)stream;
   // all checks before the first launch
   if (int rc = qcache_attend_check(a)) return rc;
-  if (int rc = check_call(c, nullptr, geo, H, softmax_scale, ws_bytes - own)) return rc;
+  if (int rc = check_call(c, nullptr, geo, H, softmax_scale, pre)) return rc;
   if (int rc = qcache_attend_launch(a)) return rc;
   return launch_call(c, geo, dtype);
 }

@@ -321,18 +321,27 @@ __global__ void __launch_bounds__(kReadThreads)
 // acc / l * 2^(M - m).  Q is scaled by a power of two into fp16's range, which is exact
 // for fp16 inputs and for bf16 down to 2^-38 of the row's largest element.
 //
-// A cluster of NS CTAs shares one unit (sequence, head, group of queries); its warps
-// take every (4 NS)-th step of KS rows, so that any length splits evenly without being
-// known to the host.  Warps merge through shared memory, CTAs through distributed
-// shared memory: no workspace and no second launch.
+// Two ways to spread the units (sequence, key/value head, group of queries) over the GPU:
+//  - few units: a cluster of NS CTAs shares one, its warps take every (4 NS)-th step of KS
+//    rows, warps merge through shared memory and CTAs through distributed shared
+//    memory: one launch, no workspace;
+//  - many: as many CTAs as fit on the SMs each take an equal run of the steps of all units in order
+//    (FLAT), whatever the lengths.  The lengths are only known here, so every CTA sums them
+//    up.  A warp fetches its first step of the next unit before the merge of this one, so that
+//    loads stay in flight across units.  A unit that crosses from one CTA to the next leaves
+//    partial rows that qcache_join_kernel merges, in order.
 constexpr int kAttWarps = 4;
 constexpr float kSlack = 4.f;
 
+// Resident CTAs per SM that the registers are limited for.  At two sets of query columns steps of 32 rows
+// on two CTAs beat steps of 16 on three (64 x 8 heads of 12 queries x 2052 rows: 72 against 84 us).
+constexpr int att_ctas(int dp, int nq) { return dp == 256 || nq == 2 ? 2 : 3; }
+
 template <int DP, int NQ>
 struct AttCfg {
-  static constexpr int kTiles = (DP == 256 || NQ == 2) ? 1 : 2;   // 16-row tiles per step
+  static constexpr int kTiles = DP == 256 ? 1 : 2;   // 16-row tiles per step
   static constexpr int kRowsQ = 8 * NQ;
-  static constexpr int kCtas = DP == 256 ? 2 : 3;                 // aimed at per SM
+  static constexpr int kCtas = att_ctas(DP, NQ);
   // per warp: O [8 NQ][DP + 4]; M, m, l [8 NQ]; the CTA's M, m, l
   static constexpr int kPitch = DP + 4;
   static constexpr size_t kBytes =
@@ -369,28 +378,285 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   return r;
 }
 
-template <typename T, int FMT, int DP, int NQ>
+// One row's four columns from `parts` partial results: stat(0 | 1 | 2, w) gives M, m, l of part
+// w, vec(w) its columns.  Maxima ignore NaN, which comes through the sums.
+template <typename S, typename V>
+__device__ __forceinline__ void att_join(int parts, S&& stat, V&& vec, float& Mx, float& mx,
+                                         float& L, float4& a) {
+  Mx = mx = -INFINITY;
+  for (int w = 0; w < parts; ++w) {
+    Mx = fmaxf(Mx, stat(0, w));
+    mx = fmaxf(mx, stat(1, w));
+  }
+  const float rM = Mx == -INFINITY ? 0.f : Mx, rm = mx == -INFINITY ? 0.f : mx;
+  L = 0.f;
+  a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int w = 0; w < parts; ++w) {
+    L += stat(2, w) * ex2(stat(1, w) - rm);
+    const float f = ex2(stat(0, w) - rM);
+    const float4 p = vec(w);
+    a.x += p.x * f;
+    a.y += p.y * f;
+    a.z += p.z * f;
+    a.w += p.w * f;
+  }
+}
+
+// O (rounded, or fp32 to o32) and LSE of four columns of row `out`.
+template <typename T>
+__device__ __forceinline__ void att_write(T* o, float* o32, float* lse, int64_t out, int d, int col,
+                                          float Mx, float mx, float L, float4 a) {
+  const bool some = !(L == 0.f);
+  const float f = some ? 1.f / L : 0.f;
+  const float back = ex2((Mx == -INFINITY ? 0.f : Mx) - (mx == -INFINITY ? 0.f : mx));
+  a.x = some ? saturated<T>(a.x * f * back) : 0.f;
+  a.y = some ? saturated<T>(a.y * f * back) : 0.f;
+  a.z = some ? saturated<T>(a.z * f * back) : 0.f;
+  a.w = some ? saturated<T>(a.w * f * back) : 0.f;
+  if (col < d) {
+    if (o32)
+      *reinterpret_cast<float4*>(o32 + out * d + col) = a;
+    else
+      *reinterpret_cast<uint2*>(o + out * d + col) =
+          make_uint2(tc::pack2<T>(a.x, a.y), tc::pack2<T>(a.z, a.w));
+  }
+  // a partial result marks an empty row by -inf, the public one by 0
+  if (col == 0 && lse) lse[out] = some ? (mx + log2f(L)) * kLn2 : (o32 ? -INFINITY : 0.f);
+}
+
+// What a CTA of the FLAT form writes for the merge: the unit that its first run ends, if that began
+// in an earlier CTA.
+struct FlatRecord {
+  int64_t unit_start;   // cost of all units before it, -1: nothing to merge
+  int64_t total;        // cost of all units
+  int64_t row;          // first row of o
+  int nq;
+};
+struct FlatWs {
+  FlatRecord* rec;      // [CTAs]
+  float* stats;         // [CTAs][2][3][8 NQ] M, m, l
+  float* part;          // [CTAs][2][8 NQ][DP]
+};
+// where the run of CTA i of n begins, in cost from the first unit's start
+__device__ __forceinline__ int64_t flat_start(int64_t total, int i, int n) {
+  return (int64_t)((uint64_t)total * (uint32_t)i / (uint32_t)n);
+}
+
+// A unit costs its steps and about kRunSteps more (its queries, merge and output, and latency that
+// one warp step cannot hide): with 2, 4, 8 a ragged batch of 64 x 8 heads of 12 queries takes 106, 90, 66 us.
+// Runs are equal in this cost; one that begins in the surplus begins with the next unit.
+constexpr int kRunSteps = 8;
+
+// A run of steps [s0, s1) of one unit.
+struct AttRun {
+  int b, hc;            // sequence; (key/value head, group of queries) of it
+  int n, steps;         // visible rows and steps of the unit
+  int s0, s1;
+  int64_t row0;         // first cache row of the unit
+};
+
+template <typename T, int FMT, int DP, int NQ, bool FLAT>
 __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     qcache_attend_kernel(const T* __restrict__ q, QCache c, const int64_t* __restrict__ lengths,
                          T* __restrict__ o, float* __restrict__ o32, float* __restrict__ lse,
-                         float scale_log2, int group, int chunks, int ns) {
+                         float scale_log2, int group, int chunks, int ns, int batch, FlatWs ws) {
   using C = AttCfg<DP, NQ>;
   constexpr int KT = C::kTiles, KS = 16 * KT;
   constexpr int NCH = DP / 64;      // 16-byte pieces of a K row per lane
   constexpr int VW = DP / 32;       // words of a V row per lane
   extern __shared__ __align__(16) float att_smem[];
   tc::griddep_launch();   // a shared prefix's kernel reads nothing of ours before its own wait
-  const int rank = blockIdx.x % ns;
-  const int64_t unit = blockIdx.x / ns;
-  const int64_t bh = unit / chunks;                       // (sequence, key/value head)
-  const int h0 = (int)(unit % chunks) * C::kRowsQ;        // first head of the group
-  const int nq = min(C::kRowsQ, group - h0);
-  const int b = (int)(bh / c.heads);
-  const int64_t qrow0 = bh * group + h0;                  // row of q, o, lse
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, cc = lane & 3;
-  const int64_t len = lengths[b];
-  const int n = (int)min(max(len, (int64_t)0), c.rows);
+  const int hcs = (int)c.heads * chunks;
+  auto visible = [&](int b) { return (int)min(max(lengths[b], (int64_t)0), c.rows); };
+  // the FLAT form gives an empty sequence a step as well: someone has to write its zeros
+  auto steps_of = [&](int n) { return FLAT ? max(1, (n + KS - 1) / KS) : (n + KS - 1) / KS; };
+  auto cost_of = [&](int n) { return (int64_t)(steps_of(n) + kRunSteps); };
+
+  AttRun cur;
+  int64_t left = 0;       // cost that this CTA takes behind the current unit
+  int stride, rank = 0;
+  if constexpr (FLAT) {
+    __shared__ int64_t scan[kAttWarps];
+    __shared__ int first[2];
+    // cost of each thread's share of the sequences, and of all before it
+    const int per = (batch + kAttWarps * 32 - 1) / (kAttWarps * 32);
+    const int b_lo = min((int)threadIdx.x * per, batch), b_hi = min(b_lo + per, batch);
+    int64_t mine = 0;
+    for (int b = b_lo; b < b_hi; ++b) mine += cost_of(visible(b));
+    int64_t incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(kFull, incl, d);
+      if (lane >= d) incl += up;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kAttWarps; ++w) {
+      if (w < warp) incl += scan[w];
+      total += scan[w];
+    }
+    total *= hcs;
+    const int64_t begin = flat_start(total, blockIdx.x, gridDim.x);
+    const int64_t end = flat_start(total, blockIdx.x + 1, gridDim.x);
+    // the sequence in which `begin` falls, and its place there
+    __shared__ int64_t inside;
+    if (begin >= (incl - mine) * hcs && begin < incl * hcs) {
+      int64_t rem = begin - (incl - mine) * hcs;
+      int b = b_lo, n = visible(b);
+      for (; rem >= cost_of(n) * hcs; n = visible(++b)) rem -= cost_of(n) * hcs;
+      first[0] = b;
+      first[1] = n;
+      inside = rem;
+    }
+    if (threadIdx.x == 0) ws.rec[blockIdx.x].unit_start = -1;
+    if (begin == end) return;                      // a few short units, more CTAs
+    __syncthreads();
+    cur.b = first[0];
+    cur.n = first[1];
+    cur.steps = steps_of(cur.n);
+    const int64_t cost = cost_of(cur.n);
+    cur.hc = (int)(inside / cost);
+    const int64_t at = inside - cur.hc * cost;     // place of `begin` in its unit
+    cur.s0 = (int)min(at, (int64_t)cur.steps);
+    cur.s1 = (int)min((int64_t)cur.steps, at + (end - begin));
+    left = max((int64_t)0, end - begin - (cost - at));
+    const int64_t unit_start = begin - at;
+    if (cur.s0 >= cur.s1) {                        // nothing of that unit: begin with the next
+      if (left == 0) return;
+      if (++cur.hc == hcs) {
+        cur.hc = 0;
+        cur.n = visible(++cur.b);
+        cur.steps = steps_of(cur.n);
+      }
+      cur.s0 = 0;
+      cur.s1 = (int)min((int64_t)cur.steps, left);
+      left = max((int64_t)0, left - cost_of(cur.n));
+    }
+    stride = kAttWarps;
+    if (threadIdx.x == 0 && cur.s0 > 0 && cur.s1 == cur.steps) {
+      FlatRecord r;
+      r.unit_start = unit_start;
+      r.total = total;
+      r.row = ((int64_t)cur.b * c.heads + cur.hc / chunks) * group + cur.hc % chunks * C::kRowsQ;
+      r.nq = min(C::kRowsQ, group - cur.hc % chunks * C::kRowsQ);
+      ws.rec[blockIdx.x] = r;
+    }
+  } else {
+    rank = blockIdx.x % ns;
+    const int unit = blockIdx.x / ns;
+    cur.b = unit / hcs;
+    cur.hc = unit % hcs;
+    cur.n = visible(cur.b);
+    cur.steps = steps_of(cur.n);
+    cur.s0 = rank * kAttWarps;
+    cur.s1 = cur.steps;
+    stride = ns * kAttWarps;
+  }
+
+  uint4 kr[KT][2][NCH];
+  uint32_t vr[KT][4][VW];
+  uint32_t sc[KT][2], sc_next[KT][2];
+  // Rows of step s of a run.  A full step's addresses are one base and constants; in a unit's last
+  // step rows behind the last visible one read that one again.
+  auto load_k = [&](const AttRun& r, int s) {
+    const uint8_t* kb = c.k + r.row0 * DP + cc * 16;
+    const uint16_t* sb = c.scales + r.row0;
+    if ((s + 1) * KS <= r.n) {
+      const int64_t row = s * KS + g;
+      kb += row * DP;
+      sb += row;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int j = 0; j < NCH; ++j) kr[t][i][j] = ldg16(kb + (t * 16 + i * 8) * DP + j * 64);
+          sc_next[t][i] = ldg2(sb + t * 16 + i * 8);
+        }
+    } else {
+      const int last = max(r.n - 1, 0);
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int64_t row = min(s * KS + t * 16 + i * 8 + g, last);
+#pragma unroll
+          for (int j = 0; j < NCH; ++j) kr[t][i][j] = ldg16(kb + row * DP + j * 64);
+          sc_next[t][i] = ldg2(sb + row);
+        }
+    }
+  };
+  auto load_vrow = [&](uint32_t (&w)[VW], const uint8_t* p) {
+    if constexpr (DP == 64) {
+      const uint2 x = ldg8(p);
+      w[0] = x.x;
+      w[1] = x.y;
+    } else {
+#pragma unroll
+      for (int j = 0; j < VW / 4; ++j) {
+        const uint4 x = ldg16(p + j * 128);
+        w[4 * j] = x.x;
+        w[4 * j + 1] = x.y;
+        w[4 * j + 2] = x.z;
+        w[4 * j + 3] = x.w;
+      }
+    }
+  };
+  auto load_v = [&](const AttRun& r, int s) {
+    const uint8_t* vb = c.v + r.row0 * DP + g * (DP == 64 ? 8 : 16);
+    if ((s + 1) * KS <= r.n) {
+      vb += (int64_t)(s * KS + 2 * cc) * DP;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          load_vrow(vr[t][i], vb + (t * 16 + (i >> 1) * 8 + (i & 1)) * DP);
+    } else {
+      const int last = max(r.n - 1, 0);
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = s * KS + t * 16 + (i >> 1) * 8 + 2 * cc + (i & 1);
+          load_vrow(vr[t][i], vb + (int64_t)min(row, last) * DP);
+        }
+    }
+  };
+
+  auto first_row = [&](const AttRun& r) {
+    return ((int64_t)r.b * c.heads + r.hc / chunks) * c.rows;
+  };
+  cur.row0 = first_row(cur);
+  int s = cur.s0 + warp;
+  if (s < cur.s1) {
+    load_k(cur, s);
+    load_v(cur, s);
+  }
+  for (;;) {
+  // the run behind this one, which starts its unit
+  AttRun nxt = cur;
+  const bool has_next = FLAT && left > 0;
+  if (has_next) {
+    nxt.hc = cur.hc + 1;
+    if (nxt.hc == hcs) {
+      nxt.hc = 0;
+      nxt.b = cur.b + 1;
+      nxt.n = visible(nxt.b);
+      nxt.steps = steps_of(nxt.n);
+    }
+    nxt.row0 = first_row(nxt);
+    nxt.s0 = 0;
+    nxt.s1 = (int)min((int64_t)nxt.steps, left);
+    left = max((int64_t)0, left - cost_of(nxt.n));
+  }
+  const int h0 = cur.hc % chunks * C::kRowsQ;             // first head of the group
+  const int nq = min(C::kRowsQ, group - h0);
+  const int64_t qrow0 = ((int64_t)cur.b * c.heads + cur.hc / chunks) * group + h0;
+  const int n = cur.n;
 
   // Q fragments, column g of each n-tile, scaled into fp16's range
   uint32_t qf[NQ][DP / 16][2];
@@ -439,51 +705,6 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     qs[t][1] = __shfl_sync(kFull, f_out, (2 * cc + 1) * 4);
   }
 
-  const uint8_t* kb = c.k + bh * c.rows * DP;
-  const uint8_t* vb = c.v + bh * c.rows * DP;
-  const uint16_t* sb = c.scales + bh * c.rows;
-  const int steps = (n + KS - 1) / KS;
-  const int stride = ns * kAttWarps;
-
-  uint4 kr[KT][2][NCH];
-  uint32_t vr[KT][4][VW];
-  uint32_t sc[KT][2], sc_next[KT][2];
-  auto load_k = [&](int s) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = min(s * KS + t * 16 + i * 8 + g, n - 1);
-        const uint8_t* p = kb + (int64_t)row * DP + cc * 16;
-#pragma unroll
-        for (int j = 0; j < NCH; ++j) kr[t][i][j] = ldg16(p + j * 64);
-        sc_next[t][i] = ldg2(sb + row);
-      }
-  };
-  auto load_v = [&](int s) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = min(s * KS + t * 16 + (i >> 1) * 8 + 2 * cc + (i & 1), n - 1);
-        const uint8_t* p = vb + (int64_t)row * DP;
-        if constexpr (DP == 64) {
-          const uint2 w = ldg8(p + g * 8);
-          vr[t][i][0] = w.x;
-          vr[t][i][1] = w.y;
-        } else {
-#pragma unroll
-          for (int j = 0; j < VW / 4; ++j) {
-            const uint4 w = ldg16(p + j * 128 + g * 16);
-            vr[t][i][4 * j] = w.x;
-            vr[t][i][4 * j + 1] = w.y;
-            vr[t][i][4 * j + 2] = w.z;
-            vr[t][i][4 * j + 3] = w.w;
-          }
-        }
-      }
-  };
-
   float acc[NQ][2 * VW][4];
   float M[NQ][2], m[NQ][2], l[NQ][2];
 #pragma unroll
@@ -494,13 +715,11 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     l[t][0] = l[t][1] = 0.f;
   }
 
-  int s = rank * kAttWarps + warp;
-  if (s < steps) {
-    load_k(s);
-    load_v(s);
-  }
-  for (; s < steps; s += stride) {
-    const bool more = s + stride < steps;
+  // whether the loads of this warp's first step in the next run are under way
+  const bool into = has_next && warp < nxt.s1;
+  bool ahead = false;
+  for (; s < cur.s1; s += stride) {
+    const bool more = s + stride < cur.s1;
     // S^T, one 16-row tile of keys by 8 query columns each
     float x[NQ][KT][4];
 #pragma unroll
@@ -524,26 +743,48 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
         }
       }
     }
-    if (more) load_k(s + stride);
+    if (more) {
+      load_k(cur, s + stride);
+    } else if (into) {
+      load_k(nxt, warp);
+    }
+    // the scale of the keys' scores and the exponent of their values' (NaN for a bad row)
+    float ks[KT][2], ev[KT][2];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t vbyte = sc[t][i] >> 8;
+        ks[t][i] = scale_value(sc[t][i] & 255u);
+        ev[t][i] = vbyte == kBadRow ? __uint_as_float(0x7fc00000u) : (float)((int)vbyte - 127);
+      }
+    const bool edge = (s + 1) * KS > n;
     // online softmax; element e of a tile is key g + 8 (e / 2), query 2 cc + e % 2
     uint32_t pb[NQ][KT][2];
 #pragma unroll
     for (int u = 0; u < NQ; ++u) {
       float y[KT][4];
-      float mx[2] = {-INFINITY, -INFINITY}, my[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = s * KS + t * 16 + (e >> 1) * 8 + g;
-          const uint32_t sv = sc[t][e >> 1] >> 8;
-          const float ev = sv == kBadRow ? __uint_as_float(0x7fc00000u) : (float)((int)sv - 127);
-          const float xs = x[u][t][e] * (scale_value(sc[t][e >> 1] & 255u) * qs[u][e & 1]);
-          const bool in = key < n;
-          x[u][t][e] = in ? xs : -INFINITY;
-          y[t][e] = in ? xs + ev : -INFINITY;
-          mx[e & 1] = fmaxf(mx[e & 1], x[u][t][e]);
-          my[e & 1] = fmaxf(my[e & 1], y[t][e]);
+          x[u][t][e] *= ks[t][e >> 1] * qs[u][e & 1];
+          y[t][e] = x[u][t][e] + ev[t][e >> 1];
+        }
+      if (edge) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (s * KS + t * 16 + (e >> 1) * 8 + g >= n) x[u][t][e] = y[t][e] = -INFINITY;
+      }
+      float mx[2] = {-INFINITY, -INFINITY}, my[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mx[i] = tc::max3f(mx[i], x[u][t][i], x[u][t][2 + i]);
+          my[i] = tc::max3f(my[i], y[t][i], y[t][2 + i]);
         }
       bool grow = false;
       float old[2];
@@ -604,7 +845,16 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
             mma_f16(acc[u][2 * w + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[u][t][0],
                     pb[u][t][1]);
       }
-    if (more) load_v(s + stride);
+    if (more) {
+      load_v(cur, s + stride);
+    } else if (into) {
+      load_v(nxt, warp);
+      ahead = true;
+    }
+  }
+  if (into && !ahead) {   // a warp without a step in this run
+    load_k(nxt, warp);
+    load_v(nxt, warp);
   }
 
   // ---- merge: lanes, then warps, then the CTAs of the cluster
@@ -646,57 +896,31 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
   float* cM = sl + kAttWarps * C::kRowsQ;   // [row] M, m, l of the CTA
   float* cm = cM + C::kRowsQ;
   float* cl = cm + C::kRowsQ;
-  auto join = [&](int parts, int row, auto&& stat, auto&& vec, float& Mx, float& mx, float& L,
-                  float4& a) {
-    Mx = mx = -INFINITY;
-    for (int w = 0; w < parts; ++w) {
-      Mx = fmaxf(Mx, *stat(0, w));
-      mx = fmaxf(mx, *stat(1, w));
-    }
-    const float rM = Mx == -INFINITY ? 0.f : Mx, rm = mx == -INFINITY ? 0.f : mx;
-    L = 0.f;
-    a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < parts; ++w) {
-      L += *stat(2, w) * ex2(*stat(1, w) - rm);
-      const float f = ex2(*stat(0, w) - rM);
-      const float4 p = *vec(w);
-      a.x += p.x * f;
-      a.y += p.y * f;
-      a.z += p.z * f;
-      a.w += p.w * f;
-    }
-  };
-  // O and LSE of a row's four columns
   auto write = [&](int row, int col, float Mx, float mx, float L, float4 a) {
-    const bool some = !(L == 0.f);
-    const float f = some ? 1.f / L : 0.f;
-    const float back = ex2((Mx == -INFINITY ? 0.f : Mx) - (mx == -INFINITY ? 0.f : mx));
-    a.x = some ? saturated<T>(a.x * f * back) : 0.f;
-    a.y = some ? saturated<T>(a.y * f * back) : 0.f;
-    a.z = some ? saturated<T>(a.z * f * back) : 0.f;
-    a.w = some ? saturated<T>(a.w * f * back) : 0.f;
-    const int64_t out = qrow0 + row;
-    if (col < c.d) {
-      if (o32)
-        *reinterpret_cast<float4*>(o32 + out * c.d + col) = a;
-      else
-        *reinterpret_cast<uint2*>(o + out * c.d + col) =
-            make_uint2(tc::pack2<T>(a.x, a.y), tc::pack2<T>(a.z, a.w));
-    }
-    // a partial result marks an empty row by -inf, the public one by 0
-    if (col == 0 && lse) lse[out] = some ? (mx + log2f(L)) * kLn2 : (o32 ? -INFINITY : 0.f);
+    att_write<T>(o, o32, lse, qrow0 + row, c.d, col, Mx, mx, L, a);
   };
   for (int idx = threadIdx.x; idx < nq * (DP / 4); idx += kAttWarps * 32) {
     const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
     float* mine = so + row * C::kPitch + col;
     float Mx, mx, L;
     float4 a;
-    join(kAttWarps, row,
-         [&](int k, int w) { return sM + (k * kAttWarps + w) * C::kRowsQ + row; },
-         [&](int w) { return reinterpret_cast<float4*>(mine + w * C::kRowsQ * C::kPitch); }, Mx,
-         mx, L, a);
-    if (ns == 1) {
+    att_join(kAttWarps,
+             [&](int k, int w) { return sM[(k * kAttWarps + w) * C::kRowsQ + row]; },
+             [&](int w) { return *reinterpret_cast<float4*>(mine + w * C::kRowsQ * C::kPitch); },
+             Mx, mx, L, a);
+    const bool whole = FLAT ? cur.s0 == 0 && cur.s1 == cur.steps : ns == 1;
+    if (whole) {
       write(row, col, Mx, mx, L, a);
+    } else if constexpr (FLAT) {
+      // the end of a unit (slot 0), or its beginning (slot 1)
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (cur.s0 > 0 ? 0 : 1);
+      *reinterpret_cast<float4*>(ws.part + (slot * C::kRowsQ + row) * DP + col) = a;
+      if (col == 0) {
+        float* st = ws.stats + slot * 3 * C::kRowsQ + row;
+        st[0] = Mx;
+        st[C::kRowsQ] = mx;
+        st[2 * C::kRowsQ] = L;
+      }
     } else {
       *reinterpret_cast<float4*>(mine) = a;
       if (col == 0) {
@@ -706,25 +930,119 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
       }
     }
   }
-  if (ns == 1) return;
-  // the CTAs of the cluster: each takes its share of the rows' columns from all of them
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
-  for (int idx = rank * (kAttWarps * 32) + threadIdx.x; idx < nq * (DP / 4);
-       idx += ns * kAttWarps * 32) {
-    const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
-    float Mx, mx, L;
-    float4 a;
-    join(ns, row,
-         [&](int k, int w) { return cluster.map_shared_rank(cM + k * C::kRowsQ + row, w); },
-         [&](int w) {
-           return reinterpret_cast<float4*>(
-               cluster.map_shared_rank(so + row * C::kPitch + col, w));
-         },
-         Mx, mx, L, a);
-    write(row, col, Mx, mx, L, a);
+  if constexpr (!FLAT) {
+    if (ns == 1) return;
+    // the CTAs of the cluster: each takes its share of the rows' columns from all of them
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int idx = rank * (kAttWarps * 32) + threadIdx.x; idx < nq * (DP / 4);
+         idx += ns * kAttWarps * 32) {
+      const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
+      float Mx, mx, L;
+      float4 a;
+      att_join(ns,
+               [&](int k, int w) { return *cluster.map_shared_rank(cM + k * C::kRowsQ + row, w); },
+               [&](int w) {
+                 return *reinterpret_cast<float4*>(
+                     cluster.map_shared_rank(so + row * C::kPitch + col, w));
+               },
+               Mx, mx, L, a);
+      write(row, col, Mx, mx, L, a);
+    }
+    cluster.sync();   // peers may still read this CTA's memory
+    return;
   }
-  cluster.sync();   // peers may still read this CTA's memory
+  if (!has_next) return;
+  __syncthreads();    // the merge has read what the next run's will overwrite
+  cur = nxt;
+  s = warp;
+  }
+}
+
+// Joins the partial rows of the units that cross CTAs of the FLAT form: block i those of the unit
+// that ends in CTA i, from the CTA in which it began.  kJoinWarps / rows warps share a row's parts
+// (a long sequence among short ones may have hundreds), then the row's first warp joins theirs.
+constexpr int kJoinWarps = 16;
+
+template <typename T, int DP, int NQ>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    qcache_join_kernel(T* __restrict__ o, float* __restrict__ o32, float* __restrict__ lse, int d,
+                       int ctas, FlatWs ws) {
+  using C = AttCfg<DP, NQ>;
+  constexpr int VEC = DP / 32;   // columns of a lane
+  __shared__ float so[kJoinWarps][DP];
+  __shared__ float st[3][kJoinWarps];
+  tc::griddep_launch();
+  tc::griddep_wait();
+  const FlatRecord r = ws.rec[blockIdx.x];
+  if (r.unit_start < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int last = blockIdx.x;
+  // the last CTA whose run does not begin behind the unit
+  int j0 = (int)((uint64_t)r.unit_start * (uint32_t)ctas / (uint64_t)r.total);
+  while (j0 + 1 < ctas && flat_start(r.total, j0 + 1, ctas) <= r.unit_start) ++j0;
+  while (j0 > 0 && flat_start(r.total, j0, ctas) > r.unit_start) --j0;
+  // the CTAs between the two are whole inside the unit; where there are more CTAs than cost,
+  // some of them had nothing and left nothing
+  const int parts = last - j0 + 1;
+  auto slot = [&](int w) { return w == 0 ? 2 * (int64_t)j0 + 1 : 2 * (int64_t)(j0 + w); };
+  int share = kJoinWarps;        // warps of a row
+  while (share * r.nq > kJoinWarps) share >>= 1;
+  const int row = warp / share, part0 = warp % share;
+  float Mx = -INFINITY, mx = -INFINITY, L = 0.f;
+  float a[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) a[i] = 0.f;
+  // (M, m, l, columns) of another part joined to (Mx, mx, L, a)
+  auto add = [&](float M2, float m2, float l2, const float* v) {
+    const float Mn = fmaxf(Mx, M2), mn = fmaxf(mx, m2);
+    const float rM = Mn == -INFINITY ? 0.f : Mn, rm = mn == -INFINITY ? 0.f : mn;
+    L = L * ex2(mx - rm) + l2 * ex2(m2 - rm);
+    const float f1 = ex2(Mx - rM), f2 = ex2(M2 - rM);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) a[i] = a[i] * f1 + v[i] * f2;
+    Mx = Mn;
+    mx = mn;
+  };
+  if (row < r.nq) {
+#pragma unroll 4
+    for (int w = part0; w < parts; w += share) {
+      if (r.total < ctas &&
+          flat_start(r.total, j0 + w, ctas) == flat_start(r.total, j0 + w + 1, ctas))
+        continue;
+      const float* p = ws.stats + slot(w) * 3 * C::kRowsQ + row;
+      const float* src = ws.part + (slot(w) * C::kRowsQ + row) * DP + lane * VEC;
+      float v[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2)
+        *reinterpret_cast<float2*>(v + i) = *reinterpret_cast<const float2*>(src + i);
+      add(p[0], p[C::kRowsQ], p[2 * C::kRowsQ], v);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) so[warp][lane * VEC + i] = a[i];
+    if (lane == 0) {
+      st[0][warp] = Mx;
+      st[1][warp] = mx;
+      st[2][warp] = L;
+    }
+  }
+  __syncthreads();
+  if (row >= r.nq || part0 != 0) return;
+  for (int w = warp + 1; w < warp + min(share, parts); ++w)
+    add(st[0][w], st[1][w], st[2][w], &so[w][lane * VEC]);
+#pragma unroll
+  for (int i = 0; i < VEC; i += 4) {
+    const int col = lane * VEC + i;
+    if constexpr (VEC >= 4) {
+      att_write<T>(o, o32, lse, r.row + row, d, col, Mx, mx, L,
+                   make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]));
+    } else {   // two columns a lane: even lanes write their neighbour's as well
+      const float2 up = make_float2(__shfl_down_sync(kFull, a[0], 1), __shfl_down_sync(kFull, a[1], 1));
+      if (lane % 2 == 0)
+        att_write<T>(o, o32, lse, r.row + row, d, col, Mx, mx, L,
+                     make_float4(a[0], a[1], up.x, up.y));
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -804,24 +1122,47 @@ int row_grid(int64_t B, int64_t H, int64_t rows, int per_cta, int unroll, int re
   return SBFA_OK;
 }
 
-// CTAs per unit of the attend kernel (a cluster, so a power of two up to 8).
-// More of them shorten a unit, which pays while there are SMs to fill.
-int attend_splits(int64_t units, int64_t rows, int slots) {
-  int ns = 1;
-  while (ns < 8 && units * ns * 2 <= slots && rows > (int64_t)ns * 128) ns *= 2;
-  return ns;
+// How a call's units are spread over the GPU.
+struct AttPlan {
+  int nq;               // groups of 8 query heads per CTA
+  int chunks;           // groups of 8 nq heads in a key/value head's group
+  bool flat;
+  int grid, ns;         // CTAs; CTAs of a cluster
+  int64_t ws_bytes;
+};
+int attend_plan(int64_t B, int64_t kv_heads, int64_t group, int64_t d, int64_t rows, AttPlan* p) {
+  const int dp = padded_dim(d);
+  // 16 query columns halve the passes over a group of more than 8; at 256 columns per row
+  // the second set of accumulators would not fit the registers
+  p->nq = dp <= 128 && group > 8 ? 2 : 1;
+  const int rows_q = 8 * p->nq;
+  p->chunks = (int)((group + rows_q - 1) / rows_q);
+  const int64_t units = B * kv_heads * p->chunks;
+  if (units >= (1ll << 27) || kv_heads * p->chunks >= (1ll << 27))
+    return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many (sequence, head) units");
+  const int64_t slots = (int64_t)device_sm_count() * att_ctas(dp, p->nq);
+  // A cluster shortens a unit while there are SMs to fill.
+  p->ns = 1;
+  while (p->ns < 8 && units * p->ns * 2 <= slots && rows > (int64_t)p->ns * 128) p->ns *= 2;
+  // What its last, partly filled wave costs in rows of a CTA beyond an equal share; the FLAT form's
+  // scan and second kernel cost 4 to 5 us, about what 960 rows of 128 bytes take.  64 x 8 heads x
+  // 2048 rows (two waves) 62 -> 52 us, 8 x 8 x 16384 60 -> 51; 64 x 8 x 256 would go from 12 to 17,
+  // 16 x 8 x 2048 from 19 to 22.
+  const int64_t waves = (units * p->ns + slots - 1) / slots;
+  const int64_t lost = waves * rows / p->ns - units * rows / slots;
+  p->flat = lost * dp > 960 * 128;
+  p->grid = p->flat ? (int)slots : (int)(units * p->ns);
+  if (p->flat) p->ns = 1;
+  p->ws_bytes = p->flat ? slots * ((int64_t)sizeof(FlatRecord) +
+                                   2 * rows_q * (dp + 3) * (int64_t)sizeof(float))
+                        : 0;
+  return SBFA_OK;
 }
 
-template <typename T, int FMT, int DP, int NQ>
-int launch_attend(const void* q, const QCache& c, const int64_t* lengths, void* o, float* o32,
-                  float* lse, int64_t B, int group, float scale, cudaStream_t s) {
+template <typename T, int FMT, int DP, int NQ, bool FLAT>
+int launch_attend(const QAttend& a, const QCache& c, const AttPlan& p) {
   using C = AttCfg<DP, NQ>;
-  const int chunks = (group + C::kRowsQ - 1) / C::kRowsQ;
-  const int64_t units = B * c.heads * chunks;
-  const int ns = attend_splits(units, c.rows, device_sm_count() * C::kCtas);
-  if (units * ns >= (1ll << 31))
-    return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many (sequence, head) units");
-  auto kern = qcache_attend_kernel<T, FMT, DP, NQ>;
+  auto kern = qcache_attend_kernel<T, FMT, DP, NQ, FLAT>;
   static std::atomic<uint64_t> ready{0};
   if (C::kBytes > 48 * 1024)
     if (int rc = once_per_device(ready, [&] {
@@ -831,21 +1172,37 @@ int launch_attend(const void* q, const QCache& c, const int64_t* lengths, void* 
               "cudaFuncSetAttribute(qcache_attend)");
         }))
       return rc;
+  FlatWs ws = {};
+  ws.rec = (FlatRecord*)a.ws;
+  ws.stats = (float*)(ws.rec + p.grid);
+  ws.part = ws.stats + (int64_t)p.grid * 2 * 3 * C::kRowsQ;
+  const int group = (int)(a.H / a.kv_heads);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * ns));
+  cfg.gridDim = dim3((unsigned)p.grid);
   cfg.blockDim = dim3(kAttWarps * 32);
   cfg.dynamicSmemBytes = C::kBytes;
-  cfg.stream = s;
+  cfg.stream = a.stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)ns;
+  at[0].val.clusterDim.x = (unsigned)p.ns;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  LaunchScope ls("qcache_attend_kernel", s);
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, (const T*)q, c, lengths, (T*)o, o32, lse,
-                                       scale * kLog2e, group, chunks, ns),
-                    "qcache_attend_kernel");
+  cfg.numAttrs = p.ns > 1 ? 1 : 0;
+  {
+    LaunchScope ls("qcache_attend_kernel", a.stream);
+    if (int rc = check_cuda(
+            cudaLaunchKernelEx(&cfg, kern, (const T*)a.q, c, a.lengths, (T*)a.o, a.o32, a.lse,
+                               (float)a.scale * kLog2e, group, p.chunks, p.ns, (int)a.B, ws),
+            "qcache_attend_kernel"))
+      return rc;
+  }
+  if constexpr (FLAT) {
+    LaunchScope ls("qcache_join_kernel", a.stream);
+    return check_cuda(launch_early(qcache_join_kernel<T, DP, NQ>, (unsigned)p.grid,
+                                   kJoinWarps * 32, 0, a.stream, true, (T*)a.o, a.o32, a.lse, c.d, p.grid, ws),
+                      "qcache_join_kernel");
+  }
+  return SBFA_OK;
 }
 
 }  // namespace
@@ -921,6 +1278,14 @@ extern "C" int sbfa_qcache_read(const void* k_codes, const void* v_codes, const 
 }
 
 namespace sbfa {
+int64_t qcache_attend_ws_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t d, int64_t rows) {
+  AttPlan p;
+  if (B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads != 0 || padded_dim(d) == 0 || rows <= 0 ||
+      attend_plan(B, kv_heads, H / kv_heads, d, rows, &p) != SBFA_OK)
+    return -1;
+  return p.ws_bytes;
+}
+
 int qcache_attend_check(const QAttend& a) {
   if (int rc = check_qcache(a.k, a.v, a.scales, a.lengths, a.B, a.kv_heads, a.d, a.dtype, a.fmt,
                             a.sink, a.window))
@@ -932,39 +1297,50 @@ int qcache_attend_check(const QAttend& a) {
     return fail(SBFA_ERR_INVALID, "softmax_scale must be positive and finite");
   if (!a.q || (!a.o && !a.o32))
     return fail(SBFA_ERR_INVALID, "8-bit cache: NULL query or output pointer");
-  if (((uintptr_t)a.q | (uintptr_t)a.o | (uintptr_t)a.o32) & 15u)
+  if (((uintptr_t)a.q | (uintptr_t)a.o | (uintptr_t)a.o32 | (uintptr_t)a.ws) & 15u)
     return fail(SBFA_ERR_INVALID, "8-bit cache: tensors must be 16-byte aligned");
+  AttPlan p;
+  if (int rc = attend_plan(a.B, a.kv_heads, a.H / a.kv_heads, a.d, a.sink + a.window, &p))
+    return rc;
+  if (p.ws_bytes > 0 && (a.ws == nullptr || a.ws_bytes < p.ws_bytes))
+    return fail(SBFA_ERR_INVALID, "8-bit cache: workspace too small (need " +
+                                      std::to_string(p.ws_bytes) + " bytes)");
   return SBFA_OK;
 }
 
 int qcache_attend_launch(const QAttend& a) {
   const QCache c = make_cache(const_cast<void*>(a.k), const_cast<void*>(a.v),
                               const_cast<void*>(a.scales), a.kv_heads, a.d, a.sink, a.window);
-  const int group = (int)(a.H / a.kv_heads);
+  AttPlan p;
+  if (int rc = attend_plan(a.B, a.kv_heads, a.H / a.kv_heads, a.d, c.rows, &p)) return rc;
   return by_format(a.dtype, a.fmt, a.d, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
     constexpr int DP = dp.value;
-    // 16 query columns halve the passes over a group of more than 8; at 256
-    // columns per row the second set of accumulators would not fit the registers
     if constexpr (DP <= 128) {
-      if (group > 8)
-        return launch_attend<T, m.value, DP, 2>(a.q, c, a.lengths, a.o, a.o32, a.lse, a.B, group,
-                                                (float)a.scale, a.stream);
+      if (p.nq == 2)
+        return p.flat ? launch_attend<T, m.value, DP, 2, true>(a, c, p)
+                      : launch_attend<T, m.value, DP, 2, false>(a, c, p);
     }
-    return launch_attend<T, m.value, DP, 1>(a.q, c, a.lengths, a.o, a.o32, a.lse, a.B, group,
-                                            (float)a.scale, a.stream);
+    return p.flat ? launch_attend<T, m.value, DP, 1, true>(a, c, p)
+                  : launch_attend<T, m.value, DP, 1, false>(a, c, p);
   });
 }
 }  // namespace sbfa
+
+extern "C" int64_t sbfa_qcache_attend_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
+                                                      int64_t head_dim, int64_t sink,
+                                                      int64_t window) {
+  return qcache_attend_ws_bytes(B, H, kv_heads <= 0 ? H : kv_heads, head_dim, sink + window);
+}
 
 extern "C" int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
                                   const void* scales, const int64_t* lengths, void* o, float* lse,
                                   int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim,
                                   int dtype, int fmt, double softmax_scale, int64_t sink,
-                                  int64_t window, void* stream) {
+                                  int64_t window, void* ws, int64_t ws_bytes, void* stream) {
   const QAttend a{q,  k_codes,  v_codes,  scales, lengths, o,    nullptr, lse, B, H,
                   kv_heads <= 0 ? H : kv_heads, head_dim, dtype, fmt, softmax_scale, sink, window,
-                  (cudaStream_t)stream};
+                  ws, ws_bytes, (cudaStream_t)stream};
   if (int rc = qcache_attend_check(a)) return rc;
   return qcache_attend_launch(a);
 }

@@ -30,9 +30,31 @@ struct QAttend {
   int dtype, fmt;
   double scale;
   int64_t sink, window;
+  void* ws;
+  int64_t ws_bytes;
   cudaStream_t stream;
 };
+// Scratch of a call, -1 for a bad shape.
+int64_t qcache_attend_ws_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t d, int64_t rows);
 int qcache_attend_check(const QAttend& a);   // an SBFA_ERR_* code; launches nothing
 int qcache_attend_launch(const QAttend& a);  // after the check
+
+// A launch whose kernel may start before the kernel ahead of it in the stream has ended (and
+// waits for it itself).
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kern)(P...), unsigned grid, unsigned block, size_t smem,
+                         cudaStream_t s, bool early, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
 
 }  // namespace sbfa

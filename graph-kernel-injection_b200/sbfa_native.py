@@ -66,7 +66,8 @@ _SIGNATURES = {
     "sbfa_qcache_append": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32,
                             _i32, _i64, _i64, _i64, _vp], _i32),
     "sbfa_qcache_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32,
-                            _f64, _i64, _i64, _vp], _i32),
+                            _f64, _i64, _i64, _vp, _i64, _vp], _i32),
+    "sbfa_qcache_attend_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "sbfa_qcache_read": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i64,
                           _i64, _vp], _i32),
     "sbfa_prefix_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
@@ -74,7 +75,7 @@ _SIGNATURES = {
     "sbfa_qcache_prefix_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                    _i64, _i64, _i32, _i32, _f64, _i64, _i64, _vp, _i64, _vp],
                                   _i32),
-    "sbfa_qcache_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64], _i64),
+    "sbfa_qcache_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "sbfa_prefix_prompt": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                             _i64, _i32, _f64, _i64, _vp, _i64, _vp], _i32),
     "sbfa_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64], _i64),

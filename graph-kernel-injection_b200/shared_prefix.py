@@ -134,10 +134,12 @@ class SharedPrefix:
         o = torch.empty_like(q)
         lse = torch.empty((B, H, 1), dtype=torch.float32, device=dev) if return_lse else None
         with native.device_guard(dev):
-            need = self._scratch.get((B, H))
+            sizes = (B, H, cache.sink_size, cache.window_size, "cache")
+            need = self._scratch.get(sizes)
             if need is None:
-                need = self._remember((B, H), native.lib().sbfa_qcache_prefix_workspace_bytes(
-                    B, H, self.heads, self.length, self.head_dim))
+                need = self._remember(sizes, native.lib().sbfa_qcache_prefix_workspace_bytes(
+                    B, H, self.heads, self.length, self.head_dim, cache.sink_size,
+                    cache.window_size))
             ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
             native.check(native.lib().sbfa_qcache_prefix_attend(
                 q.data_ptr(), *cache._cache_ptrs, self.k.data_ptr(), self.v.data_ptr(),

@@ -158,6 +158,7 @@ class QuantizedStreamingKVCache:
         self.lengths = torch.zeros(batch, dtype=torch.int64, device=dev)
         self._tickets = torch.zeros(batch, dtype=torch.int32, device=dev)
         self._codes = (native.dtype_code(dtype), code)
+        self._scratch = {}   # scratch bytes of attend by the number of query heads
         self._cache_ptrs = (self._k.data_ptr(), self._v.data_ptr(), self.scales.data_ptr(),
                             self.lengths.data_ptr())
 
@@ -222,10 +223,17 @@ class QuantizedStreamingKVCache:
         lse = (torch.empty(self.batch, hq, 1, dtype=torch.float32, device=self.device)
                if return_lse else None)
         with native.device_guard(self.device):
+            need = self._scratch.get(hq)
+            if need is None:
+                need = self._scratch[hq] = native.lib().sbfa_qcache_attend_workspace_bytes(
+                    self.batch, hq, self.heads, self.head_dim, self.sink_size, self.window_size)
+            # from torch's allocator, so of the call's stream or graph
+            ws = (torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None)
             native.check(native.lib().sbfa_qcache_attend(
                 q.data_ptr(), *self._cache_ptrs, o.data_ptr(), native.ptr(lse), self.batch, hq,
                 self.heads, self.head_dim, *self._codes, scale, self.sink_size,
-                self.window_size, native.stream_ptr(self.device)), "qcache_attend")
+                self.window_size, native.ptr(ws), need, native.stream_ptr(self.device)),
+                "qcache_attend")
         return (o, lse) if return_lse else o
 
     def read(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

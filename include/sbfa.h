@@ -331,12 +331,18 @@ int sbfa_qcache_append(void* k_codes, void* v_codes, void* scales, int64_t* leng
 /* Attention of each sequence's query at its last position over its visible
  * rows.  q: contiguous [B, H, head_dim], H a multiple of kv_heads (<= 0 means H);
  * o: the same shape and dtype; lse (may be NULL): fp32 [B, H].  A sequence of
- * length 0 gives O = 0 and LSE = 0.  softmax_scale > 0.  No workspace. */
+ * length 0 gives O = 0 and LSE = 0.  softmax_scale > 0.  ws: 16-byte aligned
+ * caller scratch of sbfa_qcache_attend_workspace_bytes() bytes. */
 int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
                        const void* scales, const int64_t* lengths, void* o, float* lse,
                        int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim, int dtype,
-                       int fmt, double softmax_scale, int64_t sink, int64_t window,
-                       void* stream);
+                       int fmt, double softmax_scale, int64_t sink, int64_t window, void* ws,
+                       int64_t ws_bytes, void* stream);
+
+/* Scratch bytes sbfa_qcache_attend needs on the current device (may be 0; ws may then be
+ * NULL), -1 for a bad shape. */
+int64_t sbfa_qcache_attend_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
+                                           int64_t head_dim, int64_t sink, int64_t window);
 
 /* The kept rows as 16-bit values in order of position: out row i of a sequence
  * is its i-th kept position (sinks, then the window from its oldest), positions[b, i] that
@@ -383,7 +389,7 @@ int sbfa_qcache_prefix_attend(const void* q, const void* k_codes, const void* v_
 
 /* Scratch bytes sbfa_qcache_prefix_attend needs on the current device, -1 for a bad shape. */
 int64_t sbfa_qcache_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t P,
-                                           int64_t head_dim);
+                                           int64_t head_dim, int64_t sink, int64_t window);
 
 /* The batch's own prompts behind the prefix, in one pass: query i of a sequence sees
  * the whole prefix and its sequence's tokens (i - window, i] of k, v (logical [B,

@@ -186,6 +186,14 @@ def check_attend(c, q, scale=None, prefix=None, label=""):
     (2, 1, 17, 96, 4, 50, [54, 9]),
     (1, 1, 33, 256, 0, 40, [39]),
     (40, 8, 2, 128, 0, 40, list(range(40))),
+    # many units: equal runs of steps over all of them
+    (64, 2, 4, 128, 4, 500, [(b * 37) % 600 for b in range(64)]),
+    (200, 2, 1, 64, 0, 33, [b % 36 for b in range(200)]),
+    (20, 6, 12, 80, 2, 300, [0] * 7 + [302] + [0] * 4 + [1, 500, 31, 32, 33, 64, 65, 0]),
+    (37, 3, 9, 256, 4, 90, [b * 5 for b in range(37)]),
+    (300, 1, 17, 64, 0, 20, [3] * 300),
+    (130, 1, 2, 128, 0, 16, [0] * 130),
+    (7, 16, 1, 128, 0, 9000, [9000, 0, 8999, 1, 4500, 12, 7]),
 ])
 def test_attend_matches_64_bits(fmt, dtype, B, H, G, D, S, W, lengths):
     g = gen(4)
@@ -195,12 +203,13 @@ def test_attend_matches_64_bits(fmt, dtype, B, H, G, D, S, W, lengths):
     assert native.device_status() == 0
 
 
-def test_attend_every_length_of_a_short_ring():
+@pytest.mark.parametrize("H", [1, 3])
+def test_attend_every_length_of_a_short_ring(H):
     S, W = 2, 70
     lengths = list(range(74))
     g = gen(5)
-    c = filled(g, len(lengths), 1, 64, S, W, torch.bfloat16, "int8", lengths)
-    check_attend(c, rows(g, (len(lengths), 3, 1, 64), torch.bfloat16), scale=0.3)
+    c = filled(g, len(lengths), H, 64, S, W, torch.bfloat16, "int8", lengths)
+    check_attend(c, rows(g, (len(lengths), 3 * H, 1, 64), torch.bfloat16), scale=0.3)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])

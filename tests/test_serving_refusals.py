@@ -43,9 +43,10 @@ def test_append_of_nothing_launches_nothing():
     assert append(native.lib(), n=0, new=None) == 0 and native.launch_count() == before
 
 
-def attend(L, q=P, o=P, lse=P, B=1, H=4, hkv=2, D=64, scale=0.1, fmt=1):
-    return L.sbfa_qcache_attend(q, P, P, P, P, o, lse, B, H, hkv, D, native.F16, fmt, scale, 4, 8,
-                                None)
+def attend(L, q=P, o=P, lse=P, B=1, H=4, hkv=2, D=64, scale=0.1, fmt=1, ws=P,
+           ws_bytes=1 << 40, window=8):
+    return L.sbfa_qcache_attend(q, P, P, P, P, o, lse, B, H, hkv, D, native.F16, fmt, scale, 4,
+                                window, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("kw,word", [
@@ -53,7 +54,8 @@ def attend(L, q=P, o=P, lse=P, B=1, H=4, hkv=2, D=64, scale=0.1, fmt=1):
     (dict(scale=-1.0), "softmax_scale"), (dict(scale=float("nan")), "softmax_scale"),
     (dict(scale=float("inf")), "softmax_scale"), (dict(q=None), "NULL"), (dict(o=None), "NULL"),
     (dict(q=P + 8), "aligned"),
-    (dict(o=P + 4), "aligned"),
+    (dict(o=P + 4), "aligned"), (dict(B=300, window=9999, ws=None), "workspace"),
+    (dict(B=300, window=9999, ws_bytes=1000), "workspace"), (dict(ws=P + 8), "aligned"),
 ])
 def test_attend_refuses(kw, word):
     assert attend(native.lib(), **kw) == INVALID and word in native.last_error()
@@ -107,8 +109,14 @@ def test_sizes():
     for bad in ((0, 4, 2, 1, 100, 64, 0), (2, 4, 3, 1, 100, 64, 0), (2, 4, 2, 1, 0, 64, 0),
                 (2, 4, 2, 1, 100, 256, 0), (2, 4, 2, 1, 100, 64, -1)):
         assert L.sbfa_prefix_workspace_bytes(*bad) == -1
-    assert L.sbfa_qcache_prefix_workspace_bytes(2, 4, 2, 100, 64) >= 2 * 4 * 65 * 4
-    assert L.sbfa_qcache_prefix_workspace_bytes(2, 3, 2, 100, 64) == -1
+    assert L.sbfa_qcache_prefix_workspace_bytes(2, 4, 2, 100, 64, 4, 8) >= 2 * 4 * 65 * 4
+    assert L.sbfa_qcache_prefix_workspace_bytes(2, 3, 2, 100, 64, 4, 8) == -1
+    # few units share clusters and need no scratch, many long ones are cut into equal runs
+    assert L.sbfa_qcache_attend_workspace_bytes(2, 4, 2, 64, 4, 8) == 0
+    assert L.sbfa_qcache_attend_workspace_bytes(300, 4, 2, 64, 4, 9999) > 0
+    for bad in ((2, 3, 2, 64, 4, 8), (2, 4, 2, 60, 4, 8), (0, 4, 2, 64, 4, 8),
+                (2, 4, 2, 64, 0, 0)):
+        assert L.sbfa_qcache_attend_workspace_bytes(*bad) == -1
 
 
 @pytest.mark.parametrize("kw,word", [
