@@ -115,24 +115,37 @@ __device__ __forceinline__ float saturated(float x) {
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
-// A group of G = DP / 8 lanes takes one (head, token): 16 bytes of K and of V per
-// lane, the row maxima by shuffles, 8 code bytes back.  Bound by HBM: 4 D bytes in,
-// 2 D + 2 out per head and token.  A CTA covers 2^hs heads x kRows / 2^hs tokens at a
-// time (tokens adjacent, so that their scale pairs share sectors; several heads only
-// where a call has few tokens) and walks the tokens that survive the call: positions
-// that a later token of it overwrites are never visited.  The last CTA of a sequence moves its
-// length on (a ticket per sequence, left at zero), which saves a second launch in every
-// decode step.
+// A group of 8 lanes (16 at 256 columns) takes one (head, token): pieces of 16 bytes of K
+// and of V, the row maxima in packed 16-bit integers (the magnitudes of both 16-bit types are
+// ordered like their bits) with one shuffle chain for both, 8 code bytes back per piece.
+// Bound by HBM (4 D bytes in, 2 D + 2 out per head and token) and nearly by instruction issue:
+// 16 x 8 x 2048 rows of 128 take 45 us with 16 lanes a row and fp32 maxima, 40 us so.  A CTA covers 2^hs heads x
+// kRows / 2^hs tokens at a time (tokens adjacent, so that their scale pairs share sectors;
+// several heads only where a call has few tokens) and walks the tokens that survive the
+// call: positions that a later token of it overwrites are never visited.  The last CTA of a
+// sequence moves its length on (a ticket per sequence, left at zero), which saves a second launch
+// in every decode step.
 constexpr int kAppThreads = 256;
-constexpr int kAppUnroll = 2;
+constexpr int kAppRounds = 2;   // of resident CTAs, with at least two passes each
+constexpr int app_lanes(int dp) { return dp == 256 ? 16 : 8; }
 
-template <typename T, int FMT, int G>
+// fp32 bits of the magnitude whose 16 bits are `h`
+template <typename T> __device__ __forceinline__ uint32_t magnitude_bits(uint32_t h);
+template <> __device__ __forceinline__ uint32_t magnitude_bits<__nv_bfloat16>(uint32_t h) {
+  return h << 16;
+}
+template <> __device__ __forceinline__ uint32_t magnitude_bits<__half>(uint32_t h) {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+}
+
+template <typename T, int FMT, int DP>
 __global__ void __launch_bounds__(kAppThreads)
     qcache_append_kernel(QCache c, int64_t* __restrict__ lengths, int32_t* __restrict__ tickets,
                          const T* __restrict__ kn, const T* __restrict__ vn, Strides3 sk,
                          Strides3 sv, const int64_t* __restrict__ counts, int n_new,
                          int head_blocks, int hs) {
-  constexpr int DP = G * 8;
+  constexpr int G = app_lanes(DP);
+  constexpr int VPL = DP / (8 * G);                          // pieces of a row per lane
   constexpr int kRows = kAppThreads / G;
   const int b = blockIdx.y;
   const int lane = threadIdx.x % G, slot = threadIdx.x / G;
@@ -147,61 +160,64 @@ __global__ void __launch_bounds__(kAppThreads)
   const int t_win = max(n_sink, cnt - window);
   const int items = n_sink + cnt - t_win;
   const int slot0 = cnt > t_win ? (int)((len + t_win - c.sink) % c.window) : 0;
-  const bool on = lane * 8 < c.d, real = head < (int)c.heads;
+  const bool real = head < (int)c.heads;
   const T* ks = kn + b * sk.b + head * sk.h + lane * 8;
   const T* vs = vn + b * sv.b + head * sv.h + lane * 8;
   const int64_t row0 = ((int64_t)b * c.heads + head) * c.rows;
-  for (int j0 = chunk * tp * kAppUnroll; j0 < items; j0 += chunks * tp * kAppUnroll) {
-    uint4 xk[kAppUnroll], xv[kAppUnroll];
-    int row[kAppUnroll];
+  for (int j0 = chunk * tp; j0 < items; j0 += chunks * tp) {
+    const int j = j0 + slot % tp;
+    uint4 x[2][VPL];
+    int row = -1;
 #pragma unroll
-    for (int u = 0; u < kAppUnroll; ++u) {
-      const int j = j0 + u * tp + slot % tp;
-      xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
-      row[u] = -1;
-      if (j < items && real) {
-        const int k = j - n_sink;
-        const int t = k < 0 ? j : t_win + k;
-        const int w = slot0 + k;                             // < 2 * window
-        row[u] = k < 0 ? (int)len + j : sink + (w >= window ? w - window : w);
-        if (on) {
-          xk[u] = __ldcs(reinterpret_cast<const uint4*>(ks + t * sk.n));
-          xv[u] = __ldcs(reinterpret_cast<const uint4*>(vs + t * sv.n));
+    for (int i = 0; i < VPL; ++i) x[0][i] = x[1][i] = make_uint4(0, 0, 0, 0);
+    if (j < items && real) {
+      const int k = j - n_sink;
+      const int t = k < 0 ? j : t_win + k;
+      const int w = slot0 + k;                               // < 2 * window
+      row = k < 0 ? (int)len + j : sink + (w >= window ? w - window : w);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if ((lane + i * G) * 8 < c.d) {
+          x[0][i] = __ldcs(reinterpret_cast<const uint4*>(ks + t * sk.n + i * G * 8));
+          x[1][i] = __ldcs(reinterpret_cast<const uint4*>(vs + t * sv.n + i * G * 8));
         }
+    }
+    uint32_t m[2] = {0, 0};
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const uint4 w = x[p][i];
+        m[p] = __vmaxu2(m[p], __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
+                                       __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+      }
+    // both rows' maxima in one word: K's in the low half, V's in the high one
+    uint32_t both = __vmaxu2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+    for (int s = G / 2; s > 0; s >>= 1)
+      both = __vmaxu2(both, __shfl_xor_sync(kFull, both, s, G));
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const uint32_t e = scale_byte<FMT>(magnitude_bits<T>(p == 0 ? both & 0xffffu : both >> 16));
+      bytes |= e << (8 * p);
+      const bool bad = e == kBadRow;
+      const float inv = bad ? 0.f : scale_inverse(e);
+      const float2 inv2 = make_float2(inv, inv);
+      uint8_t* dst = (p == 0 ? c.k : c.v) + (row0 + row) * DP + lane * 8;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const uint4 w = x[p][i];
+        const float2 f0 = __fmul2_rn(unpack2<T>(w.x), inv2), f1 = __fmul2_rn(unpack2<T>(w.y), inv2);
+        const float2 f2 = __fmul2_rn(unpack2<T>(w.z), inv2), f3 = __fmul2_rn(unpack2<T>(w.w), inv2);
+        const uint32_t lo = encode4<FMT>(f0.x, f0.y, f1.x, f1.y);
+        const uint32_t hi = encode4<FMT>(f2.x, f2.y, f3.x, f3.y);
+        if (row >= 0)
+          *reinterpret_cast<uint2*>(dst + i * G * 8) =
+              bad ? make_uint2(0, 0) : make_uint2(lo, hi);
       }
     }
-#pragma unroll
-    for (int u = 0; u < kAppUnroll; ++u) {
-      uint32_t bytes = 0;
-      uint2 codes[2];
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const uint4 w = part == 0 ? xk[u] : xv[u];
-        float2 f[4] = {unpack2<T>(w.x), unpack2<T>(w.y), unpack2<T>(w.z), unpack2<T>(w.w)};
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          m = max(m, max(__float_as_uint(f[j].x) & 0x7fffffffu,
-                         __float_as_uint(f[j].y) & 0x7fffffffu));
-#pragma unroll
-        for (int s = G / 2; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(kFull, m, s, G));
-        const uint32_t e = scale_byte<FMT>(m);
-        bytes |= e << (8 * part);
-        if (e == kBadRow) {
-          codes[part] = make_uint2(0, 0);
-        } else {
-          const float inv = scale_inverse(e);
-          codes[part].x = encode4<FMT>(f[0].x * inv, f[0].y * inv, f[1].x * inv, f[1].y * inv);
-          codes[part].y = encode4<FMT>(f[2].x * inv, f[2].y * inv, f[3].x * inv, f[3].y * inv);
-        }
-      }
-      if (row[u] >= 0) {
-        const int64_t dst = row0 + row[u];
-        reinterpret_cast<uint2*>(c.k + dst * DP)[lane] = codes[0];
-        reinterpret_cast<uint2*>(c.v + dst * DP)[lane] = codes[1];
-        if (lane == 0) c.scales[dst] = (uint16_t)bytes;
-      }
-    }
+    if (row >= 0 && lane == 0) c.scales[row0 + row] = (uint16_t)bytes;
   }
   // every CTA of this sequence has read its length before the last one writes it
   __syncthreads();
@@ -223,10 +239,12 @@ __global__ void __launch_bounds__(kAppThreads)
 // ---------------------------------------------------------------------------
 // Out row i of a sequence is its i-th kept position in order (sinks, then the
 // window from its oldest), rows behind the last one are zero with position -1.
-// A group of DP / 8 lanes per row as above, CTAs walk the rows of one head; bound by HBM
-// (2 D + 2 bytes in, 4 D out per kept row and head).
+// A group of DP / 8 lanes per row, CTAs walk the rows of one head; bound by HBM (2 D + 2
+// bytes in, 4 D out per kept row and head).  64 x 8 x 2052 rows of 128 take 175, 144, 138, 131 us with
+// 1, 2, 4, 8 rounds of resident CTAs: many short CTAs keep loads and stores of different ones apart.
 constexpr int kReadThreads = 256;
 constexpr int kReadUnroll = 4;
+constexpr int kReadRounds = 8;   // of resident CTAs
 
 template <typename T, int FMT>
 __device__ __forceinline__ uint4 values8(uint2 codes, float scale) {
@@ -1101,18 +1119,18 @@ int by_format(int dtype, int fmt, int64_t D, F&& f) {
 
 // Grid of the append and read kernels for `rows` rows of each head: 2^hs heads per CTA
 // where a head has fewer rows than a CTA takes at a time, else as many CTAs along a head as
-// keep every SM busy with about two rounds of resident CTAs.
+// make `ctas` per SM in all, each with at least `passes` passes.
 struct RowGrid {
   dim3 grid;
   int head_blocks, hs;
 };
-int row_grid(int64_t B, int64_t H, int64_t rows, int per_cta, int unroll, int resident,
+int row_grid(int64_t B, int64_t H, int64_t rows, int per_cta, int unroll, int passes, int ctas,
              RowGrid* g) {
   int hs = 0;
   while ((1 << (hs + 1)) <= per_cta && (1 << hs) < H && (per_cta >> (hs + 1)) >= rows) ++hs;
   const int64_t blocks = (H + (1ll << hs) - 1) >> hs;
-  const int64_t step = (int64_t)(per_cta >> hs) * unroll;
-  const int64_t want = (int64_t)device_sm_count() * resident * 2;
+  const int64_t step = (int64_t)(per_cta >> hs) * unroll * passes;
+  const int64_t want = (int64_t)device_sm_count() * ctas;
   const int64_t chunks = std::max<int64_t>(
       1, std::min((rows + step - 1) / step, (want + B * blocks - 1) / (B * blocks)));
   if (blocks * chunks >= (1ll << 31)) return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many heads");
@@ -1239,12 +1257,12 @@ extern "C" int sbfa_qcache_append(void* k_codes, void* v_codes, void* scales, in
   cudaStream_t s = (cudaStream_t)stream;
   return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
-    constexpr int G = dp.value / 8;
     RowGrid g;
-    if (int rc = row_grid(B, H, std::min(n_new, c.rows), kAppThreads / G, kAppUnroll, 5, &g))
+    if (int rc = row_grid(B, H, std::min(n_new, c.rows), kAppThreads / app_lanes(dp.value), 1, 2,
+                          5 * kAppRounds, &g))
       return rc;
     LaunchScope ls("qcache_append_kernel", s);
-    qcache_append_kernel<T, m.value, G><<<g.grid, kAppThreads, 0, s>>>(
+    qcache_append_kernel<T, m.value, dp.value><<<g.grid, kAppThreads, 0, s>>>(
         c, lengths, tickets, (const T*)k_new, (const T*)v_new, st[0], st[1], counts, (int)n_new,
         g.head_blocks, g.hs);
     return check_launch("qcache_append_kernel");
@@ -1269,7 +1287,8 @@ extern "C" int sbfa_qcache_read(const void* k_codes, const void* v_codes, const 
     using T = decltype(t);
     constexpr int G = dp.value / 8;
     RowGrid g;
-    if (int rc = row_grid(B, H, c.rows, kReadThreads / G, kReadUnroll, 4, &g)) return rc;
+    if (int rc = row_grid(B, H, c.rows, kReadThreads / G, kReadUnroll, 1,
+                          4 * kReadRounds, &g)) return rc;
     LaunchScope ls("qcache_read_kernel", s);
     qcache_read_kernel<T, m.value, G><<<g.grid, kReadThreads, 0, s>>>(
         c, lengths, (T*)k_out, (T*)v_out, positions, g.head_blocks, g.hs);
