@@ -608,6 +608,14 @@ __global__ void __launch_bounds__(kMergeThreads)
   const int64_t out = live ? out_row(geo, unit / geo.pairs, row) : 0;
   const bool on = lane * 4 < geo.d;
   const float own_l2 = live && po.own_kind != kOwnNone ? po.own_lse[out] * kLog2e : -INFINITY;
+  // the first slices' columns are under way while the weights are worked out
+  constexpr int kAhead = 8;
+  const float* src = po.part + (live ? at : 0) * D + lane * 4;
+  float4 p[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    p[j] = live && j < geo.splits ? *reinterpret_cast<const float4*>(src + j * all * D)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
   // every slice's m and l at once, a lane each (at most 64 slices, 16 or 32 lanes)
   float2 st[64 / kLanes];
   float M = own_l2;
@@ -632,7 +640,6 @@ __global__ void __launch_bounds__(kMergeThreads)
   const float f_own = own_l2 == -INFINITY ? 0.f : ex2(own_l2 - ref);
   l += f_own;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float* src = po.part + (live ? at : 0) * D + lane * 4;
   auto add = [&](float4 p, float f) {
     a.x += p.x * f;
     a.y += p.y * f;
@@ -640,9 +647,12 @@ __global__ void __launch_bounds__(kMergeThreads)
     a.w += p.w * f;
   };
 #pragma unroll
+  for (int j = 0; j < kAhead; ++j)   // a slice that is not there has weight 0 and zero columns
+    add(p[j], __shfl_sync(0xffffffffu, w[0], j, kLanes));
+#pragma unroll
   for (int i = 0; i < 64 / kLanes; ++i)
 #pragma unroll 8
-    for (int j = 0; j < kLanes; ++j) {
+    for (int j = i == 0 ? kAhead : 0; j < kLanes; ++j) {
       if (i * kLanes + j >= geo.splits) break;
       add(*reinterpret_cast<const float4*>(src + (i * kLanes + j) * all * D),
           __shfl_sync(0xffffffffu, w[i], j, kLanes));

@@ -33,9 +33,9 @@ def no_gradients(*tensors: torch.Tensor) -> None:
 
 
 def vector_readable(t: torch.Tensor) -> torch.Tensor:
-    """``t`` when its rows can be read in place in 16-byte pieces, else a contiguous copy."""
-    st = t.stride()
-    if st[-1] != 1 or t.data_ptr() % 16 or any(x < 0 or x % 8 for x in st[:-1]):
+    """The 4-D ``t`` when its rows can be read in place in 16-byte pieces, else a contiguous copy."""
+    b, h, n, d = t.stride()
+    if d != 1 or (b | h | n) & 7 or t.data_ptr() & 15:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
