@@ -20,7 +20,10 @@
 // the same pass: a tile of 128 keys of one sequence, or of 128 / 2^k short
 // sequences with 2^k >= n_q rows each, in which each query row sees one interval
 // of columns.  So a prompt takes one launch, and its two parts share one softmax and
-// one rounding.
+// one rounding.  A value row in a tile belongs to some of the tile's query rows only, and a
+// weight of zero does not keep a NaN or an infinity out of the others' sums: a fourth
+// warp looks over every own V tile as it arrives, replaces such elements by zeros and
+// has the epilogue add them to the rows that do see them.
 //
 // Slices.  Whole waves of CTAs take all keys of their rows and write O themselves.  The
 // rest (all of them in a decode step) would leave most SMs idle, so their keys are cut
@@ -77,6 +80,8 @@ struct PrefixOut {
   const void* own_o;
   const float* own_lse;
   int own_kind;
+  const void* own_v;     // own value rows and their strides (prompts)
+  Strides3 sv;
   float* part;           // [splits][n_tail * 256][D]
   float2* stats;         // [splits][n_tail * 256] (m, l)
 };
@@ -147,9 +152,12 @@ struct PrefixLayout {
   static constexpr int kPVDone = 9 + 2 * STAGES;  // [2]
   static constexpr int kOFull = 11 + 2 * STAGES;  // [2]
   static constexpr int kDrain = 13 + 2 * STAGES;  // [2]
-  static constexpr int kNumBars = 15 + 2 * STAGES;
-  static constexpr uint32_t MISC = BAR + kNumBars * 8;
+  static constexpr int kVRaw = 15 + 2 * STAGES;   // [STAGES] an own V tile has arrived
+  static constexpr int kNumBars = 15 + 3 * STAGES;
+  static constexpr uint32_t MISC = BAR + kNumBars * 8;  // TMEM base, abort flag, bad V flag
   static constexpr uint32_t kAlloc = MISC + 16 + 1024;
+  // key tiles from one own V tile to the next in the same ring slot
+  static constexpr int kVPeriod = STAGES % 2 ? STAGES : STAGES / 2;
 };
 
 template <typename T, int D, int STAGES>
@@ -172,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar = [&](int i) -> uint32_t { return sb + L::BAR + 8u * (uint32_t)i; };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
+  volatile int* bad_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bid = (int)blockIdx.x;
@@ -188,15 +197,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   // slices of n_all / splits tiles, none empty (splits <= n_tiles)
   const int t0 = (int)((int64_t)split * n_all / splits);
   const int n = (int)((int64_t)(split + 1) * n_all / splits) - t0;
+  const int j_own = max(0, geo.n_tiles - t0);   // the first of them with own keys (n if none)
 
-  // K (part 0) or V (part 1) of key tile t into ring slot s
+  // phase of kVRaw in which own tile j arrives: how often its slot has held an own V before
+  auto own_phase = [&](int j) { return (uint32_t)(((j - j_own) / L::kVPeriod) & 1); };
+  // K (part 0) or V (part 1) of key tile t into ring slot s.  Own V tiles complete on kVRaw, and
+  // the warp that looks them over completes kKVFull.
   auto load_tile = [&](int t, int part, int s) {
     const uint32_t dst = sb + L::KV + (uint32_t)s * L::kTile;
-    mbar_expect_tx(bar(L::kKVFull + s), L::kTile);
+    const uint32_t full = bar((part == 1 && t >= geo.n_tiles ? L::kVRaw : L::kKVFull) + s);
+    mbar_expect_tx(full, L::kTile);
     if (t < geo.n_tiles) {
       for (int r = 0; r < kBoxes; ++r)
-        tma_load_4d(dst + r * 16384u, part == 0 ? &tmk : &tmv, bar(L::kKVFull + s), 64 * r,
-                    t * kTN, kvh, 0);
+        tma_load_4d(dst + r * 16384u, part == 0 ? &tmk : &tmv, full, 64 * r, t * kTN, kvh, 0);
       return;
     }
     int b, kt;
@@ -205,8 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < seqs; ++i)   // a sequence behind the last one reads as zeros
       for (int r = 0; r < kBoxes; ++r)
         tma_load_4d(dst + r * 16384u + (uint32_t)(i * geo.box) * 128u,
-                    part == 0 ? &tmok : &tmov, bar(L::kKVFull + s), 64 * r, kt * kTN, kvh,
-                    b * seqs + i);
+                    part == 0 ? &tmok : &tmov, full, 64 * r, kt * kTN, kvh, b * seqs + i);
   };
 
   if (threadIdx.x == 0) {
@@ -214,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar(L::kKVFull + s), 1);
       mbar_init(bar(L::kKVEmpty + s), nx);
+      mbar_init(bar(L::kVRaw + s), 1);
     }
     for (int x = 0; x < kPair; ++x) {
       mbar_init(bar(L::kSFull + 2 * x), 1);
@@ -225,6 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(L::kDrain + x), 1);
     }
     *abort_flag = 0;
+    *bad_flag = 0;
     mbar_init_fence();
     // the first K and V on their way before the TMEM allocation and the CTA-wide sync
     load_tile(t0, 0, 0);
@@ -259,8 +273,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       for (int s = 0; s < STAGES; ++s) {  // our own copies still in flight
-        const int fills = issued > s ? (issued - 1 - s) / STAGES + 1 : 0;
-        if (fills) wait_bar_drain(bar(L::kKVFull + s), (uint32_t)((fills - 1) & 1), status);
+        if (issued <= s) continue;
+        const int e = s + (issued - 1 - s) / STAGES * STAGES;   // the slot's last entry
+        if (e % 2 && e / 2 >= j_own)
+          wait_bar_drain(bar(L::kVRaw + s), own_phase(e / 2), status);
+        else
+          wait_bar_drain(bar(L::kKVFull + s), (uint32_t)((e / STAGES) & 1), status);
       }
     } else if ((warp == 1 || warp == 2) && warp <= nx) {
       // ---------------------------------------------------------- MMA issuers
@@ -326,6 +344,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_commit_w(bar(L::kOFull + x));
       tc_commit_w(bar(L::kDrain + x));
       wait_bar_drain(bar(L::kDrain + x), 0, status);
+    } else if (warp == 3) {
+      // ---------------------------------------------------------- own V tiles
+      constexpr uint32_t kInf = kBF16 ? 0x7f80u : 0x7c00u;   // 16 bits of infinity
+      for (int j = j_own; j < n; ++j) {
+        const int e = 2 * j + 1, s = e % STAGES;
+        if (!wait_bar_w(bar(L::kVRaw + s), own_phase(j), abort_flag, status)) break;
+        const uint32_t tile = sb + L::KV + (uint32_t)s * L::kTile + 16u * (uint32_t)lane;
+        bool bad = false;
+#pragma unroll 8
+        for (uint32_t off = 0; off < L::kTile; off += 512u) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(tile + off));
+          const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                                      __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+          bad |= (m & 0xffffu) >= kInf || (m >> 16) >= kInf;
+        }
+        if (__any_sync(0xffffffffu, bad)) {   // rare: zeros in the place of such elements
+          for (uint32_t off = 0; off < L::kTile; off += 512u)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+              uint32_t w;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(tile + off + 4u * i));
+              if ((w & 0x7fffu) >= kInf) w &= 0xffff0000u;
+              if ((w >> 16 & 0x7fffu) >= kInf) w &= 0xffffu;
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(tile + off + 4u * i), "r"(w) : "memory");
+            }
+          *bad_flag = 1;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::kKVFull + s));
+      }
     }
   } else {
     regs_inc<kRegsSoftmax>();
@@ -521,6 +572,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         };
+        // columns [c0, c0 + 32) of what the fourth warp took out of the value rows that this row sees
+        const bool patch = live && *bad_flag != 0;
+        auto put_back = [&](float* f, int c0) {
+          const T* v = (const T*)out.own_v + seq * out.sv.b + (int64_t)kvh * out.sv.h + c0;
+          for (int k = max(iq - geo.window + 1, 0); k <= iq; ++k)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c0 + i < geo.d) {
+                const float y = Elem<T>::to(v[k * out.sv.n + i]);
+                if (!(fabsf(y) < INFINITY)) f[i] += y;
+              }
+        };
         if (sliced) {
           const int64_t all = (int64_t)geo.n_tail * (kPair * kTM);
           const int64_t slot = split * all + (int64_t)tail * (kPair * kTM) + x * kTM + r;
@@ -532,6 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               uint32_t ov[32];
               tmem_ld32(t_o + (uint32_t)(half * (D / 2) + 32 * c), ov);
               tmem_wait_ld();
+              if (patch) put_back(reinterpret_cast<float*>(ov), half * (D / 2) + 32 * c);
 #pragma unroll
               for (int i = 0; i < 8; ++i)
                 put(8 * c + i, ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
@@ -556,6 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float f[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(ov[i]) * w_pre;
+            if (patch) put_back(f, 32 * c);
             if (f_own != 0.f) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
@@ -969,6 +1034,7 @@ extern "C" int sbfa_prefix_prompt(const void* q, const void* k, const void* v,
   c.v = v_prefix;
   c.own_k = k;
   c.own_v = v;
+  c.out.own_v = v;
   const int64_t hk = geo.kv_heads;
   const Strides3 dense{hk * n_q * head_dim, n_q * head_dim, head_dim};
   c.sk = strides ? Strides3{strides[3], strides[4], strides[5]} : dense;
@@ -976,6 +1042,7 @@ extern "C" int sbfa_prefix_prompt(const void* q, const void* k, const void* v,
   if (!tma_compatible(k, c.sk) || !tma_compatible(v, c.sv))
     return fail(SBFA_ERR_INVALID, "sbfa_prefix_prompt: k and v must be 16-byte aligned with "
                                   "strides that are positive multiples of 8 elements");
+  c.out.sv = c.sv;
   c.out.o = o;
   c.out.lse = lse;
   c.ws = ws;

@@ -113,7 +113,8 @@ def test_decode_behind_a_prefix_with_the_16_bit_cache(dtype):
     (1, 2, 2, 300, 129, 64, 128),
     (37, 1, 2, 5, 200, 64, 3), (150, 2, 1, 1, 10, 128, 7), (9, 1, 5, 64, 128, 40, 20),
     (3, 1, 7, 65, 64, 96, 65), (2, 2, 1, 513, 5, 128, 200), (1, 1, 2, 700, 1500, 64, 701),
-    (5, 1, 1, 129, 1000, 128, 129), (6, 1, 3, 8, 9000, 128, 8)])
+    (5, 1, 1, 129, 1000, 128, 129), (6, 1, 3, 8, 9000, 128, 8), (2, 1, 2, 300, 5000, 128, 300),
+    (2, 1, 2, 600, 3333, 64, 500)])
 def test_prompts_behind_a_prefix(dtype, B, Hkv, G, N, P, D, W):
     g = gen(25)
     pre = make(g, Hkv, P, D, dtype)
@@ -132,6 +133,41 @@ def test_prompts_behind_a_prefix(dtype, B, Hkv, G, N, P, D, W):
             ds = (q[b, h].double().abs() @ kk.abs().T).amax(-1) / math.sqrt(D) * D * 2.0 ** -23
             ref.check(o[b, h], w @ vv, w @ vv.abs(), ds, u, u)
             ref.check_lse(lse[b, h], torch.logsumexp(x, -1), ds)
+    assert native.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,G,N,P,D,W", [(5, 3, 20, 100, 64, 7), (3, 2, 200, 40, 128, 30),
+                                         (40, 1, 3, 3000, 80, 3), (2, 1, 90, 9000, 128, 50)])
+def test_prompts_with_nan_and_infinities_in_some_rows(dtype, B, G, N, P, D, W):
+    """Rows of one sequence do not reach another's, nor a query ahead of them (padding may hold
+    anything); the queries that see them get what 64 bits give."""
+    g = gen(30)
+    pre = make(g, 1, P, D, dtype)
+    q, k, v = (rows(g, (B, N, h, D), dtype, 0.2).transpose(1, 2) for h in (G, 1, 1))
+    clean = pre.attend_prompt(q, k, v, window_size=W)
+    k, v = k.clone(), v.clone()
+    at = N // 2
+    v[1, 0, at, 3], v[1, 0, at, D - 1] = math.nan, -math.inf      # seen by queries at .. at + W - 1
+    v[1, 0, min(at + 1, N - 1), 5] = math.inf
+    v[0, 0, N - 1, 2] = math.inf                                  # seen by the last query alone
+    k[B - 1, 0, N - 1] = math.nan
+    k[0, 0, N - 1, 0] = math.nan
+    o = pre.attend_prompt(q, k, v, window_size=W)
+    i = torch.arange(N, device=DEV)
+    gap = i[:, None] - i[None, :]
+    seen = (gap >= 0) & (gap < W)
+    bad = ~torch.isfinite(v)
+    for b in range(B):
+        # a column is not finite where a seen value of it is not (or a seen key is NaN)
+        col = (seen.double() @ bad[b, 0].double()) > 0
+        row = (seen.double() @ (~torch.isfinite(k[b, 0]).all(-1)).double()) > 0
+        want = (col | row[:, None]).expand(G, N, D)
+        assert torch.equal(~torch.isfinite(o[b]), want), b
+        assert torch.equal(o[b][~want], clean[b][~want]), b
+    one = o[1, :, at, D - 1]
+    assert torch.equal(one, torch.full_like(one, -math.inf))
+    assert torch.isnan(o[1, :, at, 3]).all()
     assert native.device_status() == 0
 
 
