@@ -969,6 +969,7 @@ extern "C" int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const
 extern "C" int64_t sbfa_qcache_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
                                                       int64_t P, int64_t head_dim, int64_t sink,
                                                       int64_t window) {
+  if (sink < 0 || window < 0 || sink >= (1 << 30) || window >= (1 << 30)) return -1;
   const int64_t rows = sink + window;
   PrefixGeom geo;
   if (!prefix_geometry(B, H, kv_heads, 1, P, head_dim, 0, &geo)) return -1;
@@ -987,7 +988,8 @@ extern "C" int sbfa_qcache_prefix_attend(
   if (int rc = check_prefix(B, H, kv_heads, 1, P, head_dim, dtype, 0, &geo)) return rc;
   const int64_t need =
       sbfa_qcache_prefix_workspace_bytes(B, H, kv_heads, P, head_dim, sink, window);
-  if (need < 0) return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: bad sizes");
+  if (need < 0)
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: sizes out of the cache's range");
   if (ws == nullptr || ws_bytes < need)
     return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: workspace too small (need " +
                                       std::to_string(need) + " bytes)");

@@ -1079,13 +1079,15 @@ int check_qcache(const void* k, const void* v, const void* scales, const void* l
   if (fmt != SBFA_Q_E4M3 && fmt != SBFA_Q_INT8)
     return fail(SBFA_ERR_INVALID, "8-bit cache: unknown format code");
   if (B <= 0 || H <= 0) return fail(SBFA_ERR_INVALID, "B and H must be positive");
-  if (B > 65535) return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: at most 65535 sequences");
+  if (B > 65535 || H >= (1 << 24))
+    return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: at most 65535 sequences and 2^24 heads");
   if (padded_dim(D) == 0)
     return fail(SBFA_ERR_UNSUPPORTED,
                 "8-bit cache: head_dim must be a multiple of 8 and at most 256");
   if (sink < 0 || window < 0)
     return fail(SBFA_ERR_INVALID, "sink_size and window_size must be non-negative");
-  if (sink + window <= 0 || sink + window >= (1ll << 30))
+  if (sink >= (1ll << 30) || window >= (1ll << 30) || sink + window <= 0 ||
+      sink + window >= (1ll << 30))
     return fail(SBFA_ERR_INVALID, "sink_size + window_size must be in [1, 2^30)");
   if (!k || !v || !scales || !lengths)
     return fail(SBFA_ERR_INVALID, "8-bit cache: NULL cache pointer");
@@ -1299,8 +1301,9 @@ extern "C" int sbfa_qcache_read(const void* k_codes, const void* v_codes, const 
 namespace sbfa {
 int64_t qcache_attend_ws_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t d, int64_t rows) {
   AttPlan p;
-  if (B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads != 0 || padded_dim(d) == 0 || rows <= 0 ||
-      attend_plan(B, kv_heads, H / kv_heads, d, rows, &p) != SBFA_OK)
+  if (B <= 0 || B > 65535 || H <= 0 || kv_heads <= 0 || kv_heads >= (1 << 24) ||
+      H % kv_heads != 0 || H / kv_heads >= (1 << 20) || padded_dim(d) == 0 || rows <= 0 ||
+      rows >= (1 << 30) || attend_plan(B, kv_heads, H / kv_heads, d, rows, &p) != SBFA_OK)
     return -1;
   return p.ws_bytes;
 }
@@ -1349,6 +1352,7 @@ int qcache_attend_launch(const QAttend& a) {
 extern "C" int64_t sbfa_qcache_attend_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
                                                       int64_t head_dim, int64_t sink,
                                                       int64_t window) {
+  if (sink < 0 || window < 0 || sink >= (1 << 30) || window >= (1 << 30)) return -1;
   return qcache_attend_ws_bytes(B, H, kv_heads <= 0 ? H : kv_heads, head_dim, sink + window);
 }
 

@@ -129,7 +129,7 @@ def dtype_code(dt: torch.dtype) -> int:
 def stream_ptr(device: torch.device) -> int:
     """torch's current ``cudaStream_t`` on ``device`` (without a Stream object around it, which
     costs 2 us, a fifth of a decode call, where the device has an index)."""
-    index = getattr(device, "index", None)
+    index = device.index if isinstance(device, torch.device) else None
     if index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return torch._C._cuda_getCurrentRawStream(index)

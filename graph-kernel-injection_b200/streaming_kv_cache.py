@@ -152,15 +152,32 @@ class QuantizedStreamingKVCache:
         code, code_dtype = _FORMATS[fmt]
         self._k = torch.zeros(batch, heads, rows, row_bytes, dtype=torch.uint8, device=dev)
         self._v = torch.zeros_like(self._k)
-        self.k = self._k[..., :head_dim].view(code_dtype)
-        self.v = self._v[..., :head_dim].view(code_dtype)
-        self.scales = torch.zeros(batch, heads, rows, 2, dtype=torch.uint8, device=dev)
-        self.lengths = torch.zeros(batch, dtype=torch.int64, device=dev)
+        self._state = (self._k[..., :head_dim].view(code_dtype),
+                       self._v[..., :head_dim].view(code_dtype),
+                       torch.zeros(batch, heads, rows, 2, dtype=torch.uint8, device=dev),
+                       torch.zeros(batch, dtype=torch.int64, device=dev))
         self._tickets = torch.zeros(batch, dtype=torch.int32, device=dev)
         self._codes = (native.dtype_code(dtype), code)
         self._scratch = {}   # scratch bytes of attend by the number of query heads
         self._cache_ptrs = (self._k.data_ptr(), self._v.data_ptr(), self.scales.data_ptr(),
                             self.lengths.data_ptr())
+
+    # the tensors themselves, whose addresses the kernels hold: written to, never replaced
+    @property
+    def k(self) -> torch.Tensor:
+        return self._state[0]
+
+    @property
+    def v(self) -> torch.Tensor:
+        return self._state[1]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._state[2]
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        return self._state[3]
 
     @property
     def memory_bytes(self) -> int:

@@ -390,5 +390,7 @@ def test_refusals():
         c.attend(q.requires_grad_(True))
     with torch.no_grad():
         assert not c.attend(q).any()
+    with pytest.raises(AttributeError):
+        c.lengths = c.lengths + 1
     c.append(x[:, :, :0], x[:, :, :0])
     assert not c.lengths.any()

@@ -24,7 +24,8 @@ def append(L, B=1, H=1, D=64, dtype=native.BF16, fmt=0, sink=4, window=8, n=1, k
 @pytest.mark.parametrize("kw,rc,word", [
     (dict(dtype=native.F32), UNSUPPORTED, "float16"), (dict(fmt=2), INVALID, "format"),
     (dict(B=0), INVALID, "positive"), (dict(H=0), INVALID, "positive"),
-    (dict(B=65536), UNSUPPORTED, "65535"), (dict(D=0), UNSUPPORTED, "head_dim"),
+    (dict(B=65536), UNSUPPORTED, "65535"), (dict(H=1 << 60), UNSUPPORTED, "heads"),
+    (dict(sink=1 << 62, window=1 << 62), INVALID, "2^30"), (dict(D=0), UNSUPPORTED, "head_dim"),
     (dict(D=60), UNSUPPORTED, "head_dim"), (dict(D=264), UNSUPPORTED, "head_dim"),
     (dict(sink=-1), INVALID, "non-negative"), (dict(sink=0, window=0), INVALID, "2^30"),
     (dict(window=1 << 30), INVALID, "2^30"), (dict(k=None), INVALID, "NULL"),
@@ -115,7 +116,8 @@ def test_sizes():
     assert L.sbfa_qcache_attend_workspace_bytes(2, 4, 2, 64, 4, 8) == 0
     assert L.sbfa_qcache_attend_workspace_bytes(300, 4, 2, 64, 4, 9999) > 0
     for bad in ((2, 3, 2, 64, 4, 8), (2, 4, 2, 60, 4, 8), (0, 4, 2, 64, 4, 8),
-                (2, 4, 2, 64, 0, 0)):
+                (2, 4, 2, 64, 0, 0), (2, 1 << 60, 1 << 59, 64, 4, 8), (2, 4, 2, 64, 1 << 62, 8),
+                (1 << 40, 4, 2, 64, 4, 8)):
         assert L.sbfa_qcache_attend_workspace_bytes(*bad) == -1
 
 
