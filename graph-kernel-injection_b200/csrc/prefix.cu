@@ -923,9 +923,8 @@ int check_prefix(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P,
   return SBFA_OK;
 }
 
-int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 int64_t own_bytes(int64_t B, int64_t H, int64_t d) {
-  return align256(B * H * (d + 1) * (int64_t)sizeof(float));
+  return (B * H * (d + 1) * (int64_t)sizeof(float) + 255) / 256 * 256;
 }
 
 }  // namespace
@@ -966,40 +965,31 @@ extern "C" int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const
   return launch_call(c, geo, dtype);
 }
 
-extern "C" int64_t sbfa_qcache_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
-                                                      int64_t P, int64_t head_dim, int64_t sink,
-                                                      int64_t window) {
-  if (sink < 0 || window < 0 || sink >= (1 << 30) || window >= (1 << 30)) return -1;
-  const int64_t rows = sink + window;
+extern "C" int64_t sbfa_qcache_prefix_workspace_bytes(const sbfa_qcache* cache, int64_t H,
+                                                      int64_t P) {
+  const int64_t bytes = qcache_attend_ws_bytes(cache, H);
   PrefixGeom geo;
-  if (!prefix_geometry(B, H, kv_heads, 1, P, head_dim, 0, &geo)) return -1;
-  const int64_t cache = qcache_attend_ws_bytes(B, H, geo.kv_heads, head_dim, rows);
-  if (cache < 0) return -1;
-  return ws_bytes_of(geo) + own_bytes(B, H, head_dim) + align256(cache);
+  if (bytes < 0 || !prefix_geometry(cache->batch, H, cache->kv_heads, 1, P, cache->head_dim, 0, &geo))
+    return -1;
+  return own_bytes(cache->batch, H, cache->head_dim) + ws_bytes_of(geo) + bytes;
 }
 
-extern "C" int sbfa_qcache_prefix_attend(
-    const void* q, const void* k_codes, const void* v_codes, const void* scales,
-    const int64_t* lengths, const void* k_prefix, const void* v_prefix, void* o, float* lse,
-    int64_t B, int64_t H, int64_t kv_heads, int64_t P, int64_t head_dim, int dtype, int fmt,
-    double softmax_scale, int64_t sink, int64_t window, void* ws, int64_t ws_bytes,
-    void* stream) {
+extern "C" int sbfa_qcache_prefix_attend(const sbfa_qcache* cache, const void* q,
+                                         const void* k_prefix, const void* v_prefix, int64_t P,
+                                         void* o, float* lse, int64_t H, double softmax_scale,
+                                         void* ws, int64_t ws_bytes, void* stream) {
+  if (cache == nullptr) return fail(SBFA_ERR_INVALID, "8-bit cache: NULL cache");
+  const int64_t B = cache->batch, head_dim = cache->head_dim;
   PrefixGeom geo;
-  if (int rc = check_prefix(B, H, kv_heads, 1, P, head_dim, dtype, 0, &geo)) return rc;
-  const int64_t need =
-      sbfa_qcache_prefix_workspace_bytes(B, H, kv_heads, P, head_dim, sink, window);
-  if (need < 0)
-    return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: sizes out of the cache's range");
-  if (ws == nullptr || ws_bytes < need)
-    return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: workspace too small (need " +
-                                      std::to_string(need) + " bytes)");
+  if (int rc = check_prefix(B, H, cache->kv_heads, 1, P, head_dim, cache->dtype, 0, &geo)) return rc;
   // the cache's own result in fp32 [B, H, d] and its LSE [B, H], the prefix's scratch, the cache's
   const int64_t own = own_bytes(B, H, head_dim), pre = ws_bytes_of(geo);
+  if (ws == nullptr || ws_bytes < own + pre)
+    return fail(SBFA_ERR_INVALID, "sbfa_qcache_prefix_attend: workspace too small");
   float* own_o = (float*)ws;
   float* own_lse = own_o + B * H * head_dim;
-  const QAttend a{q, k_codes, v_codes, scales, lengths, nullptr, own_o, own_lse, B, H,
-                  geo.kv_heads, head_dim, dtype, fmt, softmax_scale, sink, window,
-                  (char*)ws + own + pre, need - own - pre, (cudaStream_t)stream};
+  const QAttend a{cache, q, nullptr, own_o, own_lse, H, softmax_scale, (char*)ws + own + pre,
+                  ws_bytes - own - pre, (cudaStream_t)stream};
   PrefixCall c = {};
   c.q = q;
   c.k = k_prefix;
@@ -1016,7 +1006,7 @@ extern "C" int sbfa_qcache_prefix_attend(
   if (int rc = qcache_attend_check(a)) return rc;
   if (int rc = check_call(c, nullptr, geo, H, softmax_scale, pre)) return rc;
   if (int rc = qcache_attend_launch(a)) return rc;
-  return launch_call(c, geo, dtype);
+  return launch_call(c, geo, cache->dtype);
 }
 
 extern "C" int sbfa_prefix_prompt(const void* q, const void* k, const void* v,

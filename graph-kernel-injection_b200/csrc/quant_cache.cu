@@ -1072,34 +1072,40 @@ int padded_dim(int64_t d) {
   return d <= 64 ? 64 : d <= 128 ? 128 : 256;
 }
 
-int check_qcache(const void* k, const void* v, const void* scales, const void* lengths, int64_t B,
-                 int64_t H, int64_t D, int dtype, int fmt, int64_t sink, int64_t window) {
-  if (dtype != SBFA_F16 && dtype != SBFA_BF16)
+// Geometry of a cache (no pointers).
+int check_geometry(const sbfa_qcache* c) {
+  if (c == nullptr) return fail(SBFA_ERR_INVALID, "8-bit cache: NULL cache");
+  if (c->dtype != SBFA_F16 && c->dtype != SBFA_BF16)
     return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: dtype must be float16 or bfloat16");
-  if (fmt != SBFA_Q_E4M3 && fmt != SBFA_Q_INT8)
+  if (c->fmt != SBFA_Q_E4M3 && c->fmt != SBFA_Q_INT8)
     return fail(SBFA_ERR_INVALID, "8-bit cache: unknown format code");
-  if (B <= 0 || H <= 0) return fail(SBFA_ERR_INVALID, "B and H must be positive");
-  if (B > 65535 || H >= (1 << 24))
+  if (c->batch <= 0 || c->kv_heads <= 0)
+    return fail(SBFA_ERR_INVALID, "batch and kv_heads must be positive");
+  if (c->batch > 65535 || c->kv_heads >= (1 << 24))
     return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: at most 65535 sequences and 2^24 heads");
-  if (padded_dim(D) == 0)
+  if (padded_dim(c->head_dim) == 0)
     return fail(SBFA_ERR_UNSUPPORTED,
                 "8-bit cache: head_dim must be a multiple of 8 and at most 256");
-  if (sink < 0 || window < 0)
+  if (c->sink < 0 || c->window < 0)
     return fail(SBFA_ERR_INVALID, "sink_size and window_size must be non-negative");
-  if (sink >= (1ll << 30) || window >= (1ll << 30) || sink + window <= 0 ||
-      sink + window >= (1ll << 30))
+  if (c->sink >= (1ll << 30) || c->window >= (1ll << 30) || c->sink + c->window <= 0 ||
+      c->sink + c->window >= (1ll << 30))
     return fail(SBFA_ERR_INVALID, "sink_size + window_size must be in [1, 2^30)");
-  if (!k || !v || !scales || !lengths)
-    return fail(SBFA_ERR_INVALID, "8-bit cache: NULL cache pointer");
-  if (((uintptr_t)k | (uintptr_t)v) & 15u)
+  return SBFA_OK;
+}
+
+int check_qcache(const sbfa_qcache* c) {
+  if (int rc = check_geometry(c)) return rc;
+  if (!c->k_codes || !c->v_codes || !c->scales || !c->lengths)
+    return fail(SBFA_ERR_INVALID, "8-bit cache: NULL cache tensor");
+  if (((uintptr_t)c->k_codes | (uintptr_t)c->v_codes) & 15u)
     return fail(SBFA_ERR_INVALID, "8-bit cache: tensors must be 16-byte aligned");
   return SBFA_OK;
 }
 
-QCache make_cache(void* k, void* v, void* scales, int64_t H, int64_t D, int64_t sink,
-                  int64_t window) {
-  return QCache{(uint8_t*)k, (uint8_t*)v, (uint16_t*)scales, H, sink + window, sink, window,
-                (int)D};
+QCache device_view(const sbfa_qcache* c) {
+  return QCache{(uint8_t*)c->k_codes, (uint8_t*)c->v_codes, (uint16_t*)c->scales, c->kv_heads,
+                c->sink + c->window, c->sink, c->window, (int)c->head_dim};
 }
 
 template <typename F>
@@ -1196,7 +1202,7 @@ int launch_attend(const QAttend& a, const QCache& c, const AttPlan& p) {
   ws.rec = (FlatRecord*)a.ws;
   ws.stats = (float*)(ws.rec + p.grid);
   ws.part = ws.stats + (int64_t)p.grid * 2 * 3 * C::kRowsQ;
-  const int group = (int)(a.H / a.kv_heads);
+  const int group = (int)(a.H / c.heads);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.grid);
   cfg.blockDim = dim3(kAttWarps * 32);
@@ -1211,8 +1217,9 @@ int launch_attend(const QAttend& a, const QCache& c, const AttPlan& p) {
   {
     LaunchScope ls("qcache_attend_kernel", a.stream);
     if (int rc = check_cuda(
-            cudaLaunchKernelEx(&cfg, kern, (const T*)a.q, c, a.lengths, (T*)a.o, a.o32, a.lse,
-                               (float)a.scale * kLog2e, group, p.chunks, p.ns, (int)a.B, ws),
+            cudaLaunchKernelEx(&cfg, kern, (const T*)a.q, c, (const int64_t*)a.cache->lengths, (T*)a.o,
+                               a.o32, a.lse, (float)a.scale * kLog2e, group, p.chunks, p.ns,
+                               (int)a.cache->batch, ws),
             "qcache_attend_kernel"))
       return rc;
   }
@@ -1232,89 +1239,82 @@ using namespace sbfa;
 
 extern "C" int64_t sbfa_qcache_row_bytes(int64_t head_dim) { return padded_dim(head_dim); }
 
-extern "C" int sbfa_qcache_append(void* k_codes, void* v_codes, void* scales, int64_t* lengths,
-                                  int32_t* tickets, const void* k_new, const void* v_new,
-                                  const int64_t* strides, const int64_t* counts, int64_t B,
-                                  int64_t H, int64_t head_dim, int dtype, int fmt, int64_t sink,
-                                  int64_t window, int64_t n_new, void* stream) {
-  if (int rc = check_qcache(k_codes, v_codes, scales, lengths, B, H, head_dim, dtype, fmt, sink,
-                            window))
-    return rc;
+extern "C" int sbfa_qcache_append(const sbfa_qcache* cache, const void* k_new, const void* v_new,
+                                  const int64_t* strides, const int64_t* counts, int64_t n_new,
+                                  void* stream) {
+  if (int rc = check_qcache(cache)) return rc;
   if (n_new < 0 || n_new >= (1ll << 31))
     return fail(SBFA_ERR_INVALID, "sbfa_qcache_append: n_new must be in [0, 2^31)");
   if (n_new == 0) return SBFA_OK;
-  if (!k_new || !v_new || !tickets)
+  if (!k_new || !v_new || !cache->tickets)
     return fail(SBFA_ERR_INVALID, "sbfa_qcache_append: NULL tensor pointer");
+  const int64_t H = cache->kv_heads, d = cache->head_dim;
   Strides3 st[2];
   for (int i = 0; i < 2; ++i) {
     st[i] = strides ? Strides3{strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}
-                    : Strides3{H * n_new * head_dim, n_new * head_dim, head_dim};
+                    : Strides3{H * n_new * d, n_new * d, d};
     if (st[i].b < 0 || st[i].h < 0 || st[i].n < 0 || st[i].b % 8 || st[i].h % 8 || st[i].n % 8)
       return fail(SBFA_ERR_INVALID, "sbfa_qcache_append: strides must be non-negative multiples "
                                     "of 8 elements");
   }
   if (((uintptr_t)k_new | (uintptr_t)v_new) & 15u)
     return fail(SBFA_ERR_INVALID, "sbfa_qcache_append: tensors must be 16-byte aligned");
-  const QCache c = make_cache(k_codes, v_codes, scales, H, head_dim, sink, window);
+  const QCache c = device_view(cache);
   cudaStream_t s = (cudaStream_t)stream;
-  return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
+  return by_format(cache->dtype, cache->fmt, d, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
     RowGrid g;
-    if (int rc = row_grid(B, H, std::min(n_new, c.rows), kAppThreads / app_lanes(dp.value), 1, 2,
-                          5 * kAppRounds, &g))
+    if (int rc = row_grid(cache->batch, H, std::min(n_new, c.rows),
+                          kAppThreads / app_lanes(dp.value), 1, 2, 5 * kAppRounds, &g))
       return rc;
     LaunchScope ls("qcache_append_kernel", s);
     qcache_append_kernel<T, m.value, dp.value><<<g.grid, kAppThreads, 0, s>>>(
-        c, lengths, tickets, (const T*)k_new, (const T*)v_new, st[0], st[1], counts, (int)n_new,
-        g.head_blocks, g.hs);
+        c, cache->lengths, cache->tickets, (const T*)k_new, (const T*)v_new, st[0], st[1], counts,
+        (int)n_new, g.head_blocks, g.hs);
     return check_launch("qcache_append_kernel");
   });
 }
 
-extern "C" int sbfa_qcache_read(const void* k_codes, const void* v_codes, const void* scales,
-                                const int64_t* lengths, void* k_out, void* v_out,
-                                int64_t* positions, int64_t B, int64_t H, int64_t head_dim,
-                                int dtype, int fmt, int64_t sink, int64_t window, void* stream) {
-  if (int rc = check_qcache(k_codes, v_codes, scales, lengths, B, H, head_dim, dtype, fmt, sink,
-                            window))
-    return rc;
+extern "C" int sbfa_qcache_read(const sbfa_qcache* cache, void* k_out, void* v_out,
+                                int64_t* positions, void* stream) {
+  if (int rc = check_qcache(cache)) return rc;
   if (!k_out || !v_out || !positions)
     return fail(SBFA_ERR_INVALID, "sbfa_qcache_read: NULL tensor pointer");
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15u)
     return fail(SBFA_ERR_INVALID, "sbfa_qcache_read: tensors must be 16-byte aligned");
-  const QCache c = make_cache(const_cast<void*>(k_codes), const_cast<void*>(v_codes),
-                              const_cast<void*>(scales), H, head_dim, sink, window);
+  const QCache c = device_view(cache);
   cudaStream_t s = (cudaStream_t)stream;
-  return by_format(dtype, fmt, head_dim, [&](auto t, auto m, auto dp) {
+  return by_format(cache->dtype, cache->fmt, cache->head_dim, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
     constexpr int G = dp.value / 8;
     RowGrid g;
-    if (int rc = row_grid(B, H, c.rows, kReadThreads / G, kReadUnroll, 1,
-                          4 * kReadRounds, &g)) return rc;
+    if (int rc = row_grid(cache->batch, c.heads, c.rows, kReadThreads / G, kReadUnroll, 1,
+                          4 * kReadRounds, &g))
+      return rc;
     LaunchScope ls("qcache_read_kernel", s);
     qcache_read_kernel<T, m.value, G><<<g.grid, kReadThreads, 0, s>>>(
-        c, lengths, (T*)k_out, (T*)v_out, positions, g.head_blocks, g.hs);
+        c, cache->lengths, (T*)k_out, (T*)v_out, positions, g.head_blocks, g.hs);
     return check_launch("qcache_read_kernel");
   });
 }
 
 namespace sbfa {
-int64_t qcache_attend_ws_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t d, int64_t rows) {
+// The plan of a call over H query heads.
+static int plan_for(const sbfa_qcache* c, int64_t H, AttPlan* p) {
+  if (H <= 0 || H % c->kv_heads != 0)
+    return fail(SBFA_ERR_INVALID, "the query head count must be a multiple of kv_heads");
+  if (H / c->kv_heads >= (1 << 20)) return fail(SBFA_ERR_UNSUPPORTED, "too many query heads");
+  return attend_plan(c->batch, c->kv_heads, H / c->kv_heads, c->head_dim, c->sink + c->window, p);
+}
+
+int64_t qcache_attend_ws_bytes(const sbfa_qcache* cache, int64_t H) {
   AttPlan p;
-  if (B <= 0 || B > 65535 || H <= 0 || kv_heads <= 0 || kv_heads >= (1 << 24) ||
-      H % kv_heads != 0 || H / kv_heads >= (1 << 20) || padded_dim(d) == 0 || rows <= 0 ||
-      rows >= (1 << 30) || attend_plan(B, kv_heads, H / kv_heads, d, rows, &p) != SBFA_OK)
-    return -1;
+  if (check_geometry(cache) != SBFA_OK || plan_for(cache, H, &p) != SBFA_OK) return -1;
   return p.ws_bytes;
 }
 
 int qcache_attend_check(const QAttend& a) {
-  if (int rc = check_qcache(a.k, a.v, a.scales, a.lengths, a.B, a.kv_heads, a.d, a.dtype, a.fmt,
-                            a.sink, a.window))
-    return rc;
-  if (a.H <= 0 || a.H % a.kv_heads != 0)
-    return fail(SBFA_ERR_INVALID, "the query head count must be a multiple of kv_heads");
-  if (a.H / a.kv_heads >= (1 << 20)) return fail(SBFA_ERR_UNSUPPORTED, "too many query heads");
+  if (int rc = check_qcache(a.cache)) return rc;
   if (!(a.scale > 0) || a.scale > 1e30)
     return fail(SBFA_ERR_INVALID, "softmax_scale must be positive and finite");
   if (!a.q || (!a.o && !a.o32))
@@ -1322,8 +1322,7 @@ int qcache_attend_check(const QAttend& a) {
   if (((uintptr_t)a.q | (uintptr_t)a.o | (uintptr_t)a.o32 | (uintptr_t)a.ws) & 15u)
     return fail(SBFA_ERR_INVALID, "8-bit cache: tensors must be 16-byte aligned");
   AttPlan p;
-  if (int rc = attend_plan(a.B, a.kv_heads, a.H / a.kv_heads, a.d, a.sink + a.window, &p))
-    return rc;
+  if (int rc = plan_for(a.cache, a.H, &p)) return rc;
   if (p.ws_bytes > 0 && (a.ws == nullptr || a.ws_bytes < p.ws_bytes))
     return fail(SBFA_ERR_INVALID, "8-bit cache: workspace too small (need " +
                                       std::to_string(p.ws_bytes) + " bytes)");
@@ -1331,11 +1330,10 @@ int qcache_attend_check(const QAttend& a) {
 }
 
 int qcache_attend_launch(const QAttend& a) {
-  const QCache c = make_cache(const_cast<void*>(a.k), const_cast<void*>(a.v),
-                              const_cast<void*>(a.scales), a.kv_heads, a.d, a.sink, a.window);
+  const QCache c = device_view(a.cache);
   AttPlan p;
-  if (int rc = attend_plan(a.B, a.kv_heads, a.H / a.kv_heads, a.d, c.rows, &p)) return rc;
-  return by_format(a.dtype, a.fmt, a.d, [&](auto t, auto m, auto dp) {
+  if (int rc = plan_for(a.cache, a.H, &p)) return rc;
+  return by_format(a.cache->dtype, a.cache->fmt, a.cache->head_dim, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
     constexpr int DP = dp.value;
     if constexpr (DP <= 128) {
@@ -1349,21 +1347,14 @@ int qcache_attend_launch(const QAttend& a) {
 }
 }  // namespace sbfa
 
-extern "C" int64_t sbfa_qcache_attend_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
-                                                      int64_t head_dim, int64_t sink,
-                                                      int64_t window) {
-  if (sink < 0 || window < 0 || sink >= (1 << 30) || window >= (1 << 30)) return -1;
-  return qcache_attend_ws_bytes(B, H, kv_heads <= 0 ? H : kv_heads, head_dim, sink + window);
+extern "C" int64_t sbfa_qcache_attend_workspace_bytes(const sbfa_qcache* cache, int64_t H) {
+  return qcache_attend_ws_bytes(cache, H);
 }
 
-extern "C" int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
-                                  const void* scales, const int64_t* lengths, void* o, float* lse,
-                                  int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim,
-                                  int dtype, int fmt, double softmax_scale, int64_t sink,
-                                  int64_t window, void* ws, int64_t ws_bytes, void* stream) {
-  const QAttend a{q,  k_codes,  v_codes,  scales, lengths, o,    nullptr, lse, B, H,
-                  kv_heads <= 0 ? H : kv_heads, head_dim, dtype, fmt, softmax_scale, sink, window,
-                  ws, ws_bytes, (cudaStream_t)stream};
+extern "C" int sbfa_qcache_attend(const sbfa_qcache* cache, const void* q, void* o, float* lse,
+                                  int64_t H, double softmax_scale, void* ws, int64_t ws_bytes,
+                                  void* stream) {
+  const QAttend a{cache, q, o, nullptr, lse, H, softmax_scale, ws, ws_bytes, (cudaStream_t)stream};
   if (int rc = qcache_attend_check(a)) return rc;
   return qcache_attend_launch(a);
 }

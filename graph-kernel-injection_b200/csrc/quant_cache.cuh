@@ -21,21 +21,18 @@ struct QCache {
 // One attend call.  The result goes to o (16 bits, LSE 0 for an empty sequence) or, where o32 is
 // given, unrounded to o32 with LSE -inf for an empty sequence.
 struct QAttend {
+  const sbfa_qcache* cache;
   const void* q;
-  const void *k, *v, *scales;
-  const int64_t* lengths;
   void* o;
   float *o32, *lse;
-  int64_t B, H, kv_heads, d;
-  int dtype, fmt;
+  int64_t H;
   double scale;
-  int64_t sink, window;
   void* ws;
   int64_t ws_bytes;
   cudaStream_t stream;
 };
 // Scratch of a call, -1 for a bad shape.
-int64_t qcache_attend_ws_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t d, int64_t rows);
+int64_t qcache_attend_ws_bytes(const sbfa_qcache* cache, int64_t H);
 int qcache_attend_check(const QAttend& a);   // an SBFA_ERR_* code; launches nothing
 int qcache_attend_launch(const QAttend& a);  // after the check
 

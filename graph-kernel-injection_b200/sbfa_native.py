@@ -30,6 +30,14 @@ _lock = threading.Lock()
 
 _i64, _i32, _f64, _vp = ctypes.c_int64, ctypes.c_int, ctypes.c_double, ctypes.c_void_p
 
+class QCache(ctypes.Structure):
+    """``struct sbfa_qcache``: an 8-bit ring cache."""
+
+    _fields_ = ([(n, _vp) for n in ("k_codes", "v_codes", "scales", "lengths", "tickets")]
+                + [(n, _i64) for n in ("batch", "kv_heads", "head_dim", "sink", "window")]
+                + [("dtype", ctypes.c_int32), ("fmt", ctypes.c_int32)])
+
+
 _SIGNATURES = {
     "sbfa_abi_version": ([], _i32),
     "sbfa_last_error": ([ctypes.c_char_p, ctypes.c_size_t], _i32),
@@ -63,19 +71,15 @@ _SIGNATURES = {
     "sbfa_ring_decode_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64], _i64),
     "sbfa_decode_supported": ([_i32, _i64], _i32),
     "sbfa_qcache_row_bytes": ([_i64], _i64),
-    "sbfa_qcache_append": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32,
-                            _i32, _i64, _i64, _i64, _vp], _i32),
-    "sbfa_qcache_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32,
-                            _f64, _i64, _i64, _vp, _i64, _vp], _i32),
-    "sbfa_qcache_attend_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
-    "sbfa_qcache_read": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i64,
-                          _i64, _vp], _i32),
+    "sbfa_qcache_append": ([_vp, _vp, _vp, _vp, _vp, _i64, _vp], _i32),
+    "sbfa_qcache_attend": ([_vp, _vp, _vp, _vp, _i64, _f64, _vp, _i64, _vp], _i32),
+    "sbfa_qcache_attend_workspace_bytes": ([_vp, _i64], _i64),
+    "sbfa_qcache_read": ([_vp, _vp, _vp, _vp, _vp], _i32),
+    "sbfa_qcache_prefix_attend": ([_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _f64, _vp, _i64,
+                                   _vp], _i32),
+    "sbfa_qcache_prefix_workspace_bytes": ([_vp, _i64, _i64], _i64),
     "sbfa_prefix_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                             _i64, _i32, _f64, _vp, _i64, _vp], _i32),
-    "sbfa_qcache_prefix_attend": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
-                                   _i64, _i64, _i32, _i32, _f64, _i64, _i64, _vp, _i64, _vp],
-                                  _i32),
-    "sbfa_qcache_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "sbfa_prefix_prompt": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                             _i64, _i32, _f64, _i64, _vp, _i64, _vp], _i32),
     "sbfa_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64], _i64),

@@ -138,13 +138,11 @@ class SharedPrefix:
             need = self._scratch.get(sizes)
             if need is None:
                 need = self._remember(sizes, native.lib().sbfa_qcache_prefix_workspace_bytes(
-                    B, H, self.heads, self.length, self.head_dim, cache.sink_size,
-                    cache.window_size))
+                    cache._handle, H, self.length))
             ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
             native.check(native.lib().sbfa_qcache_prefix_attend(
-                q.data_ptr(), *cache._cache_ptrs, self.k.data_ptr(), self.v.data_ptr(),
-                o.data_ptr(), native.ptr(lse), B, H, self.heads, self.length, self.head_dim,
-                *cache._codes, scale, cache.sink_size, cache.window_size, ws.data_ptr(), need,
+                cache._handle, q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.length,
+                o.data_ptr(), native.ptr(lse), H, scale, ws.data_ptr(), need,
                 native.stream_ptr(dev)), "qcache_prefix_attend")
         return (o, lse) if return_lse else o
 

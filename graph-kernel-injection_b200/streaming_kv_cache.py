@@ -18,6 +18,7 @@ every sequence of the batch has before its own and that are held once.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional, Tuple
 
@@ -157,10 +158,12 @@ class QuantizedStreamingKVCache:
                        torch.zeros(batch, heads, rows, 2, dtype=torch.uint8, device=dev),
                        torch.zeros(batch, dtype=torch.int64, device=dev))
         self._tickets = torch.zeros(batch, dtype=torch.int32, device=dev)
-        self._codes = (native.dtype_code(dtype), code)
         self._scratch = {}   # scratch bytes of attend by the number of query heads
-        self._cache_ptrs = (self._k.data_ptr(), self._v.data_ptr(), self.scales.data_ptr(),
-                            self.lengths.data_ptr())
+        self._struct = native.QCache(
+            self._k.data_ptr(), self._v.data_ptr(), self.scales.data_ptr(),
+            self.lengths.data_ptr(), self._tickets.data_ptr(), batch, heads, head_dim, sink_size,
+            window_size, native.dtype_code(dtype), code)
+        self._handle = ctypes.addressof(self._struct)
 
     # the tensors themselves, whose addresses the kernels hold: written to, never replaced
     @property
@@ -210,12 +213,9 @@ class QuantizedStreamingKVCache:
             return
         k_new, v_new = vector_readable(k_new), vector_readable(v_new)
         strides = stride_array(k_new.stride()[:3] + v_new.stride()[:3])
-        k, v, scales, lengths = self._cache_ptrs
         with native.device_guard(self.device):
             native.check(native.lib().sbfa_qcache_append(
-                k, v, scales, lengths, self._tickets.data_ptr(), k_new.data_ptr(),
-                v_new.data_ptr(), strides, native.ptr(counts), self.batch, self.heads,
-                self.head_dim, *self._codes, self.sink_size, self.window_size, n,
+                self._handle, k_new.data_ptr(), v_new.data_ptr(), strides, native.ptr(counts), n,
                 native.stream_ptr(self.device)), "qcache_append")
 
     def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
@@ -243,14 +243,12 @@ class QuantizedStreamingKVCache:
             need = self._scratch.get(hq)
             if need is None:
                 need = self._scratch[hq] = native.lib().sbfa_qcache_attend_workspace_bytes(
-                    self.batch, hq, self.heads, self.head_dim, self.sink_size, self.window_size)
+                    self._handle, hq)
             # from torch's allocator, so of the call's stream or graph
             ws = (torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None)
             native.check(native.lib().sbfa_qcache_attend(
-                q.data_ptr(), *self._cache_ptrs, o.data_ptr(), native.ptr(lse), self.batch, hq,
-                self.heads, self.head_dim, *self._codes, scale, self.sink_size,
-                self.window_size, native.ptr(ws), need, native.stream_ptr(self.device)),
-                "qcache_attend")
+                self._handle, q.data_ptr(), o.data_ptr(), native.ptr(lse), hq, scale,
+                native.ptr(ws), need, native.stream_ptr(self.device)), "qcache_attend")
         return (o, lse) if return_lse else o
 
     def read(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -264,8 +262,7 @@ class QuantizedStreamingKVCache:
         positions = torch.empty(self.batch, rows, dtype=torch.int64, device=self.device)
         with native.device_guard(self.device):
             native.check(native.lib().sbfa_qcache_read(
-                *self._cache_ptrs, k.data_ptr(), v.data_ptr(), positions.data_ptr(), self.batch,
-                self.heads, self.head_dim, *self._codes, self.sink_size, self.window_size,
+                self._handle, k.data_ptr(), v.data_ptr(), positions.data_ptr(),
                 native.stream_ptr(self.device)), "qcache_read")
         return k, v, positions
 

@@ -295,12 +295,8 @@ int64_t sbfa_ring_decode_workspace_bytes(int64_t B, int64_t H, int64_t head_dim,
  * step moves on when it is replayed, and (c) kv_heads key/value heads shared by
  * groups of query heads.
  *
- * Cache tensors, all contiguous, 16-byte aligned, owned by the caller:
- *   k_codes, v_codes: 8-bit [B, kv_heads, sink + window, DP],
- *     DP = sbfa_qcache_row_bytes(head_dim); the columns behind head_dim hold 0;
- *   scales: uint8 [B, kv_heads, sink + window, 2], K's byte and V's;
- *   lengths: int64 [B], tokens appended to each sequence;
- *   tickets: int32 [B], zero before the first append and after each one.
+ * A cache is described by struct sbfa_qcache below; its tensors are contiguous, 16-byte
+ * aligned and owned by the caller, the struct itself is only read during a call.
  * A row x is stored with e = the least integer >= -126 such that
  * max|x| <= top * 2^e (top: 448 for SBFA_Q_E4M3, 127 for SBFA_Q_INT8; e = 0 for a
  * row of zeros) as the byte e + 127 and the codes of x * 2^-e rounded to
@@ -312,46 +308,49 @@ int64_t sbfa_ring_decode_workspace_bytes(int64_t B, int64_t H, int64_t head_dim,
  * sink + window)).
  * ------------------------------------------------------------------------- */
 
+struct sbfa_qcache {
+  void* k_codes;      /* 8-bit [batch, kv_heads, sink + window, DP], DP = */
+  void* v_codes;      /*   sbfa_qcache_row_bytes(head_dim); columns behind head_dim hold 0 */
+  void* scales;       /* uint8 [batch, kv_heads, sink + window, 2], K's byte and V's */
+  int64_t* lengths;   /* [batch], tokens appended to each sequence */
+  int32_t* tickets;   /* [batch], zero before the first append and after each one */
+  int64_t batch, kv_heads, head_dim, sink, window;
+  int32_t dtype, fmt; /* enum sbfa_dtype, enum sbfa_qformat */
+};
+
 /* DP for this head_dim (64, 128 or 256), 0 when it is not supported. */
 int64_t sbfa_qcache_row_bytes(int64_t head_dim);
 
 /* Quantises the next tokens of every sequence into their ring rows and adds
- * their number to lengths.  k_new, v_new: logical [B, kv_heads, n_new, head_dim];
+ * their number to lengths.  k_new, v_new: logical [batch, kv_heads, n_new, head_dim];
  * strides: (batch, head, row) element strides of k_new then v_new, non-negative
- * multiples of 8, or NULL for contiguous tensors.  counts: int64[B] on the
+ * multiples of 8, or NULL for contiguous tensors.  counts: int64[batch] on the
  * device, how many of the n_new tokens each sequence takes (clamped to [0,
  * n_new]), or NULL for all; rows behind a count are not read.  Two appends to one cache
  * must not run at the same time. */
-int sbfa_qcache_append(void* k_codes, void* v_codes, void* scales, int64_t* lengths,
-                       int32_t* tickets, const void* k_new, const void* v_new,
-                       const int64_t* strides, const int64_t* counts, int64_t B,
-                       int64_t kv_heads, int64_t head_dim, int dtype, int fmt, int64_t sink,
-                       int64_t window, int64_t n_new, void* stream);
+int sbfa_qcache_append(const struct sbfa_qcache* cache, const void* k_new, const void* v_new,
+                       const int64_t* strides, const int64_t* counts, int64_t n_new,
+                       void* stream);
 
 /* Attention of each sequence's query at its last position over its visible
- * rows.  q: contiguous [B, H, head_dim], H a multiple of kv_heads (<= 0 means H);
- * o: the same shape and dtype; lse (may be NULL): fp32 [B, H].  A sequence of
+ * rows.  q: contiguous [batch, H, head_dim], H a multiple of kv_heads;
+ * o: the same shape and dtype; lse (may be NULL): fp32 [batch, H].  A sequence of
  * length 0 gives O = 0 and LSE = 0.  softmax_scale > 0.  ws: 16-byte aligned
  * caller scratch of sbfa_qcache_attend_workspace_bytes() bytes. */
-int sbfa_qcache_attend(const void* q, const void* k_codes, const void* v_codes,
-                       const void* scales, const int64_t* lengths, void* o, float* lse,
-                       int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim, int dtype,
-                       int fmt, double softmax_scale, int64_t sink, int64_t window, void* ws,
-                       int64_t ws_bytes, void* stream);
+int sbfa_qcache_attend(const struct sbfa_qcache* cache, const void* q, void* o, float* lse,
+                       int64_t H, double softmax_scale, void* ws, int64_t ws_bytes,
+                       void* stream);
 
 /* Scratch bytes sbfa_qcache_attend needs on the current device (may be 0; ws may then be
  * NULL), -1 for a bad shape. */
-int64_t sbfa_qcache_attend_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads,
-                                           int64_t head_dim, int64_t sink, int64_t window);
+int64_t sbfa_qcache_attend_workspace_bytes(const struct sbfa_qcache* cache, int64_t H);
 
 /* The kept rows as 16-bit values in order of position: out row i of a sequence
  * is its i-th kept position (sinks, then the window from its oldest), positions[b, i] that
- * position; rows behind the last are zero with position -1.  k_out, v_out:
- * contiguous [B, kv_heads, sink + window, head_dim]; positions: int64 [B, sink + window]. */
-int sbfa_qcache_read(const void* k_codes, const void* v_codes, const void* scales,
-                     const int64_t* lengths, void* k_out, void* v_out, int64_t* positions,
-                     int64_t B, int64_t kv_heads, int64_t head_dim, int dtype, int fmt,
-                     int64_t sink, int64_t window, void* stream);
+ * position; rows behind the last are zero with position -1.  k_out, v_out: contiguous
+ * [batch, kv_heads, sink + window, head_dim]; positions: int64 [batch, sink + window]. */
+int sbfa_qcache_read(const struct sbfa_qcache* cache, void* k_out, void* v_out,
+                     int64_t* positions, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Attention of a batch to a prefix that all its sequences share (no upstream
@@ -380,16 +379,13 @@ int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const void* k_pr
  * sbfa_prefix_attend (n_q = 1, head_dim <= 128) with one rounding at the end and their
  * launches overlapped.  A sequence of length 0 sees the prefix alone.  ws:
  * sbfa_qcache_prefix_workspace_bytes() bytes. */
-int sbfa_qcache_prefix_attend(const void* q, const void* k_codes, const void* v_codes,
-                              const void* scales, const int64_t* lengths, const void* k_prefix,
-                              const void* v_prefix, void* o, float* lse, int64_t B, int64_t H,
-                              int64_t kv_heads, int64_t P, int64_t head_dim, int dtype, int fmt,
-                              double softmax_scale, int64_t sink, int64_t window, void* ws,
+int sbfa_qcache_prefix_attend(const struct sbfa_qcache* cache, const void* q,
+                              const void* k_prefix, const void* v_prefix, int64_t P, void* o,
+                              float* lse, int64_t H, double softmax_scale, void* ws,
                               int64_t ws_bytes, void* stream);
 
 /* Scratch bytes sbfa_qcache_prefix_attend needs on the current device, -1 for a bad shape. */
-int64_t sbfa_qcache_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t P,
-                                           int64_t head_dim, int64_t sink, int64_t window);
+int64_t sbfa_qcache_prefix_workspace_bytes(const struct sbfa_qcache* cache, int64_t H, int64_t P);
 
 /* The batch's own prompts behind the prefix, in one pass: query i of a sequence sees
  * the whole prefix and its sequence's tokens (i - window, i] of k, v (logical [B,

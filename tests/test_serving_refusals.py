@@ -14,11 +14,15 @@ INVALID, UNSUPPORTED = 1, 2
 P = 4096   # a non-null, 16-byte aligned address that is never read
 
 
-def append(L, B=1, H=1, D=64, dtype=native.BF16, fmt=0, sink=4, window=8, n=1, k=P, new=P,
-           strides=None, tickets=P):
+def cache(B=1, H=1, D=64, dtype=native.BF16, fmt=0, sink=4, window=8, k=P, tickets=P):
+    c = native.QCache(k, P, P, P, tickets, B, H, D, sink, window, dtype, fmt)
+    return c, ctypes.addressof(c)
+
+
+def append(L, n=1, new=P, strides=None, **kw):
     st = None if strides is None else (ctypes.c_int64 * 6)(*strides)
-    return L.sbfa_qcache_append(k, P, P, P, tickets, new, P, st, None, B, H, D, dtype, fmt, sink,
-                                window, n, None)
+    keep, at = cache(**kw)
+    return L.sbfa_qcache_append(at, new, P, st, None, n, None)
 
 
 @pytest.mark.parametrize("kw,rc,word", [
@@ -44,10 +48,19 @@ def test_append_of_nothing_launches_nothing():
     assert append(native.lib(), n=0, new=None) == 0 and native.launch_count() == before
 
 
-def attend(L, q=P, o=P, lse=P, B=1, H=4, hkv=2, D=64, scale=0.1, fmt=1, ws=P,
-           ws_bytes=1 << 40, window=8):
-    return L.sbfa_qcache_attend(q, P, P, P, P, o, lse, B, H, hkv, D, native.F16, fmt, scale, 4,
-                                window, ws, ws_bytes, None)
+def test_a_null_cache_is_refused():
+    L = native.lib()
+    assert L.sbfa_qcache_append(None, P, P, None, None, 1, None) == INVALID
+    assert L.sbfa_qcache_attend(None, P, P, None, 4, 0.1, None, 0, None) == INVALID
+    assert L.sbfa_qcache_read(None, P, P, P, None) == INVALID
+    assert L.sbfa_qcache_prefix_attend(None, P, P, P, 9, P, None, 4, 0.1, P, 99, None) == INVALID
+    assert L.sbfa_qcache_attend_workspace_bytes(None, 4) == -1
+    assert L.sbfa_qcache_prefix_workspace_bytes(None, 4, 9) == -1
+
+
+def attend(L, q=P, o=P, lse=P, B=1, H=4, hkv=2, scale=0.1, ws=P, ws_bytes=1 << 40, window=8):
+    keep, at = cache(B=B, H=hkv, window=window, dtype=native.F16, fmt=1)
+    return L.sbfa_qcache_attend(at, q, o, lse, H, scale, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("kw,word", [
@@ -94,9 +107,9 @@ def test_prefix_refuses(kw, rc, word):
 def test_decode_behind_a_prefix_refuses(kw, rc, word):
     a = dict(q=P, k=P, H=4, length=100, D=64, dtype=native.F16, fmt=0, scale=0.1, ws=P,
              ws_bytes=1 << 40) | kw
-    got = native.lib().sbfa_qcache_prefix_attend(
-        a["q"], P, P, P, P, a["k"], P, P, None, 2, a["H"], 2, a["length"], a["D"], a["dtype"],
-        a["fmt"], a["scale"], 4, 8, a["ws"], a["ws_bytes"], None)
+    keep, at = cache(B=2, H=2, D=a["D"], dtype=a["dtype"], fmt=a["fmt"])
+    got = native.lib().sbfa_qcache_prefix_attend(at, a["q"], a["k"], P, a["length"], P, None,
+                                                 a["H"], a["scale"], a["ws"], a["ws_bytes"], None)
     assert got == rc and word in native.last_error()
 
 
@@ -110,15 +123,20 @@ def test_sizes():
     for bad in ((0, 4, 2, 1, 100, 64, 0), (2, 4, 3, 1, 100, 64, 0), (2, 4, 2, 1, 0, 64, 0),
                 (2, 4, 2, 1, 100, 256, 0), (2, 4, 2, 1, 100, 64, -1)):
         assert L.sbfa_prefix_workspace_bytes(*bad) == -1
-    assert L.sbfa_qcache_prefix_workspace_bytes(2, 4, 2, 100, 64, 4, 8) >= 2 * 4 * 65 * 4
-    assert L.sbfa_qcache_prefix_workspace_bytes(2, 3, 2, 100, 64, 4, 8) == -1
+
+    def bytes_of(H=4, P=None, **kw):
+        keep, at = cache(**({"B": 2, "H": 2} | kw))
+        return (L.sbfa_qcache_attend_workspace_bytes(at, H) if P is None
+                else L.sbfa_qcache_prefix_workspace_bytes(at, H, P))
+
+    assert bytes_of(P=100) >= 2 * 4 * 65 * 4
+    assert bytes_of(H=3, P=100) == -1 and bytes_of(D=136, P=100) == -1
     # few units share clusters and need no scratch, many long ones are cut into equal runs
-    assert L.sbfa_qcache_attend_workspace_bytes(2, 4, 2, 64, 4, 8) == 0
-    assert L.sbfa_qcache_attend_workspace_bytes(300, 4, 2, 64, 4, 9999) > 0
-    for bad in ((2, 3, 2, 64, 4, 8), (2, 4, 2, 60, 4, 8), (0, 4, 2, 64, 4, 8),
-                (2, 4, 2, 64, 0, 0), (2, 1 << 60, 1 << 59, 64, 4, 8), (2, 4, 2, 64, 1 << 62, 8),
-                (1 << 40, 4, 2, 64, 4, 8)):
-        assert L.sbfa_qcache_attend_workspace_bytes(*bad) == -1
+    assert bytes_of() == 0 and bytes_of(B=300, window=9999) > 0
+    for bad in (dict(H=3), dict(D=60), dict(B=0), dict(sink=0, window=0), dict(sink=1 << 62),
+                dict(B=1 << 40)):
+        kw = {k: v for k, v in bad.items() if k != "H"}
+        assert bytes_of(H=bad.get("H", 4), **kw) == -1
 
 
 @pytest.mark.parametrize("kw,word", [
