@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
   volatile int* bad_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 8);
 
+  griddep_launch();   // the cache's kernel or the merge may take what SMs are left
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bid = (int)blockIdx.x;
   const bool sliced = bid >= geo.n_full;
@@ -543,7 +544,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(bar(L::kPFull + 2 * x + h));
       }
       if (ok) ok = wait_bar_w(bar(L::kOFull + x), 0, abort_flag, status);
-      griddep_wait();   // the cache's kernel before this one, if any
       if (ok) {
         tc_fence_after();
         // A row's 2 D bytes pass through this warp's part of the Q tile, which is no
@@ -625,9 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (32 * c + i < geo.d)
-                  f[i] += w_own * (out.own_kind == kOwn32
-                                       ? ((const float*)out.own_o)[at * geo.d + 32 * c + i]
-                                       : Elem<T>::to(((const T*)out.own_o)[at * geo.d + 32 * c + i]));
+                  f[i] += w_own * Elem<T>::to(((const T*)out.own_o)[at * geo.d + 32 * c + i]);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -641,10 +639,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
-  // complete only after the kernel before this one, so that the merge, which waits for this
-  // one, sees both
-  griddep_wait();
-  griddep_launch();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -749,17 +743,21 @@ int tile_dim(int64_t d) {
   return d <= 64 ? 64 : 128;
 }
 
-// Slices of the tail units: whole waves of one CTA per SM, each as long as its tiles plus
-// a set-up worth about three (Q gather, pipeline fill, epilogue), against the partial
-// rows that every slice writes and the merge reads (a tile's time moves about 6 MB).
-int prefix_splits(int64_t units, int n_tiles, int64_t part_bytes) {
+// Slices of the tail units, by the time that they take in us: whole waves of one CTA per SM, each
+// as long as its tiles (2.15 us for two query tiles, 1.5 for one) plus 6 us (Q gather, pipeline
+// fill, epilogue), and the partial rows that every slice writes and the merge reads back (3 MB
+// a us; half as dear with the waves of fewer, longer slices beside another kernel).
+// beside: SM time that a kernel running beside this one needs; it fills what SMs this one leaves.
+int prefix_splits(int64_t units, int n_tiles, bool two, int64_t part_bytes, double beside) {
   const int64_t sms = device_sm_count();
+  const double tile = two ? 2.15 : 1.5, per_us = beside > 0 ? 6e6 : 3e6;
   int best = 1;
   double best_cost = 1e300;
   for (int ns = 1; ns <= std::min(n_tiles, 64); ++ns) {
     const int64_t waves = (units * ns + sms - 1) / sms;
-    const double cost =
-        (double)waves * ((n_tiles + ns - 1) / ns + 3) + (ns > 1 ? ns * part_bytes / 3e6 + 2 : 0);
+    const double cta = (n_tiles + ns - 1) / ns * tile + 6;
+    const double busy = (beside + units * ns * cta) / sms;
+    const double cost = std::max(waves * cta, busy) + (ns > 1 ? ns * part_bytes / per_us + 4 : 0);
     if (cost < best_cost) {
       best_cost = cost;
       best = ns;
@@ -769,7 +767,8 @@ int prefix_splits(int64_t units, int n_tiles, int64_t part_bytes) {
 }
 
 bool prefix_geometry(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P,
-                     int64_t head_dim, int64_t window, PrefixGeom* geo) {
+                     int64_t head_dim, int64_t window, PrefixGeom* geo,
+                     const sbfa_qcache* cache = nullptr) {
   if (B <= 0 || H <= 0 || n_q <= 0 || P <= 0 || P >= (1ll << 31) - kTN || window < 0 ||
       tile_dim(head_dim) == 0)
     return false;
@@ -799,13 +798,24 @@ bool prefix_geometry(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_
   int box = 8;
   while (box < n_q && box < kTN) box *= 2;
   geo->box = box;
+  const int64_t unit_bytes = (int64_t)kPair * kTM * tile_dim(head_dim) * 4;
+  const bool two = geo->rows > kTM;
+  if (cache != nullptr) {
+    // beside the cache's kernel, which reads a full cache at about 30 GB/s per SM, its ramps and
+    // last wave counted; its result is joined by the merge, so every unit leaves partial rows
+    const double beside = 2.0 * B * kv_heads * (double)(cache->sink + cache->window) *
+                          (double)(head_dim + 1) / 30e3;
+    geo->n_full = 0;
+    geo->n_tail = (int)units;
+    geo->splits = prefix_splits(units, geo->n_tiles, two, units * unit_bytes, beside);
+    return true;
+  }
   const int sms = device_sm_count();
   geo->n_full = (int)(units / sms * sms);
   geo->n_tail = (int)(units - geo->n_full);
   geo->splits = 1;
   if (geo->n_tail > 0)
-    geo->splits = prefix_splits(geo->n_tail, geo->n_tiles,
-                                (int64_t)geo->n_tail * kPair * kTM * tile_dim(head_dim) * 4);
+    geo->splits = prefix_splits(geo->n_tail, geo->n_tiles, two, geo->n_tail * unit_bytes, 0);
   if (geo->splits == 1) {  // nothing to cut
     geo->n_full += geo->n_tail;
     geo->n_tail = 0;
@@ -828,7 +838,7 @@ struct PrefixCall {
   PrefixOut out;
   float scale;
   void* ws;
-  bool chained;                 // the kernel before this one is the cache's attend kernel
+  const QAttend* beside;        // a cache's attend call that runs beside the prefix, or NULL
   cudaStream_t stream;
 };
 
@@ -862,13 +872,12 @@ int launch_prefix(const PrefixCall& c, const PrefixGeom& geo) {
     return rc;
   {
     LaunchScope ls("prefix_tc_kernel", c.stream);
-    if (int rc = check_cuda(
-            launch_early(kern, (unsigned)(geo.n_full + geo.n_tail * geo.splits), kThreads,
-                         L::kAlloc, c.stream, c.chained, (const T*)c.q, mk, mv, mok, mov, out,
-                         c.scale * kLog2e, geo, device_status_ptr()),
-            "prefix_tc_kernel"))
-      return rc;
+    kern<<<(unsigned)(geo.n_full + geo.n_tail * geo.splits), kThreads, L::kAlloc, c.stream>>>(
+        (const T*)c.q, mk, mv, mok, mov, out, c.scale * kLog2e, geo, device_status_ptr());
   }
+  if (int rc = check_launch("prefix_tc_kernel")) return rc;
+  if (c.beside != nullptr)
+    if (int rc = qcache_attend_launch(*c.beside)) return rc;
   if (geo.n_tail == 0) return SBFA_OK;
   const int64_t rows_per = kMergeThreads / (D / 4);
   const int64_t blocks = ((int64_t)geo.n_tail * kPair * kTM + rows_per - 1) / rows_per;
@@ -911,16 +920,23 @@ int launch_call(const PrefixCall& c, const PrefixGeom& geo, int dtype) {
 }
 
 int check_prefix(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim,
-                 int dtype, int64_t window, PrefixGeom* geo) {
+                 int dtype, int64_t window, PrefixGeom* geo, const sbfa_qcache* cache = nullptr) {
   if (dtype != SBFA_F16 && dtype != SBFA_BF16)
     return fail(SBFA_ERR_UNSUPPORTED, "prefix attention: dtype must be float16 or bfloat16");
   if (tile_dim(head_dim) == 0)
     return fail(SBFA_ERR_UNSUPPORTED,
                 "prefix attention: head_dim must be a multiple of 8 and at most 128");
-  if (!prefix_geometry(B, H, kv_heads, n_q, P, head_dim, window, geo))
+  if (!prefix_geometry(B, H, kv_heads, n_q, P, head_dim, window, geo, cache))
     return fail(SBFA_ERR_INVALID, "prefix attention: sizes must be positive, H a multiple of "
                                   "kv_heads, P and B * H / kv_heads * n_q below 2^31");
   return SBFA_OK;
+}
+
+// SMs that the prefix's kernel holds for most of its time: none when it comes in several waves,
+// behind whose last the cache's kernel starts.
+int busy_sms(const PrefixGeom& g) {
+  const int64_t ctas = (int64_t)g.n_tail * g.splits;
+  return ctas < device_sm_count() ? (int)ctas : 0;
 }
 
 int64_t own_bytes(int64_t B, int64_t H, int64_t d) {
@@ -967,10 +983,11 @@ extern "C" int sbfa_prefix_attend(const void* q, const int64_t* q_strides, const
 
 extern "C" int64_t sbfa_qcache_prefix_workspace_bytes(const sbfa_qcache* cache, int64_t H,
                                                       int64_t P) {
-  const int64_t bytes = qcache_attend_ws_bytes(cache, H);
   PrefixGeom geo;
-  if (bytes < 0 || !prefix_geometry(cache->batch, H, cache->kv_heads, 1, P, cache->head_dim, 0, &geo))
+  if (qcache_attend_ws_bytes(cache, H, 0) < 0 ||   // refuses what is no cache
+      !prefix_geometry(cache->batch, H, cache->kv_heads, 1, P, cache->head_dim, 0, &geo, cache))
     return -1;
+  const int64_t bytes = qcache_attend_ws_bytes(cache, H, busy_sms(geo));
   return own_bytes(cache->batch, H, cache->head_dim) + ws_bytes_of(geo) + bytes;
 }
 
@@ -981,7 +998,8 @@ extern "C" int sbfa_qcache_prefix_attend(const sbfa_qcache* cache, const void* q
   if (cache == nullptr) return fail(SBFA_ERR_INVALID, "8-bit cache: NULL cache");
   const int64_t B = cache->batch, head_dim = cache->head_dim;
   PrefixGeom geo;
-  if (int rc = check_prefix(B, H, cache->kv_heads, 1, P, head_dim, cache->dtype, 0, &geo)) return rc;
+  if (int rc = check_prefix(B, H, cache->kv_heads, 1, P, head_dim, cache->dtype, 0, &geo, cache))
+    return rc;
   // the cache's own result in fp32 [B, H, d] and its LSE [B, H], the prefix's scratch, the cache's
   const int64_t own = own_bytes(B, H, head_dim), pre = ws_bytes_of(geo);
   if (ws == nullptr || ws_bytes < own + pre)
@@ -989,7 +1007,7 @@ extern "C" int sbfa_qcache_prefix_attend(const sbfa_qcache* cache, const void* q
   float* own_o = (float*)ws;
   float* own_lse = own_o + B * H * head_dim;
   const QAttend a{cache, q, nullptr, own_o, own_lse, H, softmax_scale, (char*)ws + own + pre,
-                  ws_bytes - own - pre, (cudaStream_t)stream};
+                  ws_bytes - own - pre, true, busy_sms(geo), (cudaStream_t)stream};
   PrefixCall c = {};
   c.q = q;
   c.k = k_prefix;
@@ -1000,12 +1018,11 @@ extern "C" int sbfa_qcache_prefix_attend(const sbfa_qcache* cache, const void* q
   c.out.own_lse = own_lse;
   c.out.own_kind = kOwn32;
   c.ws = (char*)ws + own;
-  c.chained = true;
+  c.beside = &a;
   c.stream = (cudaStream_t)stream;
   // all checks before the first launch
   if (int rc = qcache_attend_check(a)) return rc;
   if (int rc = check_call(c, nullptr, geo, H, softmax_scale, pre)) return rc;
-  if (int rc = qcache_attend_launch(a)) return rc;
   return launch_call(c, geo, cache->dtype);
 }
 

@@ -477,13 +477,19 @@ template <typename T, int FMT, int DP, int NQ, bool FLAT>
 __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     qcache_attend_kernel(const T* __restrict__ q, QCache c, const int64_t* __restrict__ lengths,
                          T* __restrict__ o, float* __restrict__ o32, float* __restrict__ lse,
-                         float scale_log2, int group, int chunks, int ns, int batch, FlatWs ws) {
+                         float scale_log2, int group, int chunks, int ns, int batch, bool beside,
+                         FlatWs ws) {
   using C = AttCfg<DP, NQ>;
   constexpr int KT = C::kTiles, KS = 16 * KT;
   constexpr int NCH = DP / 64;      // 16-byte pieces of a K row per lane
   constexpr int VW = DP / 32;       // words of a V row per lane
   extern __shared__ __align__(16) float att_smem[];
-  tc::griddep_launch();   // a shared prefix's kernel reads nothing of ours before its own wait
+  tc::griddep_launch();   // what follows (a merge) waits for this kernel's results itself
+  // Beside a shared prefix's kernel the last CTA completes after it, and with it this kernel, so that
+  // whoever waits for this one has both.  (All CTAs waiting would keep others from starting.)
+  auto leave = [&] {
+    if (beside && blockIdx.x == gridDim.x - 1) tc::griddep_wait();
+  };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, cc = lane & 3;
   const int hcs = (int)c.heads * chunks;
@@ -531,7 +537,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
       inside = rem;
     }
     if (threadIdx.x == 0) ws.rec[blockIdx.x].unit_start = -1;
-    if (begin == end) return;                      // a few short units, more CTAs
+    if (begin == end) {                            // a few short units, more CTAs
+      leave();
+      return;
+    }
     __syncthreads();
     cur.b = first[0];
     cur.n = first[1];
@@ -544,7 +553,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     left = max((int64_t)0, end - begin - (cost - at));
     const int64_t unit_start = begin - at;
     if (cur.s0 >= cur.s1) {                        // nothing of that unit: begin with the next
-      if (left == 0) return;
+      if (left == 0) {
+        leave();
+        return;
+      }
       if (++cur.hc == hcs) {
         cur.hc = 0;
         cur.n = visible(++cur.b);
@@ -949,7 +961,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     }
   }
   if constexpr (!FLAT) {
-    if (ns == 1) return;
+    if (ns == 1) {
+      leave();
+      return;
+    }
     // the CTAs of the cluster: each takes its share of the rows' columns from all of them
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
@@ -968,9 +983,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
       write(row, col, Mx, mx, L, a);
     }
     cluster.sync();   // peers may still read this CTA's memory
+    leave();
     return;
   }
-  if (!has_next) return;
+  if (!has_next) {
+    leave();
+    return;
+  }
   __syncthreads();    // the merge has read what the next run's will overwrite
   cur = nxt;
   s = warp;
@@ -1156,7 +1175,8 @@ struct AttPlan {
   int grid, ns;         // CTAs; CTAs of a cluster
   int64_t ws_bytes;
 };
-int attend_plan(int64_t B, int64_t kv_heads, int64_t group, int64_t d, int64_t rows, AttPlan* p) {
+int attend_plan(int64_t B, int64_t kv_heads, int64_t group, int64_t d, int64_t rows, int busy_sms,
+                AttPlan* p) {
   const int dp = padded_dim(d);
   // 16 query columns halve the passes over a group of more than 8; at 256 columns per row
   // the second set of accumulators would not fit the registers
@@ -1166,7 +1186,7 @@ int attend_plan(int64_t B, int64_t kv_heads, int64_t group, int64_t d, int64_t r
   const int64_t units = B * kv_heads * p->chunks;
   if (units >= (1ll << 27) || kv_heads * p->chunks >= (1ll << 27))
     return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many (sequence, head) units");
-  const int64_t slots = (int64_t)device_sm_count() * att_ctas(dp, p->nq);
+  const int64_t slots = (int64_t)(device_sm_count() - busy_sms) * att_ctas(dp, p->nq);
   // A cluster shortens a unit while there are SMs to fill.
   p->ns = 1;
   while (p->ns < 8 && units * p->ns * 2 <= slots && rows > (int64_t)p->ns * 128) p->ns *= 2;
@@ -1176,7 +1196,8 @@ int attend_plan(int64_t B, int64_t kv_heads, int64_t group, int64_t d, int64_t r
   // 16 x 8 x 2048 from 19 to 22.
   const int64_t waves = (units * p->ns + slots - 1) / slots;
   const int64_t lost = waves * rows / p->ns - units * rows / slots;
-  p->flat = lost * dp > 960 * 128;
+  // Beside a prefix's kernel SMs come free meanwhile, so a last wave costs about half of that.
+  p->flat = lost * dp > 960 * 128 * (busy_sms > 0 ? 2 : 1);
   p->grid = p->flat ? (int)slots : (int)(units * p->ns);
   if (p->flat) p->ns = 1;
   p->ws_bytes = p->flat ? slots * ((int64_t)sizeof(FlatRecord) +
@@ -1208,18 +1229,25 @@ int launch_attend(const QAttend& a, const QCache& c, const AttPlan& p) {
   cfg.blockDim = dim3(kAttWarps * 32);
   cfg.dynamicSmemBytes = C::kBytes;
   cfg.stream = a.stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)p.ns;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
   cfg.attrs = at;
-  cfg.numAttrs = p.ns > 1 ? 1 : 0;
+  if (p.ns > 1) {
+    cudaLaunchAttribute& x = at[cfg.numAttrs++];
+    x.id = cudaLaunchAttributeClusterDimension;
+    x.val.clusterDim.x = (unsigned)p.ns;
+    x.val.clusterDim.y = x.val.clusterDim.z = 1;
+  }
+  if (a.beside) {
+    cudaLaunchAttribute& x = at[cfg.numAttrs++];
+    x.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    x.val.programmaticStreamSerializationAllowed = 1;
+  }
   {
     LaunchScope ls("qcache_attend_kernel", a.stream);
     if (int rc = check_cuda(
             cudaLaunchKernelEx(&cfg, kern, (const T*)a.q, c, (const int64_t*)a.cache->lengths, (T*)a.o,
                                a.o32, a.lse, (float)a.scale * kLog2e, group, p.chunks, p.ns,
-                               (int)a.cache->batch, ws),
+                               (int)a.cache->batch, a.beside, ws),
             "qcache_attend_kernel"))
       return rc;
   }
@@ -1300,16 +1328,17 @@ extern "C" int sbfa_qcache_read(const sbfa_qcache* cache, void* k_out, void* v_o
 
 namespace sbfa {
 // The plan of a call over H query heads.
-static int plan_for(const sbfa_qcache* c, int64_t H, AttPlan* p) {
+static int plan_for(const sbfa_qcache* c, int64_t H, int busy_sms, AttPlan* p) {
   if (H <= 0 || H % c->kv_heads != 0)
     return fail(SBFA_ERR_INVALID, "the query head count must be a multiple of kv_heads");
   if (H / c->kv_heads >= (1 << 20)) return fail(SBFA_ERR_UNSUPPORTED, "too many query heads");
-  return attend_plan(c->batch, c->kv_heads, H / c->kv_heads, c->head_dim, c->sink + c->window, p);
+  return attend_plan(c->batch, c->kv_heads, H / c->kv_heads, c->head_dim, c->sink + c->window,
+                     busy_sms, p);
 }
 
-int64_t qcache_attend_ws_bytes(const sbfa_qcache* cache, int64_t H) {
+int64_t qcache_attend_ws_bytes(const sbfa_qcache* cache, int64_t H, int busy_sms) {
   AttPlan p;
-  if (check_geometry(cache) != SBFA_OK || plan_for(cache, H, &p) != SBFA_OK) return -1;
+  if (check_geometry(cache) != SBFA_OK || plan_for(cache, H, busy_sms, &p) != SBFA_OK) return -1;
   return p.ws_bytes;
 }
 
@@ -1322,7 +1351,7 @@ int qcache_attend_check(const QAttend& a) {
   if (((uintptr_t)a.q | (uintptr_t)a.o | (uintptr_t)a.o32 | (uintptr_t)a.ws) & 15u)
     return fail(SBFA_ERR_INVALID, "8-bit cache: tensors must be 16-byte aligned");
   AttPlan p;
-  if (int rc = plan_for(a.cache, a.H, &p)) return rc;
+  if (int rc = plan_for(a.cache, a.H, a.busy_sms, &p)) return rc;
   if (p.ws_bytes > 0 && (a.ws == nullptr || a.ws_bytes < p.ws_bytes))
     return fail(SBFA_ERR_INVALID, "8-bit cache: workspace too small (need " +
                                       std::to_string(p.ws_bytes) + " bytes)");
@@ -1332,7 +1361,7 @@ int qcache_attend_check(const QAttend& a) {
 int qcache_attend_launch(const QAttend& a) {
   const QCache c = device_view(a.cache);
   AttPlan p;
-  if (int rc = plan_for(a.cache, a.H, &p)) return rc;
+  if (int rc = plan_for(a.cache, a.H, a.busy_sms, &p)) return rc;
   return by_format(a.cache->dtype, a.cache->fmt, a.cache->head_dim, [&](auto t, auto m, auto dp) {
     using T = decltype(t);
     constexpr int DP = dp.value;
@@ -1348,13 +1377,14 @@ int qcache_attend_launch(const QAttend& a) {
 }  // namespace sbfa
 
 extern "C" int64_t sbfa_qcache_attend_workspace_bytes(const sbfa_qcache* cache, int64_t H) {
-  return qcache_attend_ws_bytes(cache, H);
+  return qcache_attend_ws_bytes(cache, H, 0);
 }
 
 extern "C" int sbfa_qcache_attend(const sbfa_qcache* cache, const void* q, void* o, float* lse,
                                   int64_t H, double softmax_scale, void* ws, int64_t ws_bytes,
                                   void* stream) {
-  const QAttend a{cache, q, o, nullptr, lse, H, softmax_scale, ws, ws_bytes, (cudaStream_t)stream};
+  const QAttend a{cache, q, o, nullptr, lse, H, softmax_scale, ws, ws_bytes,
+                  false, 0, (cudaStream_t)stream};
   if (int rc = qcache_attend_check(a)) return rc;
   return qcache_attend_launch(a);
 }

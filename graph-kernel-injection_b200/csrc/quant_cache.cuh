@@ -29,10 +29,14 @@ struct QAttend {
   double scale;
   void* ws;
   int64_t ws_bytes;
+  // Whether the kernel ahead in the stream is a shared prefix's, beside which this call may run: it
+  // starts early, and does not complete before that one has.
+  bool beside;
+  int busy_sms;   // that the prefix's kernel takes meanwhile
   cudaStream_t stream;
 };
 // Scratch of a call, -1 for a bad shape.
-int64_t qcache_attend_ws_bytes(const sbfa_qcache* cache, int64_t H);
+int64_t qcache_attend_ws_bytes(const sbfa_qcache* cache, int64_t H, int busy_sms);
 int qcache_attend_check(const QAttend& a);   // an SBFA_ERR_* code; launches nothing
 int qcache_attend_launch(const QAttend& a);  // after the check
 
