@@ -112,6 +112,19 @@ __device__ __forceinline__ float saturated(float x) {
   return fabsf(x) > top ? copysignf(top, x) : x;
 }
 
+// two values rounded to T within its finite range (NaN stays)
+template <typename T> __device__ __forceinline__ uint32_t pack2_sat(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2_sat<__half>(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2_sat<__nv_bfloat16>(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
@@ -254,8 +267,9 @@ __device__ __forceinline__ uint4 values8(uint2 codes, float scale) {
   uint32_t r[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[j]));
-    r[j] = tc::pack2<T>(saturated<T>(f.x * scale), saturated<T>(f.y * scale));
+    const float2 f = __fmul2_rn(__half22float2(*reinterpret_cast<__half2*>(&h[j])),
+                                make_float2(scale, scale));
+    r[j] = pack2_sat<T>(f.x, f.y);
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
@@ -427,16 +441,17 @@ __device__ __forceinline__ void att_write(T* o, float* o32, float* lse, int64_t 
   const bool some = !(L == 0.f);
   const float f = some ? 1.f / L : 0.f;
   const float back = ex2((Mx == -INFINITY ? 0.f : Mx) - (mx == -INFINITY ? 0.f : mx));
-  a.x = some ? saturated<T>(a.x * f * back) : 0.f;
-  a.y = some ? saturated<T>(a.y * f * back) : 0.f;
-  a.z = some ? saturated<T>(a.z * f * back) : 0.f;
-  a.w = some ? saturated<T>(a.w * f * back) : 0.f;
+  a.x = some ? a.x * f * back : 0.f;
+  a.y = some ? a.y * f * back : 0.f;
+  a.z = some ? a.z * f * back : 0.f;
+  a.w = some ? a.w * f * back : 0.f;
   if (col < d) {
     if (o32)
-      *reinterpret_cast<float4*>(o32 + out * d + col) = a;
+      *reinterpret_cast<float4*>(o32 + out * d + col) =
+          make_float4(saturated<T>(a.x), saturated<T>(a.y), saturated<T>(a.z), saturated<T>(a.w));
     else
       *reinterpret_cast<uint2*>(o + out * d + col) =
-          make_uint2(tc::pack2<T>(a.x, a.y), tc::pack2<T>(a.z, a.w));
+          make_uint2(pack2_sat<T>(a.x, a.y), pack2_sat<T>(a.z, a.w));
   }
   // a partial result marks an empty row by -inf, the public one by 0
   if (col == 0 && lse) lse[out] = some ? (mx + log2f(L)) * kLn2 : (o32 ? -INFINITY : 0.f);
