@@ -132,14 +132,15 @@ template <> __device__ __forceinline__ uint32_t pack2_sat<__nv_bfloat16>(float a
 // and of V, the row maxima in packed 16-bit integers (the magnitudes of both 16-bit types are
 // ordered like their bits) with one shuffle chain for both, 8 code bytes back per piece.
 // Bound by HBM (4 D bytes in, 2 D + 2 out per head and token) and nearly by instruction issue:
-// 16 x 8 x 2048 rows of 128 take 45 us with 16 lanes a row and fp32 maxima, 40 us so.  A CTA covers 2^hs heads x
+// 16 x 8 x 2048 rows of 128 take 45 us with 16 lanes a row and fp32 maxima, 38 us so.  A CTA covers 2^hs heads x
 // kRows / 2^hs tokens at a time (tokens adjacent, so that their scale pairs share sectors;
 // several heads only where a call has few tokens) and walks the tokens that survive the
 // call: positions that a later token of it overwrites are never visited.  The last CTA of a
 // sequence moves its length on (a ticket per sequence, left at zero), which saves a second launch
 // in every decode step.
 constexpr int kAppThreads = 256;
-constexpr int kAppRounds = 2;   // of resident CTAs, with at least two passes each
+constexpr int kAppCtas = 6;     // resident per SM
+constexpr int kAppRounds = 2;   // of them, with at least two passes each
 constexpr int app_lanes(int dp) { return dp == 256 ? 16 : 8; }
 
 // fp32 bits of the magnitude whose 16 bits are `h`
@@ -152,7 +153,7 @@ template <> __device__ __forceinline__ uint32_t magnitude_bits<__half>(uint32_t 
 }
 
 template <typename T, int FMT, int DP>
-__global__ void __launch_bounds__(kAppThreads)
+__global__ void __launch_bounds__(kAppThreads, kAppCtas)
     qcache_append_kernel(QCache c, int64_t* __restrict__ lengths, int32_t* __restrict__ tickets,
                          const T* __restrict__ kn, const T* __restrict__ vn, Strides3 sk,
                          Strides3 sv, const int64_t* __restrict__ counts, int n_new,
@@ -253,8 +254,9 @@ __global__ void __launch_bounds__(kAppThreads)
 // Out row i of a sequence is its i-th kept position in order (sinks, then the
 // window from its oldest), rows behind the last one are zero with position -1.
 // A group of DP / 8 lanes per row, CTAs walk the rows of one head; bound by HBM (2 D + 2
-// bytes in, 4 D out per kept row and head).  64 x 8 x 2052 rows of 128 take 175, 144, 138, 131 us with
-// 1, 2, 4, 8 rounds of resident CTAs: many short CTAs keep loads and stores of different ones apart.
+// bytes in, 4 D out per kept row and head).  64 x 8 x 2052 rows of 128 took 175, 144, 138, 131 us with
+// 1, 2, 4, 8 rounds of resident CTAs (many short ones keep loads and stores of different CTAs
+// apart), and take 128.5 us since the conversion saturates by itself.
 constexpr int kReadThreads = 256;
 constexpr int kReadUnroll = 4;
 constexpr int kReadRounds = 8;   // of resident CTAs
@@ -1308,7 +1310,7 @@ extern "C" int sbfa_qcache_append(const sbfa_qcache* cache, const void* k_new, c
     using T = decltype(t);
     RowGrid g;
     if (int rc = row_grid(cache->batch, H, std::min(n_new, c.rows),
-                          kAppThreads / app_lanes(dp.value), 1, 2, 5 * kAppRounds, &g))
+                          kAppThreads / app_lanes(dp.value), 1, 2, kAppCtas * kAppRounds, &g))
       return rc;
     LaunchScope ls("qcache_append_kernel", s);
     qcache_append_kernel<T, m.value, dp.value><<<g.grid, kAppThreads, 0, s>>>(
