@@ -128,16 +128,16 @@ template <> __device__ __forceinline__ uint32_t pack2_sat<__nv_bfloat16>(float a
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
-// A group of 8 lanes (16 at 256 columns) takes one (head, token): pieces of 16 bytes of K
-// and of V, the row maxima in packed 16-bit integers (the magnitudes of both 16-bit types are
-// ordered like their bits) with one shuffle chain for both, 8 code bytes back per piece.
-// Bound by HBM (4 D bytes in, 2 D + 2 out per head and token) and nearly by instruction issue:
-// 16 x 8 x 2048 rows of 128 take 45 us with 16 lanes a row and fp32 maxima, 38 us so.  A CTA covers 2^hs heads x
-// kRows / 2^hs tokens at a time (tokens adjacent, so that their scale pairs share sectors;
-// several heads only where a call has few tokens) and walks the tokens that survive the
-// call: positions that a later token of it overwrites are never visited.  The last CTA of a
-// sequence moves its length on (a ticket per sequence, left at zero), which saves a second launch
-// in every decode step.
+// A group of 8 lanes (16 at 256 columns) takes one (head, token): pieces of 16 bytes of K and
+// of V, the row maxima in packed 16-bit integers (the magnitudes of both 16-bit types are
+// ordered like their bits) with one shuffle chain for both, 8 code bytes back per piece. Bound
+// by HBM (4 D bytes in, 2 D + 2 out per head and token) and nearly by instruction issue: 16 x 8
+// x 2048 rows of 128 take 45 us with 16 lanes a row and fp32 maxima, 38 us so.  A CTA covers
+// 2^hs heads x kRows / 2^hs tokens at a time (tokens adjacent, so that their scale pairs share
+// sectors; several heads only where a call has few tokens) and walks the tokens that survive
+// the call: positions that a later token of it overwrites are never visited.  The last CTA of a
+// sequence moves its length on (a ticket per sequence, left at zero), which saves a second
+// launch in every decode step.
 constexpr int kAppThreads = 256;
 constexpr int kAppCtas = 6;     // resident per SM
 constexpr int kAppRounds = 2;   // of them, with at least two passes each
@@ -251,12 +251,12 @@ __global__ void __launch_bounds__(kAppThreads, kAppCtas)
 // ---------------------------------------------------------------------------
 // read back
 // ---------------------------------------------------------------------------
-// Out row i of a sequence is its i-th kept position in order (sinks, then the
-// window from its oldest), rows behind the last one are zero with position -1.
-// A group of DP / 8 lanes per row, CTAs walk the rows of one head; bound by HBM (2 D + 2
-// bytes in, 4 D out per kept row and head).  64 x 8 x 2052 rows of 128 took 175, 144, 138, 131 us with
-// 1, 2, 4, 8 rounds of resident CTAs (many short ones keep loads and stores of different CTAs
-// apart), and take 128.5 us since the conversion saturates by itself.
+// Out row i of a sequence is its i-th kept position in order (sinks, then the window from its
+// oldest), rows behind the last one are zero with position -1. A group of DP / 8 lanes per row,
+// CTAs walk the rows of one head; bound by HBM (2 D + 2 bytes in, 4 D out per kept row and
+// head).  64 x 8 x 2052 rows of 128 took 175, 144, 138, 131 us with 1, 2, 4, 8 rounds of
+// resident CTAs (many short ones keep loads and stores of different CTAs apart), and take 128.5
+// us since the conversion saturates by itself.
 constexpr int kReadThreads = 256;
 constexpr int kReadUnroll = 4;
 constexpr int kReadRounds = 8;   // of resident CTAs
@@ -323,7 +323,8 @@ __global__ void __launch_bounds__(kReadThreads)
           const int64_t dst = (row0 + i) * c.d + lane * 8;
           __stcs(reinterpret_cast<uint4*>(ko + dst),
                  values8<T, FMT>(xk[u], scale_value(sc[u] & 255u)));
-          __stcs(reinterpret_cast<uint4*>(vo + dst), values8<T, FMT>(xv[u], scale_value(sc[u] >> 8)));
+          __stcs(reinterpret_cast<uint4*>(vo + dst),
+                 values8<T, FMT>(xv[u], scale_value(sc[u] >> 8)));
         }
       }
     }
@@ -367,8 +368,9 @@ __global__ void __launch_bounds__(kReadThreads)
 constexpr int kAttWarps = 4;
 constexpr float kSlack = 4.f;
 
-// Resident CTAs per SM that the registers are limited for.  At two sets of query columns steps of 32 rows
-// on two CTAs beat steps of 16 on three (64 x 8 heads of 12 queries x 2052 rows: 72 against 84 us).
+// Resident CTAs per SM that the registers are limited for.  At two sets of query columns steps
+// of 32 rows on two CTAs beat steps of 16 on three (64 x 8 heads of 12 queries x 2052 rows: 72
+// against 84 us).
 constexpr int att_ctas(int dp, int nq) { return dp == 256 || nq == 2 ? 2 : 3; }
 
 template <int DP, int NQ>
@@ -477,9 +479,10 @@ __device__ __forceinline__ int64_t flat_start(int64_t total, int i, int n) {
   return (int64_t)((uint64_t)total * (uint32_t)i / (uint32_t)n);
 }
 
-// A unit costs its steps and about kRunSteps more (its queries, merge and output, and latency that
-// one warp step cannot hide): with 2, 4, 8 a ragged batch of 64 x 8 heads of 12 queries takes 106, 90, 66 us.
-// Runs are equal in this cost; one that begins in the surplus begins with the next unit.
+// A unit costs its steps and about kRunSteps more (its queries, merge and output, and latency
+// that one warp step cannot hide): with 2, 4, 8 a ragged batch of 64 x 8 heads of 12 queries
+// takes 106, 90, 66 us. Runs are equal in this cost; one that begins in the surplus begins with
+// the next unit.
 constexpr int kRunSteps = 8;
 
 // A run of steps [s0, s1) of one unit.
@@ -502,8 +505,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
   constexpr int VW = DP / 32;       // words of a V row per lane
   extern __shared__ __align__(16) float att_smem[];
   tc::griddep_launch();   // what follows (a merge) waits for this kernel's results itself
-  // Beside a shared prefix's kernel the last CTA completes after it, and with it this kernel, so that
-  // whoever waits for this one has both.  (All CTAs waiting would keep others from starting.)
+  // Beside a shared prefix's kernel the last CTA completes after it, and with it this kernel,
+  // so that whoever waits for this one has both.  (All CTAs waiting would keep others from
+  // starting.)
   auto leave = [&] {
     if (beside && blockIdx.x == gridDim.x - 1) tc::griddep_wait();
   };
@@ -684,332 +688,336 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     load_v(cur, s);
   }
   for (;;) {
-  // the run behind this one, which starts its unit
-  AttRun nxt = cur;
-  const bool has_next = FLAT && left > 0;
-  if (has_next) {
-    nxt.hc = cur.hc + 1;
-    if (nxt.hc == hcs) {
-      nxt.hc = 0;
-      nxt.b = cur.b + 1;
-      nxt.n = visible(nxt.b);
-      nxt.steps = steps_of(nxt.n);
+    // the run behind this one, which starts its unit
+    AttRun nxt = cur;
+    const bool has_next = FLAT && left > 0;
+    if (has_next) {
+      nxt.hc = cur.hc + 1;
+      if (nxt.hc == hcs) {
+        nxt.hc = 0;
+        nxt.b = cur.b + 1;
+        nxt.n = visible(nxt.b);
+        nxt.steps = steps_of(nxt.n);
+      }
+      nxt.row0 = first_row(nxt);
+      nxt.s0 = 0;
+      nxt.s1 = (int)min((int64_t)nxt.steps, left);
+      left = max((int64_t)0, left - cost_of(nxt.n));
     }
-    nxt.row0 = first_row(nxt);
-    nxt.s0 = 0;
-    nxt.s1 = (int)min((int64_t)nxt.steps, left);
-    left = max((int64_t)0, left - cost_of(nxt.n));
-  }
-  const int h0 = cur.hc % chunks * C::kRowsQ;             // first head of the group
-  const int nq = min(C::kRowsQ, group - h0);
-  const int64_t qrow0 = ((int64_t)cur.b * c.heads + cur.hc / chunks) * group + h0;
-  const int n = cur.n;
+    const int h0 = cur.hc % chunks * C::kRowsQ;             // first head of the group
+    const int nq = min(C::kRowsQ, group - h0);
+    const int64_t qrow0 = ((int64_t)cur.b * c.heads + cur.hc / chunks) * group + h0;
+    const int n = cur.n;
 
-  // Q fragments, column g of each n-tile, scaled into fp16's range
-  uint32_t qf[NQ][DP / 16][2];
-  float qs[NQ][2];   // softmax scale (base 2) over the two query columns of this lane
+    // Q fragments, column g of each n-tile, scaled into fp16's range
+    uint32_t qf[NQ][DP / 16][2];
+    float qs[NQ][2];   // softmax scale (base 2) over the two query columns of this lane
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    const int r = t * 8 + g;
-    uint32_t raw[NCH][8];
-    uint32_t m = 0;
+    for (int t = 0; t < NQ; ++t) {
+      const int r = t * 8 + g;
+      uint32_t raw[NCH][8];
+      uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
+      for (int j = 0; j < NCH; ++j)
 #pragma unroll
-      for (int hlf = 0; hlf < 2; ++hlf) {
-        const int col = j * 64 + cc * 16 + hlf * 8;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (r < nq && col < c.d)
-          w = __ldg(reinterpret_cast<const uint4*>(q + (qrow0 + r) * c.d + col));
-        raw[j][4 * hlf] = w.x;
-        raw[j][4 * hlf + 1] = w.y;
-        raw[j][4 * hlf + 2] = w.z;
-        raw[j][4 * hlf + 3] = w.w;
-      }
+        for (int hlf = 0; hlf < 2; ++hlf) {
+          const int col = j * 64 + cc * 16 + hlf * 8;
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (r < nq && col < c.d)
+            w = __ldg(reinterpret_cast<const uint4*>(q + (qrow0 + r) * c.d + col));
+          raw[j][4 * hlf] = w.x;
+          raw[j][4 * hlf + 1] = w.y;
+          raw[j][4 * hlf + 2] = w.z;
+          raw[j][4 * hlf + 3] = w.w;
+        }
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
+      for (int j = 0; j < NCH; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 f = unpack2<T>(raw[j][i]);
-        m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-      }
-    m = max(m, __shfl_xor_sync(kFull, m, 1));
-    m = max(m, __shfl_xor_sync(kFull, m, 2));
-    // largest element to [2^14, 2^15); fp16 needs none of it (its own range)
-    int e = 0;
-    if (sizeof(T) == 2 && !std::is_same<T, __half>::value && m != 0 && m < 0x7f800000u)
-      e = max(-120, (int)(m >> 23) - 127 - 14);
-    const float f_in = __uint_as_float((uint32_t)(127 - e) << 23);
+        for (int i = 0; i < 8; ++i) {
+          const float2 f = unpack2<T>(raw[j][i]);
+          m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+        }
+      m = max(m, __shfl_xor_sync(kFull, m, 1));
+      m = max(m, __shfl_xor_sync(kFull, m, 2));
+      // largest element to [2^14, 2^15); fp16 needs none of it (its own range)
+      int e = 0;
+      if (sizeof(T) == 2 && !std::is_same<T, __half>::value && m != 0 && m < 0x7f800000u)
+        e = max(-120, (int)(m >> 23) - 127 - 14);
+      const float f_in = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
+      for (int j = 0; j < NCH; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 f = unpack2<T>(raw[j][i]);
-        qf[t][j * 4 + (i >> 1)][i & 1] = tc::pack2<__half>(f.x * f_in, f.y * f_in);
-      }
-    const float f_out = __uint_as_float((uint32_t)(127 + e) << 23) * scale_log2;
-    qs[t][0] = __shfl_sync(kFull, f_out, (2 * cc) * 4);
-    qs[t][1] = __shfl_sync(kFull, f_out, (2 * cc + 1) * 4);
-  }
+        for (int i = 0; i < 8; ++i) {
+          const float2 f = unpack2<T>(raw[j][i]);
+          qf[t][j * 4 + (i >> 1)][i & 1] = tc::pack2<__half>(f.x * f_in, f.y * f_in);
+        }
+      const float f_out = __uint_as_float((uint32_t)(127 + e) << 23) * scale_log2;
+      qs[t][0] = __shfl_sync(kFull, f_out, (2 * cc) * 4);
+      qs[t][1] = __shfl_sync(kFull, f_out, (2 * cc + 1) * 4);
+    }
 
-  float acc[NQ][2 * VW][4];
-  float M[NQ][2], m[NQ][2], l[NQ][2];
+    float acc[NQ][2 * VW][4];
+    float M[NQ][2], m[NQ][2], l[NQ][2];
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
+    for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-    for (int i = 0; i < 2 * VW; ++i) acc[t][i][0] = acc[t][i][1] = acc[t][i][2] = acc[t][i][3] = 0.f;
-    M[t][0] = M[t][1] = m[t][0] = m[t][1] = -INFINITY;
-    l[t][0] = l[t][1] = 0.f;
-  }
+      for (int i = 0; i < 2 * VW; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][i][e] = 0.f;
+      M[t][0] = M[t][1] = m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+    }
 
-  // whether the loads of this warp's first step in the next run are under way
-  const bool into = has_next && warp < nxt.s1;
-  bool ahead = false;
-  for (; s < cur.s1; s += stride) {
-    const bool more = s + stride < cur.s1;
-    // S^T, one 16-row tile of keys by 8 query columns each
-    float x[NQ][KT][4];
+    // whether the loads of this warp's first step in the next run are under way
+    const bool into = has_next && warp < nxt.s1;
+    bool ahead = false;
+    for (; s < cur.s1; s += stride) {
+      const bool more = s + stride < cur.s1;
+      // S^T, one 16-row tile of keys by 8 query columns each
+      float x[NQ][KT][4];
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      sc[t][0] = sc_next[t][0];
-      sc[t][1] = sc_next[t][1];
+      for (int t = 0; t < KT; ++t) {
+        sc[t][0] = sc_next[t][0];
+        sc[t][1] = sc_next[t][1];
 #pragma unroll
-      for (int u = 0; u < NQ; ++u) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.f;
+        for (int u = 0; u < NQ; ++u) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.f;
 #pragma unroll
-      for (int j = 0; j < NCH; ++j) {
-        const uint32_t w0[4] = {kr[t][0][j].x, kr[t][0][j].y, kr[t][0][j].z, kr[t][0][j].w};
-        const uint32_t w1[4] = {kr[t][1][j].x, kr[t][1][j].y, kr[t][1][j].z, kr[t][1][j].w};
+        for (int j = 0; j < NCH; ++j) {
+          const uint32_t w0[4] = {kr[t][0][j].x, kr[t][0][j].y, kr[t][0][j].z, kr[t][0][j].w};
+          const uint32_t w1[4] = {kr[t][1][j].x, kr[t][1][j].y, kr[t][1][j].z, kr[t][1][j].w};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t a0, a1, a2, a3;
-          decode4<FMT>(w0[w], a0, a2);
-          decode4<FMT>(w1[w], a1, a3);
+          for (int w = 0; w < 4; ++w) {
+            uint32_t a0, a1, a2, a3;
+            decode4<FMT>(w0[w], a0, a2);
+            decode4<FMT>(w1[w], a1, a3);
 #pragma unroll
-          for (int u = 0; u < NQ; ++u)
-            mma_f16(x[u][t], a0, a1, a2, a3, qf[u][j * 4 + w][0], qf[u][j * 4 + w][1]);
+            for (int u = 0; u < NQ; ++u)
+              mma_f16(x[u][t], a0, a1, a2, a3, qf[u][j * 4 + w][0], qf[u][j * 4 + w][1]);
+          }
         }
       }
-    }
-    if (more) {
-      load_k(cur, s + stride);
-    } else if (into) {
-      load_k(nxt, warp);
-    }
-    // the scale of the keys' scores and the exponent of their values' (NaN for a bad row)
-    float ks[KT][2], ev[KT][2];
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t vbyte = sc[t][i] >> 8;
-        ks[t][i] = scale_value(sc[t][i] & 255u);
-        ev[t][i] = vbyte == kBadRow ? __uint_as_float(0x7fc00000u) : (float)((int)vbyte - 127);
+      if (more) {
+        load_k(cur, s + stride);
+      } else if (into) {
+        load_k(nxt, warp);
       }
-    const bool edge = (s + 1) * KS > n;
-    // online softmax; element e of a tile is key g + 8 (e / 2), query 2 cc + e % 2
-    uint32_t pb[NQ][KT][2];
-#pragma unroll
-    for (int u = 0; u < NQ; ++u) {
-      float y[KT][4];
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[u][t][e] *= ks[t][e >> 1] * qs[u][e & 1];
-          y[t][e] = x[u][t][e] + ev[t][e >> 1];
-        }
-      if (edge) {
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (s * KS + t * 16 + (e >> 1) * 8 + g >= n) x[u][t][e] = y[t][e] = -INFINITY;
-      }
-      float mx[2] = {-INFINITY, -INFINITY}, my[2] = {-INFINITY, -INFINITY};
+      // the scale of the keys' scores and the exponent of their values' (NaN for a bad row)
+      float ks[KT][2], ev[KT][2];
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          mx[i] = tc::max3f(mx[i], x[u][t][i], x[u][t][2 + i]);
-          my[i] = tc::max3f(my[i], y[t][i], y[t][2 + i]);
+          const uint32_t vbyte = sc[t][i] >> 8;
+          ks[t][i] = scale_value(sc[t][i] & 255u);
+          ev[t][i] = vbyte == kBadRow ? __uint_as_float(0x7fc00000u) : (float)((int)vbyte - 127);
         }
-      bool grow = false;
-      float old[2];
+      const bool edge = (s + 1) * KS > n;
+      // online softmax; element e of a tile is key g + 8 (e / 2), query 2 cc + e % 2
+      uint32_t pb[NQ][KT][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // row sum: this lane's own keys against its own maximum
-        const float mn = fmaxf(m[u][i], mx[i]);
-        const float r = mn == -INFINITY ? 0.f : mn;
-        l[u][i] *= ex2(m[u][i] - r);
-        m[u][i] = mn;
+      for (int u = 0; u < NQ; ++u) {
+        float y[KT][4];
 #pragma unroll
         for (int t = 0; t < KT; ++t)
-          l[u][i] += ex2(x[u][t][i] - r) + ex2(x[u][t][2 + i] - r);
-        // the accumulator's reference is shared by the warp's keys of a query
-        my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 4));
-        my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 8));
-        my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 16));
-        old[i] = M[u][i];
-        if (my[i] > M[u][i] + (M[u][i] == -INFINITY ? 0.f : kSlack)) {
-          M[u][i] = my[i];
-          grow = true;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[u][t][e] *= ks[t][e >> 1] * qs[u][e & 1];
+            y[t][e] = x[u][t][e] + ev[t][e >> 1];
+          }
+        if (edge) {
+#pragma unroll
+          for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (s * KS + t * 16 + (e >> 1) * 8 + g >= n) x[u][t][e] = y[t][e] = -INFINITY;
+        }
+        float mx[2] = {-INFINITY, -INFINITY}, my[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mx[i] = tc::max3f(mx[i], x[u][t][i], x[u][t][2 + i]);
+            my[i] = tc::max3f(my[i], y[t][i], y[t][2 + i]);
+          }
+        bool grow = false;
+        float old[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // row sum: this lane's own keys against its own maximum
+          const float mn = fmaxf(m[u][i], mx[i]);
+          const float r = mn == -INFINITY ? 0.f : mn;
+          l[u][i] *= ex2(m[u][i] - r);
+          m[u][i] = mn;
+#pragma unroll
+          for (int t = 0; t < KT; ++t)
+            l[u][i] += ex2(x[u][t][i] - r) + ex2(x[u][t][2 + i] - r);
+          // the accumulator's reference is shared by the warp's keys of a query
+          my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 4));
+          my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 8));
+          my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 16));
+          old[i] = M[u][i];
+          if (my[i] > M[u][i] + (M[u][i] == -INFINITY ? 0.f : kSlack)) {
+            M[u][i] = my[i];
+            grow = true;
+          }
+        }
+        if (__any_sync(kFull, grow)) {
+          float a[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) a[i] = old[i] == M[u][i] ? 1.f : ex2(old[i] - M[u][i]);
+#pragma unroll
+          for (int i = 0; i < 2 * VW; ++i) {
+            acc[u][i][0] *= a[0];
+            acc[u][i][1] *= a[1];
+            acc[u][i][2] *= a[0];
+            acc[u][i][3] *= a[1];
+          }
+        }
+        const float r0 = M[u][0] == -INFINITY ? 0.f : M[u][0];
+        const float r1 = M[u][1] == -INFINITY ? 0.f : M[u][1];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          pb[u][t][0] = movmatrix(tc::pack2<__half>(ex2(y[t][0] - r0), ex2(y[t][1] - r1)));
+          pb[u][t][1] = movmatrix(tc::pack2<__half>(ex2(y[t][2] - r0), ex2(y[t][3] - r1)));
         }
       }
-      if (__any_sync(kFull, grow)) {
-        float a[2];
+      // O^T += V^T P^T
 #pragma unroll
-        for (int i = 0; i < 2; ++i) a[i] = old[i] == M[u][i] ? 1.f : ex2(old[i] - M[u][i]);
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int i = 0; i < 2 * VW; ++i) {
-          acc[u][i][0] *= a[0];
-          acc[u][i][1] *= a[1];
-          acc[u][i][2] *= a[0];
-          acc[u][i][3] *= a[1];
+        for (int w = 0; w < VW; ++w) {
+          uint32_t a[2][4];   // the word's four columns make two m16 tiles
+          decode4<FMT>(__byte_perm(vr[t][0][w], vr[t][1][w], 0x5140), a[0][0], a[0][1]);
+          decode4<FMT>(__byte_perm(vr[t][2][w], vr[t][3][w], 0x5140), a[0][2], a[0][3]);
+          decode4<FMT>(__byte_perm(vr[t][0][w], vr[t][1][w], 0x7362), a[1][0], a[1][1]);
+          decode4<FMT>(__byte_perm(vr[t][2][w], vr[t][3][w], 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+          for (int u = 0; u < NQ; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              mma_f16(acc[u][2 * w + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[u][t][0],
+                      pb[u][t][1]);
         }
-      }
-      const float r0 = M[u][0] == -INFINITY ? 0.f : M[u][0];
-      const float r1 = M[u][1] == -INFINITY ? 0.f : M[u][1];
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        pb[u][t][0] = movmatrix(tc::pack2<__half>(ex2(y[t][0] - r0), ex2(y[t][1] - r1)));
-        pb[u][t][1] = movmatrix(tc::pack2<__half>(ex2(y[t][2] - r0), ex2(y[t][3] - r1)));
+      if (more) {
+        load_v(cur, s + stride);
+      } else if (into) {
+        load_v(nxt, warp);
+        ahead = true;
       }
     }
-    // O^T += V^T P^T
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        uint32_t a[2][4];   // the word's four columns make two m16 tiles
-        decode4<FMT>(__byte_perm(vr[t][0][w], vr[t][1][w], 0x5140), a[0][0], a[0][1]);
-        decode4<FMT>(__byte_perm(vr[t][2][w], vr[t][3][w], 0x5140), a[0][2], a[0][3]);
-        decode4<FMT>(__byte_perm(vr[t][0][w], vr[t][1][w], 0x7362), a[1][0], a[1][1]);
-        decode4<FMT>(__byte_perm(vr[t][2][w], vr[t][3][w], 0x7362), a[1][2], a[1][3]);
-#pragma unroll
-        for (int u = 0; u < NQ; ++u)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            mma_f16(acc[u][2 * w + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[u][t][0],
-                    pb[u][t][1]);
-      }
-    if (more) {
-      load_v(cur, s + stride);
-    } else if (into) {
+    if (into && !ahead) {   // a warp without a step in this run
+      load_k(nxt, warp);
       load_v(nxt, warp);
-      ahead = true;
     }
-  }
-  if (into && !ahead) {   // a warp without a step in this run
-    load_k(nxt, warp);
-    load_v(nxt, warp);
-  }
 
-  // ---- merge: lanes, then warps, then the CTAs of the cluster
-  float* so = att_smem;                                         // [warp][row][kPitch]
-  float* sM = so + kAttWarps * C::kRowsQ * C::kPitch;           // [warp][row] M, m, l
-  float* sm = sM + kAttWarps * C::kRowsQ;
-  float* sl = sm + kAttWarps * C::kRowsQ;
+    // ---- merge: lanes, then warps, then the CTAs of the cluster
+    float* so = att_smem;                                         // [warp][row][kPitch]
+    float* sM = so + kAttWarps * C::kRowsQ * C::kPitch;           // [warp][row] M, m, l
+    float* sm = sM + kAttWarps * C::kRowsQ;
+    float* sl = sm + kAttWarps * C::kRowsQ;
 #pragma unroll
-  for (int u = 0; u < NQ; ++u)
+    for (int u = 0; u < NQ; ++u)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        const float m2 = __shfl_xor_sync(kFull, m[u][i], d);
-        const float l2 = __shfl_xor_sync(kFull, l[u][i], d);
-        const float mn = fmaxf(m[u][i], m2);
-        const float r = mn == -INFINITY ? 0.f : mn;
-        l[u][i] = l[u][i] * ex2(m[u][i] - r) + l2 * ex2(m2 - r);
-        m[u][i] = mn;
+        for (int d = 4; d < 32; d <<= 1) {
+          const float m2 = __shfl_xor_sync(kFull, m[u][i], d);
+          const float l2 = __shfl_xor_sync(kFull, l[u][i], d);
+          const float mn = fmaxf(m[u][i], m2);
+          const float r = mn == -INFINITY ? 0.f : mn;
+          l[u][i] = l[u][i] * ex2(m[u][i] - r) + l2 * ex2(m2 - r);
+          m[u][i] = mn;
+        }
+        const int row = warp * C::kRowsQ + u * 8 + 2 * cc + i;
+        if (g == 0) {
+          sM[row] = M[u][i];
+          sm[row] = m[u][i];
+          sl[row] = l[u][i];
+        }
+        // lane g's columns: word w, bytes 2 t, 2 t + 1 (m16 tile t of the word)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          const int col = DP == 64 ? g * 8 + 4 * w : (w >> 2) * 128 + g * 16 + 4 * (w & 3);
+          *reinterpret_cast<float4*>(so + row * C::kPitch + col) =
+              make_float4(acc[u][2 * w][i], acc[u][2 * w][2 + i], acc[u][2 * w + 1][i],
+                          acc[u][2 * w + 1][2 + i]);
+        }
       }
-      const int row = warp * C::kRowsQ + u * 8 + 2 * cc + i;
-      if (g == 0) {
-        sM[row] = M[u][i];
-        sm[row] = m[u][i];
-        sl[row] = l[u][i];
-      }
-      // lane g's columns: word w, bytes 2 t, 2 t + 1 (m16 tile t of the word)
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const int col = DP == 64 ? g * 8 + 4 * w : (w >> 2) * 128 + g * 16 + 4 * (w & 3);
-        *reinterpret_cast<float4*>(so + row * C::kPitch + col) =
-            make_float4(acc[u][2 * w][i], acc[u][2 * w][2 + i], acc[u][2 * w + 1][i],
-                        acc[u][2 * w + 1][2 + i]);
+    __syncthreads();
+    // the CTA's warps into warp 0's place (each thread its own four columns of a row); maxima
+    // ignore NaN, which comes through the sums
+    float* cM = sl + kAttWarps * C::kRowsQ;   // [row] M, m, l of the CTA
+    float* cm = cM + C::kRowsQ;
+    float* cl = cm + C::kRowsQ;
+    auto write = [&](int row, int col, float Mx, float mx, float L, float4 a) {
+      att_write<T>(o, o32, lse, qrow0 + row, c.d, col, Mx, mx, L, a);
+    };
+    for (int idx = threadIdx.x; idx < nq * (DP / 4); idx += kAttWarps * 32) {
+      const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
+      float* mine = so + row * C::kPitch + col;
+      float Mx, mx, L;
+      float4 a;
+      att_join(kAttWarps,
+               [&](int k, int w) { return sM[(k * kAttWarps + w) * C::kRowsQ + row]; },
+               [&](int w) { return *reinterpret_cast<float4*>(mine + w * C::kRowsQ * C::kPitch); },
+               Mx, mx, L, a);
+      const bool whole = FLAT ? cur.s0 == 0 && cur.s1 == cur.steps : ns == 1;
+      if (whole) {
+        write(row, col, Mx, mx, L, a);
+      } else if constexpr (FLAT) {
+        // the end of a unit (slot 0), or its beginning (slot 1)
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (cur.s0 > 0 ? 0 : 1);
+        *reinterpret_cast<float4*>(ws.part + (slot * C::kRowsQ + row) * DP + col) = a;
+        if (col == 0) {
+          float* st = ws.stats + slot * 3 * C::kRowsQ + row;
+          st[0] = Mx;
+          st[C::kRowsQ] = mx;
+          st[2 * C::kRowsQ] = L;
+        }
+      } else {
+        *reinterpret_cast<float4*>(mine) = a;
+        if (col == 0) {
+          cM[row] = Mx;
+          cm[row] = mx;
+          cl[row] = L;
+        }
       }
     }
-  __syncthreads();
-  // the CTA's warps into warp 0's place (each thread its own four columns of a row); maxima
-  // ignore NaN, which comes through the sums
-  float* cM = sl + kAttWarps * C::kRowsQ;   // [row] M, m, l of the CTA
-  float* cm = cM + C::kRowsQ;
-  float* cl = cm + C::kRowsQ;
-  auto write = [&](int row, int col, float Mx, float mx, float L, float4 a) {
-    att_write<T>(o, o32, lse, qrow0 + row, c.d, col, Mx, mx, L, a);
-  };
-  for (int idx = threadIdx.x; idx < nq * (DP / 4); idx += kAttWarps * 32) {
-    const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
-    float* mine = so + row * C::kPitch + col;
-    float Mx, mx, L;
-    float4 a;
-    att_join(kAttWarps,
-             [&](int k, int w) { return sM[(k * kAttWarps + w) * C::kRowsQ + row]; },
-             [&](int w) { return *reinterpret_cast<float4*>(mine + w * C::kRowsQ * C::kPitch); },
-             Mx, mx, L, a);
-    const bool whole = FLAT ? cur.s0 == 0 && cur.s1 == cur.steps : ns == 1;
-    if (whole) {
-      write(row, col, Mx, mx, L, a);
-    } else if constexpr (FLAT) {
-      // the end of a unit (slot 0), or its beginning (slot 1)
-      const int64_t slot = 2 * (int64_t)blockIdx.x + (cur.s0 > 0 ? 0 : 1);
-      *reinterpret_cast<float4*>(ws.part + (slot * C::kRowsQ + row) * DP + col) = a;
-      if (col == 0) {
-        float* st = ws.stats + slot * 3 * C::kRowsQ + row;
-        st[0] = Mx;
-        st[C::kRowsQ] = mx;
-        st[2 * C::kRowsQ] = L;
+    if constexpr (!FLAT) {
+      if (ns == 1) {
+        leave();
+        return;
       }
-    } else {
-      *reinterpret_cast<float4*>(mine) = a;
-      if (col == 0) {
-        cM[row] = Mx;
-        cm[row] = mx;
-        cl[row] = L;
+      // the CTAs of the cluster: each takes its share of the rows' columns from all of them
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      for (int idx = rank * (kAttWarps * 32) + threadIdx.x; idx < nq * (DP / 4);
+           idx += ns * kAttWarps * 32) {
+        const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
+        float Mx, mx, L;
+        float4 a;
+        att_join(ns,
+                 [&](int k, int w) {
+                   return *cluster.map_shared_rank(cM + k * C::kRowsQ + row, w);
+                 },
+                 [&](int w) {
+                   return *reinterpret_cast<float4*>(
+                       cluster.map_shared_rank(so + row * C::kPitch + col, w));
+                 },
+                 Mx, mx, L, a);
+        write(row, col, Mx, mx, L, a);
       }
-    }
-  }
-  if constexpr (!FLAT) {
-    if (ns == 1) {
+      cluster.sync();   // peers may still read this CTA's memory
       leave();
       return;
     }
-    // the CTAs of the cluster: each takes its share of the rows' columns from all of them
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    for (int idx = rank * (kAttWarps * 32) + threadIdx.x; idx < nq * (DP / 4);
-         idx += ns * kAttWarps * 32) {
-      const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
-      float Mx, mx, L;
-      float4 a;
-      att_join(ns,
-               [&](int k, int w) { return *cluster.map_shared_rank(cM + k * C::kRowsQ + row, w); },
-               [&](int w) {
-                 return *reinterpret_cast<float4*>(
-                     cluster.map_shared_rank(so + row * C::kPitch + col, w));
-               },
-               Mx, mx, L, a);
-      write(row, col, Mx, mx, L, a);
+    if (!has_next) {
+      leave();
+      return;
     }
-    cluster.sync();   // peers may still read this CTA's memory
-    leave();
-    return;
-  }
-  if (!has_next) {
-    leave();
-    return;
-  }
-  __syncthreads();    // the merge has read what the next run's will overwrite
-  cur = nxt;
-  s = warp;
+    __syncthreads();    // the merge has read what the next run's will overwrite
+    cur = nxt;
+    s = warp;
   }
 }
 
@@ -1091,7 +1099,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
       att_write<T>(o, o32, lse, r.row + row, d, col, Mx, mx, L,
                    make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]));
     } else {   // two columns a lane: even lanes write their neighbour's as well
-      const float2 up = make_float2(__shfl_down_sync(kFull, a[0], 1), __shfl_down_sync(kFull, a[1], 1));
+      const float2 up = make_float2(__shfl_down_sync(kFull, a[0], 1),
+                                    __shfl_down_sync(kFull, a[1], 1));
       if (lane % 2 == 0)
         att_write<T>(o, o32, lse, r.row + row, d, col, Mx, mx, L,
                      make_float4(a[0], a[1], up.x, up.y));
@@ -1177,7 +1186,8 @@ int row_grid(int64_t B, int64_t H, int64_t rows, int per_cta, int unroll, int pa
   const int64_t want = (int64_t)device_sm_count() * ctas;
   const int64_t chunks = std::max<int64_t>(
       1, std::min((rows + step - 1) / step, (want + B * blocks - 1) / (B * blocks)));
-  if (blocks * chunks >= (1ll << 31)) return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many heads");
+  if (blocks * chunks >= (1ll << 31))
+    return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many heads");
   g->grid = dim3((unsigned)(blocks * chunks), (unsigned)B);
   g->head_blocks = (int)blocks;
   g->hs = hs;
@@ -1262,8 +1272,8 @@ int launch_attend(const QAttend& a, const QCache& c, const AttPlan& p) {
   {
     LaunchScope ls("qcache_attend_kernel", a.stream);
     if (int rc = check_cuda(
-            cudaLaunchKernelEx(&cfg, kern, (const T*)a.q, c, (const int64_t*)a.cache->lengths, (T*)a.o,
-                               a.o32, a.lse, (float)a.scale * kLog2e, group, p.chunks, p.ns,
+            cudaLaunchKernelEx(&cfg, kern, (const T*)a.q, c, (const int64_t*)a.cache->lengths,
+                               (T*)a.o, a.o32, a.lse, (float)a.scale * kLog2e, group, p.chunks, p.ns,
                                (int)a.cache->batch, a.beside, ws),
             "qcache_attend_kernel"))
       return rc;
@@ -1271,7 +1281,8 @@ int launch_attend(const QAttend& a, const QCache& c, const AttPlan& p) {
   if constexpr (FLAT) {
     LaunchScope ls("qcache_join_kernel", a.stream);
     return check_cuda(launch_early(qcache_join_kernel<T, DP, NQ>, (unsigned)p.grid,
-                                   kJoinWarps * 32, 0, a.stream, true, (T*)a.o, a.o32, a.lse, c.d, p.grid, ws),
+                                   kJoinWarps * 32, 0, a.stream, true, (T*)a.o, a.o32, a.lse,
+                                   c.d, p.grid, ws),
                       "qcache_join_kernel");
   }
   return SBFA_OK;
