@@ -367,6 +367,53 @@ def test_offsets_beyond_32_bits():
     assert ((o[0, 0, 0].double() - want).abs() <= 2.0 ** -7 * want).all()
 
 
+@pytest.mark.parametrize("B,H,G,W,top", [(65535, 1, 1, 9, 12), (3000, 3, 2, 40, 90),
+                                         (1, 70000, 1, 5, 4), (2, 300, 9, 33, 30)])
+def test_many_sequences_and_heads(B, H, G, W, top):
+    """Grids at their limits: every sequence's length, and a sample of the results."""
+    g = gen(13)
+    D = 64
+    c = Cache(B, H, D, 1, W, fmt="int8", device=DEV)
+    k, v = (torch.randn(B, H, 2, D, generator=g, device=DEV).bfloat16() for _ in range(2))
+    c.append(k, v)
+    assert (c.lengths == 2).all() and not c._tickets.any()
+    c._k.random_(0, 255, generator=g)
+    c._v.random_(0, 255, generator=g)
+    c.scales.random_(118, 124, generator=g)
+    c.lengths.random_(0, top + 1, generator=g)
+    q = torch.randn(B, H * G, 1, D, generator=g, device=DEV).bfloat16()
+    o, lse = c.attend(q, return_lse=True)
+    empty = c.lengths == 0
+    assert not o[empty].any() and not lse[empty].any()
+    assert (lse[~empty] != 0).all() and torch.isfinite(o).all()
+    for b, h in {(0, 0), (B - 1, H - 1), (B // 2, H // 3), (B // 3, H // 2), (B - 1, 0)}:
+        n = min(int(c.lengths[b]), 1 + W)
+        kk, vv = (x[:n] for x in ref.values(c, b, h))
+        hs = slice(h * G, (h + 1) * G)
+        eo, _, A, ds = ref.attention(q[b, hs, 0], kk, vv, 1 / math.sqrt(D))
+        big = vv.abs().max().item() if n else 0.0
+        ref.check(o[b, hs, 0], eo, A, ds, 2.0 ** -8, ref.U16, n * 2.0 ** -25 * big, f"b{b} h{h}")
+
+
+def test_two_attends_at_the_same_time():
+    g = gen(14)
+    c = filled(g, 32, 8, 128, 4, 1500, torch.bfloat16, "e4m3", [b * 50 for b in range(32)])
+    qs = [rows(g, (32, 32, 1, 128), torch.bfloat16) for _ in range(2)]
+    want = [c.attend(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    outs = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(c.attend(qs[i]))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
 def test_refusals():
     c = Cache(2, 2, 64, 4, 12, device=DEV)
     x = torch.zeros(2, 2, 3, 64, dtype=torch.bfloat16, device=DEV)

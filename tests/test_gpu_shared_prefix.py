@@ -234,6 +234,37 @@ def test_captured_and_replayed():
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
 
 
+def test_many_sequences_behind_a_prefix_on_two_streams():
+    """Several waves of prefix CTAs beside a cache cut into equal runs, twice at the same time."""
+    g = gen(31)
+    B, H, G, D, P, W = 700, 2, 4, 64, 260, 2500
+    pre = make(g, H, P, D, torch.float16)
+    c = filled(g, 4, H, D, 0, W, torch.float16, "int8", [0, 7, 2500, 9000])
+    big = QuantizedStreamingKVCache(B, H, D, 0, W, dtype=torch.float16, fmt="int8", device=DEV)
+    pick = torch.arange(B, device=DEV) % 4
+    big.load(c.k[pick], c.v[pick], c.scales[pick], c.lengths[pick])
+    qs = [rows(g, (4, H * G, 1, D), torch.float16, 0.2) for _ in range(2)]
+    want = [check_attend(c, q, prefix=pre) for q in qs]
+    outs = [big.attend(q[pick], return_lse=True, prefix=pre) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    again = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                again[i].append(big.attend(qs[i][pick], return_lse=True, prefix=pre))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for i in range(2):
+        # the same sums in another split: within the output's rounding and the weights'
+        tol = 4 * 2.0 ** -11 * want[i][0].double().abs().amax() + 1e-30
+        assert ((outs[i][0].double() - want[i][0][pick].double()).abs() <= tol).all()
+        assert ((outs[i][1] - want[i][1][pick]).abs() <= 1e-4 * (1 + want[i][1][pick].abs())).all()
+        assert all(torch.equal(a, b) for o in again[i] for a, b in zip(o, outs[i]))
+    assert native.device_status() == 0
+
+
 def test_prefix_copies_only_what_it_must():
     g = gen(28)
     k = rows(g, (2, 50, 64), torch.float16)
