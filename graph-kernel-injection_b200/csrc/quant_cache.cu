@@ -22,6 +22,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "quant_cache.cuh"
 #include "tc_prims.cuh"
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(kReadThreads)
 // Scales: a key's 2^ek multiplies its score in fp32.  A value row's 2^ev is folded
 // into the exponent of its weight: P' = 2^(x + ev - M), M a running bound of x + ev, so P'
 // is at most 2^kSlack and keeps fp16's 11 bits whatever the magnitudes of the rows, while
-// the row sum l = sum 2^(x - m) has its own per-lane maximum m (both in fp32); the result is
+// the row sum l = sum 2^(x - m) has its own per-lane reference m (both in fp32); the result is
 // acc / l * 2^(M - m).  Q is scaled by a power of two into fp16's range, which is exact
 // for fp16 inputs and for bf16 down to 2^-38 of the row's largest element.
 //
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
 
     // Q fragments, column g of each n-tile, scaled into fp16's range
     uint32_t qf[NQ][DP / 16][2];
-    float qs[NQ][2];   // softmax scale (base 2) over the two query columns of this lane
+    float2 qs[NQ];   // softmax scale (base 2) of the two query columns of this lane
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
       const int r = t * 8 + g;
@@ -752,20 +753,20 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
           qf[t][j * 4 + (i >> 1)][i & 1] = tc::pack2<__half>(f.x * f_in, f.y * f_in);
         }
       const float f_out = __uint_as_float((uint32_t)(127 + e) << 23) * scale_log2;
-      qs[t][0] = __shfl_sync(kFull, f_out, (2 * cc) * 4);
-      qs[t][1] = __shfl_sync(kFull, f_out, (2 * cc + 1) * 4);
+      qs[t] = make_float2(__shfl_sync(kFull, f_out, (2 * cc) * 4),
+                          __shfl_sync(kFull, f_out, (2 * cc + 1) * 4));
     }
 
     float acc[NQ][2 * VW][4];
-    float M[NQ][2], m[NQ][2], l[NQ][2];
+    float2 M[NQ], m[NQ], l[NQ];
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
 #pragma unroll
       for (int i = 0; i < 2 * VW; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[t][i][e] = 0.f;
-      M[t][0] = M[t][1] = m[t][0] = m[t][1] = -INFINITY;
-      l[t][0] = l[t][1] = 0.f;
+      M[t] = m[t] = make_float2(-FLT_MAX, -FLT_MAX);   // below every score, and finite
+      l[t] = make_float2(0.f, 0.f);
     }
 
     // whether the loads of this warp's first step in the next run are under way
@@ -812,74 +813,71 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
           ev[t][i] = vbyte == kBadRow ? __uint_as_float(0x7fc00000u) : (float)((int)vbyte - 127);
         }
       const bool edge = (s + 1) * KS > n;
-      // online softmax; element e of a tile is key g + 8 (e / 2), query 2 cc + e % 2
+      // Online softmax; element e of a tile is key g + 8 (e / 2), query 2 cc + e % 2, and the two
+      // queries go through packed fp32 pairs.  Both references only move when a score is above
+      // them by more than kSlack (rare behind the first steps), which a warp votes on once.
       uint32_t pb[NQ][KT][2];
 #pragma unroll
       for (int u = 0; u < NQ; ++u) {
-        float y[KT][4];
+        float2 xs[KT][2], ys[KT][2];
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[u][t][e] *= ks[t][e >> 1] * qs[u][e & 1];
-            y[t][e] = x[u][t][e] + ev[t][e >> 1];
+          for (int i = 0; i < 2; ++i) {
+            xs[t][i] = __fmul2_rn(make_float2(x[u][t][2 * i], x[u][t][2 * i + 1]),
+                                  __fmul2_rn(qs[u], make_float2(ks[t][i], ks[t][i])));
+            ys[t][i] = __fadd2_rn(xs[t][i], make_float2(ev[t][i], ev[t][i]));
           }
         if (edge) {
 #pragma unroll
           for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (s * KS + t * 16 + (e >> 1) * 8 + g >= n) x[u][t][e] = y[t][e] = -INFINITY;
+            for (int i = 0; i < 2; ++i)
+              if (s * KS + t * 16 + i * 8 + g >= n)
+                xs[t][i] = ys[t][i] = make_float2(-INFINITY, -INFINITY);
         }
-        float mx[2] = {-INFINITY, -INFINITY}, my[2] = {-INFINITY, -INFINITY};
+        float2 mx = xs[0][0], my = ys[0][0];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {   // maxima ignore NaN
+          mx.x = tc::max3f(mx.x, xs[t][0].x, xs[t][1].x);
+          mx.y = tc::max3f(mx.y, xs[t][0].y, xs[t][1].y);
+          my.x = tc::max3f(my.x, ys[t][0].x, ys[t][1].x);
+          my.y = tc::max3f(my.y, ys[t][0].y, ys[t][1].y);
+        }
+        const bool grow = mx.x > m[u].x + kSlack || mx.y > m[u].y + kSlack ||
+                          my.x > M[u].x + kSlack || my.y > M[u].y + kSlack;
+        if (__any_sync(kFull, grow)) {
+          // the row sum's reference is this lane's own
+          const float2 mn = make_float2(fmaxf(m[u].x, mx.x), fmaxf(m[u].y, mx.y));
+          l[u].x *= ex2(m[u].x - mn.x);
+          l[u].y *= ex2(m[u].y - mn.y);
+          m[u] = mn;
+          // the accumulator's is shared by the warp's keys of a query
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            my.x = fmaxf(my.x, __shfl_xor_sync(kFull, my.x, d));
+            my.y = fmaxf(my.y, __shfl_xor_sync(kFull, my.y, d));
+          }
+          const float2 Mn = make_float2(fmaxf(M[u].x, my.x), fmaxf(M[u].y, my.y));
+          const float2 f = make_float2(ex2(M[u].x - Mn.x), ex2(M[u].y - Mn.y));
+          M[u] = Mn;
+#pragma unroll
+          for (int i = 0; i < 2 * VW; ++i) {
+            acc[u][i][0] *= f.x;
+            acc[u][i][1] *= f.y;
+            acc[u][i][2] *= f.x;
+            acc[u][i][3] *= f.y;
+          }
+        }
+        const float2 nm = make_float2(-m[u].x, -m[u].y), nM = make_float2(-M[u].x, -M[u].y);
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            mx[i] = tc::max3f(mx[i], x[u][t][i], x[u][t][2 + i]);
-            my[i] = tc::max3f(my[i], y[t][i], y[t][2 + i]);
+            const float2 a = __fadd2_rn(xs[t][i], nm), b = __fadd2_rn(ys[t][i], nM);
+            l[u] = __fadd2_rn(l[u], make_float2(ex2(a.x), ex2(a.y)));
+            pb[u][t][i] = movmatrix(tc::pack2<__half>(ex2(b.x), ex2(b.y)));
           }
-        bool grow = false;
-        float old[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          // row sum: this lane's own keys against its own maximum
-          const float mn = fmaxf(m[u][i], mx[i]);
-          const float r = mn == -INFINITY ? 0.f : mn;
-          l[u][i] *= ex2(m[u][i] - r);
-          m[u][i] = mn;
-#pragma unroll
-          for (int t = 0; t < KT; ++t)
-            l[u][i] += ex2(x[u][t][i] - r) + ex2(x[u][t][2 + i] - r);
-          // the accumulator's reference is shared by the warp's keys of a query
-          my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 4));
-          my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 8));
-          my[i] = fmaxf(my[i], __shfl_xor_sync(kFull, my[i], 16));
-          old[i] = M[u][i];
-          if (my[i] > M[u][i] + (M[u][i] == -INFINITY ? 0.f : kSlack)) {
-            M[u][i] = my[i];
-            grow = true;
-          }
-        }
-        if (__any_sync(kFull, grow)) {
-          float a[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) a[i] = old[i] == M[u][i] ? 1.f : ex2(old[i] - M[u][i]);
-#pragma unroll
-          for (int i = 0; i < 2 * VW; ++i) {
-            acc[u][i][0] *= a[0];
-            acc[u][i][1] *= a[1];
-            acc[u][i][2] *= a[0];
-            acc[u][i][3] *= a[1];
-          }
-        }
-        const float r0 = M[u][0] == -INFINITY ? 0.f : M[u][0];
-        const float r1 = M[u][1] == -INFINITY ? 0.f : M[u][1];
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          pb[u][t][0] = movmatrix(tc::pack2<__half>(ex2(y[t][0] - r0), ex2(y[t][1] - r1)));
-          pb[u][t][1] = movmatrix(tc::pack2<__half>(ex2(y[t][2] - r0), ex2(y[t][3] - r1)));
-        }
       }
       // O^T += V^T P^T
 #pragma unroll
@@ -919,20 +917,20 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     for (int u = 0; u < NQ; ++u)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        float mi = i == 0 ? m[u].x : m[u].y, li = i == 0 ? l[u].x : l[u].y;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
-          const float m2 = __shfl_xor_sync(kFull, m[u][i], d);
-          const float l2 = __shfl_xor_sync(kFull, l[u][i], d);
-          const float mn = fmaxf(m[u][i], m2);
-          const float r = mn == -INFINITY ? 0.f : mn;
-          l[u][i] = l[u][i] * ex2(m[u][i] - r) + l2 * ex2(m2 - r);
-          m[u][i] = mn;
+          const float m2 = __shfl_xor_sync(kFull, mi, d);
+          const float l2 = __shfl_xor_sync(kFull, li, d);
+          const float mn = fmaxf(mi, m2);
+          li = li * ex2(mi - mn) + l2 * ex2(m2 - mn);
+          mi = mn;
         }
         const int row = warp * C::kRowsQ + u * 8 + 2 * cc + i;
         if (g == 0) {
-          sM[row] = M[u][i];
-          sm[row] = m[u][i];
-          sl[row] = l[u][i];
+          sM[row] = i == 0 ? M[u].x : M[u].y;
+          sm[row] = mi;
+          sl[row] = li;
         }
         // lane g's columns: word w, bytes 2 t, 2 t + 1 (m16 tile t of the word)
 #pragma unroll

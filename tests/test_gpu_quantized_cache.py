@@ -428,7 +428,8 @@ def test_refusals():
                 lambda: c.attend(q[:, :0]), lambda: c.attend(q.half()),
                 lambda: c.load(c.k, c.v, c.scales, c.lengths - 1),
                 lambda: c.load(c.k, c.v, c.scales, c.lengths.int()),
-                lambda: c.load(c.k[:1], c.v, c.scales, c.lengths)):
+                lambda: c.load(c.k[:1], c.v, c.scales, c.lengths),
+                lambda: c.load(c.k.view(torch.int8), c.v, c.scales, c.lengths)):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(RuntimeError, match="softmax_scale"):
