@@ -139,11 +139,26 @@ def stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def launch(name: str, device: torch.device, *args) -> None:
+    """Calls entry point ``name``, whose last argument is the stream, on ``device``'s current one,
+    with ``device`` (which has an index) current.  One short path for the serving operators, whose
+    small calls are bound by the host."""
+    fn = getattr(lib(), name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name.removeprefix("sbfa_"))
+
+
 _NO_GUARD = contextlib.nullcontext()
 
 
 def device_guard(device: torch.device):
-    """Makes ``device`` current for a launch; free when it already is."""
+    """Makes ``device`` current; free when it already is."""
     return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 

@@ -94,23 +94,22 @@ class SharedPrefix:
         q = vector_readable(q)
         B, H, N, D = q.shape
         dev = self.device
-        o = torch.empty((B, H, N, D), dtype=self.dtype, device=dev)
-        lse = torch.empty((B, H, N), dtype=torch.float32, device=dev) if return_lse else None
-        with native.device_guard(dev):
-            ws, ws_bytes = self._workspace(B, H, N, 0)
-            native.check(native.lib().sbfa_prefix_attend(
-                q.data_ptr(), stride_array(q.stride()[:3]), self.k.data_ptr(),
-                self.v.data_ptr(), native.ptr(own_o), native.ptr(own_lse),
-                o.data_ptr(), native.ptr(lse), B, H, self.heads, N, self.length, D, self._code,
-                scale, native.ptr(ws), ws_bytes, native.stream_ptr(dev)), "prefix_attend")
+        o = torch.empty(B, H, N, D, dtype=self.dtype, device=dev)
+        lse = torch.empty(B, H, N, dtype=torch.float32, device=dev) if return_lse else None
+        ws, ws_bytes = self._workspace(B, H, N, 0)
+        native.launch("sbfa_prefix_attend", dev, q.data_ptr(), stride_array(q.stride()[:3]),
+                      self.k.data_ptr(), self.v.data_ptr(), native.ptr(own_o),
+                      native.ptr(own_lse), o.data_ptr(), native.ptr(lse), B, H, self.heads, N,
+                      self.length, D, self._code, scale, native.ptr(ws), ws_bytes)
         return o, lse
 
     def _workspace(self, B: int, H: int, N: int, window: int):
         """Scratch of one call (from torch's allocator, so of its stream or graph) and its bytes."""
         need = self._scratch.get((B, H, N, window))
         if need is None:
-            need = self._remember((B, H, N, window), native.lib().sbfa_prefix_workspace_bytes(
-                B, H, self.heads, N, self.length, self.head_dim, window))
+            with native.device_guard(self.device):
+                need = self._remember((B, H, N, window), native.lib().sbfa_prefix_workspace_bytes(
+                    B, H, self.heads, N, self.length, self.head_dim, window))
         if need <= 0:   # none, or a bad shape that the call refuses
             return None, 0
         return torch.empty(need, dtype=torch.uint8, device=self.device), need
@@ -132,18 +131,17 @@ class SharedPrefix:
         B, H = q.shape[:2]
         dev = self.device
         o = torch.empty_like(q)
-        lse = torch.empty((B, H, 1), dtype=torch.float32, device=dev) if return_lse else None
-        with native.device_guard(dev):
-            sizes = (B, H, cache.sink_size, cache.window_size, "cache")
-            need = self._scratch.get(sizes)
-            if need is None:
+        lse = torch.empty(B, H, 1, dtype=torch.float32, device=dev) if return_lse else None
+        sizes = (B, H, cache.sink_size, cache.window_size, "cache")
+        need = self._scratch.get(sizes)
+        if need is None:
+            with native.device_guard(dev):
                 need = self._remember(sizes, native.lib().sbfa_qcache_prefix_workspace_bytes(
                     cache._handle, H, self.length))
-            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-            native.check(native.lib().sbfa_qcache_prefix_attend(
-                cache._handle, q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.length,
-                o.data_ptr(), native.ptr(lse), H, scale, ws.data_ptr(), need,
-                native.stream_ptr(dev)), "qcache_prefix_attend")
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        native.launch("sbfa_qcache_prefix_attend", dev, cache._handle, q.data_ptr(),
+                      self.k.data_ptr(), self.v.data_ptr(), self.length, o.data_ptr(),
+                      native.ptr(lse), H, scale, ws.data_ptr(), need)
         return (o, lse) if return_lse else o
 
     def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
@@ -174,16 +172,14 @@ class SharedPrefix:
         scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
         q, k, v = vector_readable(q), tma_readable(k), tma_readable(v)
         dev = self.device
-        o = torch.empty((B, H, N, D), dtype=self.dtype, device=dev)
-        lse = torch.empty((B, H, N), dtype=torch.float32, device=dev) if return_lse else None
-        with native.device_guard(dev):
-            ws, ws_bytes = self._workspace(B, H, N, window_size)
-            strides = stride_array((*q.stride()[:3], *stk._strides3(k), *stk._strides3(v)))
-            native.check(native.lib().sbfa_prefix_prompt(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, self.k.data_ptr(),
-                self.v.data_ptr(), o.data_ptr(), native.ptr(lse), B, H, self.heads, N,
-                self.length, D, self._code, scale, window_size, native.ptr(ws), ws_bytes,
-                native.stream_ptr(dev)), "prefix_prompt")
+        o = torch.empty(B, H, N, D, dtype=self.dtype, device=dev)
+        lse = torch.empty(B, H, N, dtype=torch.float32, device=dev) if return_lse else None
+        ws, ws_bytes = self._workspace(B, H, N, window_size)
+        strides = stride_array((*q.stride()[:3], *stk._strides3(k), *stk._strides3(v)))
+        native.launch("sbfa_prefix_prompt", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides,
+                      self.k.data_ptr(), self.v.data_ptr(), o.data_ptr(), native.ptr(lse), B, H,
+                      self.heads, N, self.length, D, self._code, scale, window_size,
+                      native.ptr(ws), ws_bytes)
         return (o, lse) if return_lse else o
 
 

@@ -189,18 +189,20 @@ class QuantizedStreamingKVCache:
     def _check(self, t: torch.Tensor, shape: Tuple[int, ...], name: str) -> None:
         if t.shape != shape:
             raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-        if t.device != self.device or t.dtype != self.dtype:
+        if t.dtype != self.dtype or t.device != self.device:
             raise ValueError(f"{name} must be {self.dtype} on {self.device}")
-        no_gradients(t)
+        if t.requires_grad:
+            no_gradients(t)
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor,
                counts: Optional[torch.Tensor] = None) -> None:
         """Quantise and append the next ``t`` tokens of every sequence ([B, H, t, D],
         views welcome).  ``counts`` (int64 [B] on the device, clamped to [0, t]) says how many
         of them each sequence takes: the rest of a right-padded batch is not read."""
-        if k_new.dim() != 4:
-            raise ValueError(f"k_new must be [B, H, t, D], got {tuple(k_new.shape)}")
-        n = k_new.shape[2]
+        shape = k_new.shape
+        if len(shape) != 4:
+            raise ValueError(f"k_new must be [B, H, t, D], got {tuple(shape)}")
+        n = shape[2]
         shape = (self.batch, self.heads, n, self.head_dim)
         self._check(k_new, shape, "k_new")
         self._check(v_new, shape, "v_new")
@@ -213,10 +215,8 @@ class QuantizedStreamingKVCache:
             return
         k_new, v_new = vector_readable(k_new), vector_readable(v_new)
         strides = stride_array(k_new.stride()[:3] + v_new.stride()[:3])
-        with native.device_guard(self.device):
-            native.check(native.lib().sbfa_qcache_append(
-                self._handle, k_new.data_ptr(), v_new.data_ptr(), strides, native.ptr(counts), n,
-                native.stream_ptr(self.device)), "qcache_append")
+        native.launch("sbfa_qcache_append", self.device, self._handle, k_new.data_ptr(),
+                      v_new.data_ptr(), strides, None if counts is None else counts.data_ptr(), n)
 
     def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
                return_lse: bool = False, prefix: Optional[SharedPrefix] = None):
@@ -225,30 +225,32 @@ class QuantizedStreamingKVCache:
         ``return_lse``, the natural-log LSE ([B, Hq, 1] fp32).  A sequence that has no
         token yet gives zeros.  With ``prefix`` every query sees that shared prefix as
         well: the merged result is rounded once."""
-        if q.dim() != 4 or q.shape[1] == 0 or q.shape[1] % self.heads:
+        shape = q.shape
+        hq = shape[1] if len(shape) == 4 else 0
+        if hq == 0 or hq % self.heads:
             raise ValueError(f"q must be [B, Hq, 1, D] with Hq a multiple of {self.heads}, got "
-                             f"{tuple(q.shape)}")
-        hq = q.shape[1]
+                             f"{tuple(shape)}")
         self._check(q, (self.batch, hq, 1, self.head_dim), "q")
         scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
         q = q.contiguous()
-        if q.data_ptr() % 16:
+        if q.data_ptr() & 15:
             q = q.clone()
         if prefix is not None:
             return prefix.attend_cached(self, q, scale, return_lse)
-        o = torch.empty_like(q)
-        lse = (torch.empty(self.batch, hq, 1, dtype=torch.float32, device=self.device)
-               if return_lse else None)
-        with native.device_guard(self.device):
-            need = self._scratch.get(hq)
-            if need is None:
+        need = self._scratch.get(hq)
+        if need is None:
+            with native.device_guard(self.device):
                 need = self._scratch[hq] = native.lib().sbfa_qcache_attend_workspace_bytes(
                     self._handle, hq)
-            # from torch's allocator, so of the call's stream or graph
-            ws = (torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None)
-            native.check(native.lib().sbfa_qcache_attend(
-                self._handle, q.data_ptr(), o.data_ptr(), native.ptr(lse), hq, scale,
-                native.ptr(ws), need, native.stream_ptr(self.device)), "qcache_attend")
+        o = torch.empty_like(q)
+        lse = ws = None
+        if return_lse:
+            lse = torch.empty(self.batch, hq, 1, dtype=torch.float32, device=self.device)
+        if need > 0:   # from torch's allocator, so of the call's stream or graph
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        native.launch("sbfa_qcache_attend", self.device, self._handle, q.data_ptr(), o.data_ptr(),
+                      None if lse is None else lse.data_ptr(), hq, scale,
+                      None if ws is None else ws.data_ptr(), need)
         return (o, lse) if return_lse else o
 
     def read(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -260,10 +262,8 @@ class QuantizedStreamingKVCache:
                         device=self.device)
         v = torch.empty_like(k)
         positions = torch.empty(self.batch, rows, dtype=torch.int64, device=self.device)
-        with native.device_guard(self.device):
-            native.check(native.lib().sbfa_qcache_read(
-                self._handle, k.data_ptr(), v.data_ptr(), positions.data_ptr(),
-                native.stream_ptr(self.device)), "qcache_read")
+        native.launch("sbfa_qcache_read", self.device, self._handle, k.data_ptr(), v.data_ptr(),
+                      positions.data_ptr())
         return k, v, positions
 
     def load(self, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor,
