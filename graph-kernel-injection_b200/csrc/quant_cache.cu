@@ -520,6 +520,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
   auto steps_of = [&](int n) { return FLAT ? max(1, (n + KS - 1) / KS) : (n + KS - 1) / KS; };
   auto cost_of = [&](int n) { return (int64_t)(steps_of(n) + kRunSteps); };
 
+  // Runs end with the last unit whatever the lengths read later say: a caller's append that races
+  // with this call spoils its result, not memory.
+  auto last_unit = [&](const AttRun& r) { return r.hc + 1 == hcs && r.b + 1 == batch; };
+
   AttRun cur;
   int64_t left = 0;       // cost that this CTA takes behind the current unit
   int stride, rank = 0;
@@ -553,7 +557,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     if (begin >= (incl - mine) * hcs && begin < incl * hcs) {
       int64_t rem = begin - (incl - mine) * hcs;
       int b = b_lo, n = visible(b);
-      for (; rem >= cost_of(n) * hcs; n = visible(++b)) rem -= cost_of(n) * hcs;
+      for (; b + 1 < b_hi && rem >= cost_of(n) * hcs; n = visible(++b)) rem -= cost_of(n) * hcs;
       first[0] = b;
       first[1] = n;
       inside = rem;
@@ -568,14 +572,14 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     cur.n = first[1];
     cur.steps = steps_of(cur.n);
     const int64_t cost = cost_of(cur.n);
-    cur.hc = (int)(inside / cost);
+    cur.hc = (int)min(inside / cost, (int64_t)hcs - 1);
     const int64_t at = inside - cur.hc * cost;     // place of `begin` in its unit
     cur.s0 = (int)min(at, (int64_t)cur.steps);
     cur.s1 = (int)min((int64_t)cur.steps, at + (end - begin));
     left = max((int64_t)0, end - begin - (cost - at));
     const int64_t unit_start = begin - at;
     if (cur.s0 >= cur.s1) {                        // nothing of that unit: begin with the next
-      if (left == 0) {
+      if (left == 0 || last_unit(cur)) {
         leave();
         return;
       }
@@ -691,7 +695,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
   for (;;) {
     // the run behind this one, which starts its unit
     AttRun nxt = cur;
-    const bool has_next = FLAT && left > 0;
+    const bool has_next = FLAT && left > 0 && !last_unit(cur);
     if (has_next) {
       nxt.hc = cur.hc + 1;
       if (nxt.hc == hcs) {
@@ -1170,7 +1174,8 @@ int by_format(int dtype, int fmt, int64_t D, F&& f) {
 
 // Grid of the append and read kernels for `rows` rows of each head: 2^hs heads per CTA
 // where a head has fewer rows than a CTA takes at a time, else as many CTAs along a head as
-// make `ctas` per SM in all, each with at least `passes` passes.
+// make `ctas` per SM in all, each with at least `passes` passes.  (One token of 8 sequences with
+// 8 heads: 2.8 us with the heads in one CTA, 3.5 with a CTA each.)
 struct RowGrid {
   dim3 grid;
   int head_blocks, hs;
@@ -1212,13 +1217,14 @@ int attend_plan(int64_t B, int64_t kv_heads, int64_t group, int64_t d, int64_t r
   if (units >= (1ll << 27) || kv_heads * p->chunks >= (1ll << 27))
     return fail(SBFA_ERR_UNSUPPORTED, "8-bit cache: too many (sequence, head) units");
   const int64_t slots = (int64_t)(device_sm_count() - busy_sms) * att_ctas(dp, p->nq);
-  // A cluster shortens a unit while there are SMs to fill.
+  // A cluster shortens a unit while there are SMs to fill (8 heads x 1028 rows: 12.4, 9.7, 7.6,
+  // 6.9 us on 1, 2, 4, 8 CTAs a unit), with some steps for each of its warps.
   p->ns = 1;
   while (p->ns < 8 && units * p->ns * 2 <= slots && rows > (int64_t)p->ns * 128) p->ns *= 2;
-  // What its last, partly filled wave costs in rows of a CTA beyond an equal share; the FLAT form's
-  // scan and second kernel cost 4 to 5 us, about what 960 rows of 128 bytes take.  64 x 8 heads x
-  // 2048 rows (two waves) 62 -> 52 us, 8 x 8 x 16384 60 -> 51; 64 x 8 x 256 would go from 12 to 17,
-  // 16 x 8 x 2048 from 19 to 22.
+  // What its last, partly filled wave costs in rows of a CTA beyond an equal share; the FLAT
+  // form's scan and second kernel cost 4 to 5 us, about what 960 rows of 128 bytes take.  64 x 8
+  // heads x 2048 rows (two waves) 62 -> 52 us, 8 x 8 x 16384 60 -> 51; 64 x 8 x 256 would go from
+  // 12 to 17, 16 x 8 x 2048 from 19 to 22.
   const int64_t waves = (units * p->ns + slots - 1) / slots;
   const int64_t lost = waves * rows / p->ns - units * rows / slots;
   // Beside a prefix's kernel SMs come free meanwhile, so a last wave costs about half of that.
