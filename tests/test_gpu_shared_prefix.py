@@ -84,10 +84,12 @@ def test_decode_behind_a_prefix(fmt, dtype, B, H, G, D, P, W, lengths):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_decode_behind_a_prefix_with_the_16_bit_cache(dtype):
+@pytest.mark.parametrize("Hkv,P,D", [(3, 300, 64), (1, 100, 128), (1, 9000, 128), (3, 1, 64)])
+def test_decode_behind_a_prefix_with_the_16_bit_cache(dtype, Hkv, P, D):
+    """One head per query head in the ring, fewer in the prefix; keys whole and cut into slices."""
     g = gen(24)
-    B, H, D, P, S, W = 2, 3, 64, 300, 2, 50
-    pre = make(g, H, P, D, dtype)
+    B, H, S, W = 2, 3, 2, 50
+    pre = make(g, Hkv, P, D, dtype)
     c = StreamingKVCache(B, H, D, S, W, dtype=dtype, device=DEV)
     k, v = (rows(g, (B, H, 90, D), dtype, 0.2) for _ in range(2))
     q = rows(g, (B, H, 1, D), dtype, 0.2)
@@ -98,8 +100,9 @@ def test_decode_behind_a_prefix_with_the_16_bit_cache(dtype):
     u = ref.half_step(dtype)
     for b in range(B):
         for h in range(H):
-            eo, el, A, ds = ref.attention(q[b, h], torch.cat((pre.k[h], k[b, h, keep])),
-                                          torch.cat((pre.v[h], v[b, h, keep])),
+            p = h * Hkv // H
+            eo, el, A, ds = ref.attention(q[b, h], torch.cat((pre.k[p], k[b, h, keep])),
+                                          torch.cat((pre.v[p], v[b, h, keep])),
                                           1 / math.sqrt(D))
             # the own part is rounded once before the merge: u A more
             ref.check(o[b, h], eo, A, ds, u, 2 * u)
