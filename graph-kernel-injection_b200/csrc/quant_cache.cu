@@ -132,8 +132,8 @@ template <> __device__ __forceinline__ uint32_t pack2_sat<__nv_bfloat16>(float a
 // A group of 8 lanes (16 at 256 columns) takes one (head, token): pieces of 16 bytes of K and
 // of V, the row maxima in packed 16-bit integers (the magnitudes of both 16-bit types are
 // ordered like their bits) with one shuffle chain for both, 8 code bytes back per piece. Bound
-// by HBM (4 D bytes in, 2 D + 2 out per head and token) and nearly by instruction issue: 16 x 8
-// x 2048 rows of 128 take 45 us with 16 lanes a row and fp32 maxima, 38 us so.  A CTA covers
+// by HBM (4 D bytes in, 2 D + 2 out per head and token): 16 x 8 x 2048 rows of 128 take 45 us
+// with 16 lanes a row and fp32 maxima, 38.5 us so (and with fewer instructions).  A CTA covers
 // 2^hs heads x kRows / 2^hs tokens at a time (tokens adjacent, so that their scale pairs share
 // sectors; several heads only where a call has few tokens) and walks the tokens that survive
 // the call: positions that a later token of it overwrites are never visited.  The last CTA of a
