@@ -38,6 +38,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kFull = 0xffffffffu;
 constexpr uint32_t kBadRow = 255;   // scale byte of a row with a NaN or an infinity
+constexpr uint32_t kZeroByte = 127;   // of a row of zeros (and of others with e = 0)
 
 // ---------------------------------------------------------------------------
 // codes and scales
@@ -47,7 +48,7 @@ constexpr uint32_t kBadRow = 255;   // scale byte of a row with a NaN or an infi
 template <int FMT>
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
   if (amax >= 0x7f800000u) return kBadRow;
-  if (amax == 0) return 127;
+  if (amax == 0) return kZeroByte;
   // amax = f * 2^E, f in [1, 2); top = 1.75 * 2^8 or 1.984375 * 2^6
   constexpr int kTopExp = FMT == SBFA_Q_E4M3 ? 8 : 6;
   constexpr uint32_t kTopMant = FMT == SBFA_Q_E4M3 ? 0x600000u : 0x7e0000u;
@@ -77,6 +78,11 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     const uint32_t z = (uint32_t)__float2int_rn(c) & 0xffu, w = (uint32_t)__float2int_rn(d) & 0xffu;
     return x | (y << 8) | (z << 16) | (w << 24);
   }
+}
+// The bits of four codes that are all zero where the codes are: e4m3 has a negative zero.
+template <int FMT>
+__device__ __forceinline__ constexpr uint32_t code_mask() {
+  return FMT == SBFA_Q_E4M3 ? 0x7f7f7f7fu : 0xffffffffu;
 }
 // Codes 0, 1 (lo) and 2, 3 (hi) of a word as half pairs (exact).
 template <int FMT>
@@ -354,7 +360,7 @@ __global__ void __launch_bounds__(kReadThreads)
 // into the exponent of its weight: P' = 2^(x + ev - M), M a running bound of x + ev, so P'
 // is at most 2^kSlack and keeps fp16's 11 bits whatever the magnitudes of the rows, while
 // the row sum l = sum 2^(x - m) has its own per-lane reference m (both in fp32); the result is
-// acc / l * 2^(M - m).  Q is scaled by a power of two into fp16's range, which is exact
+// acc / l * 2^(M - m).  A row of zeros, which has a scale all the same, does not enter M.  Q is scaled by a power of two into fp16's range, which is exact
 // for fp16 inputs and for bf16 down to 2^-38 of the row's largest element.
 //
 // Two ways to spread the units (sequence, key/value head, group of queries) over the GPU:
@@ -808,6 +814,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
       }
       // the scale of the keys' scores and the exponent of their values' (NaN for a bad row)
       float ks[KT][2], ev[KT][2];
+      bool maybe_zero = false;
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -815,7 +822,31 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
           const uint32_t vbyte = sc[t][i] >> 8;
           ks[t][i] = scale_value(sc[t][i] & 255u);
           ev[t][i] = vbyte == kBadRow ? __uint_as_float(0x7fc00000u) : (float)((int)vbyte - 127);
+          maybe_zero |= vbyte == kZeroByte;
         }
+      // A value row of zeros shares its byte with rows whose largest value is next to the top code.
+      // It adds nothing to O, so its weight must not set the others' reference either: an attention
+      // sink of zeros 10 powers of two above values of 2^-10 left none of their bits.  (Where every
+      // row has this byte, 64 x 32 heads x 2052 rows take 184 us instead of 176.)
+      if (__any_sync(kFull, maybe_zero)) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          uint32_t holds[4];   // lanes that hold a code other than 0 of their row i
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int w = 0; w < VW; ++w) any |= vr[t][i][w];
+            holds[i] = __ballot_sync(kFull, (any & code_mask<FMT>()) != 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {   // row g + 8 i is row 2 i + g % 2 of the lanes with cc = g / 2
+            const uint32_t row = g & 1 ? holds[2 * i + 1] : holds[2 * i];
+            if (sc[t][i] >> 8 == kZeroByte && (row & (0x11111111u << (g >> 1))) == 0)
+              ev[t][i] = -INFINITY;
+          }
+        }
+      }
       const bool edge = (s + 1) * KS > n;
       // Online softmax; element e of a tile is key g + 8 (e / 2), query 2 cc + e % 2, and the two
       // queries go through packed fp32 pairs.  Both references only move when a score is above
