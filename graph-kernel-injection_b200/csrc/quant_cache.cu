@@ -357,11 +357,14 @@ __global__ void __launch_bounds__(kReadThreads)
 // P^T comes out of the score fragment with movmatrix.  Codes become fp16 exactly.
 //
 // Scales: a key's 2^ek multiplies its score in fp32.  A value row's 2^ev is folded
-// into the exponent of its weight: P' = 2^(x + ev - M), M a running bound of x + ev, so P'
-// is at most 2^kSlack and keeps fp16's 11 bits whatever the magnitudes of the rows, while
-// the row sum l = sum 2^(x - m) has its own per-lane reference m (both in fp32); the result is
-// acc / l * 2^(M - m).  A row of zeros, which has a scale all the same, does not enter M.  Q is scaled by a power of two into fp16's range, which is exact
-// for fp16 inputs and for bf16 down to 2^-38 of the row's largest element.
+// into the exponent of its weight: P' = 2^(x + ev - M), M a running reference kLift below the largest
+// x + ev so far, so P' is at most 2^(kLift + kSlack), just below fp16's largest: a weight times
+// scale keeps fp16's 11 bits down to 2^-25 of the largest one and is off by up to 2^-36 of it below.
+// The row sum l = sum 2^(x - m) has its own per-lane reference m (both in fp32); the result is
+// acc / l * 2^(M - m).  A row of zeros, which has a scale all the same, does not enter M.  Q is
+// scaled by a power of two into fp16's range, which is exact for fp16 inputs and for bf16 down to
+// 2^-31 of the row's largest element (8 significant bits above fp16's step of 2^-24; smaller
+// elements lose their last ones).
 //
 // Two ways to spread the units (sequence, key/value head, group of queries) over the GPU:
 //  - few units: a cluster of NS CTAs shares one, its warps take every (4 NS)-th step of KS
@@ -373,7 +376,8 @@ __global__ void __launch_bounds__(kReadThreads)
 //    loads stay in flight across units.  A unit that crosses from one CTA to the next leaves
 //    partial rows that qcache_join_kernel merges, in order.
 constexpr int kAttWarps = 4;
-constexpr float kSlack = 4.f;
+constexpr float kSlack = 4.f;   // how far scores may pass a reference before it moves
+constexpr float kLift = 11.f;   // 2^(kLift + kSlack) * 448 * rows fits fp32, 2^(kLift + kSlack) fp16
 
 // Resident CTAs per SM that the registers are limited for.  At two sets of query columns steps
 // of 32 rows on two CTAs beat steps of 16 on three (64 x 8 heads of 12 queries x 2052 rows: 72
@@ -849,8 +853,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
       }
       const bool edge = (s + 1) * KS > n;
       // Online softmax; element e of a tile is key g + 8 (e / 2), query 2 cc + e % 2, and the two
-      // queries go through packed fp32 pairs.  Both references only move when a score is above
-      // them by more than kSlack (rare behind the first steps), which a warp votes on once.
+      // queries go through packed fp32 pairs.  Both references only move when a score passes what
+      // they hold by more than kSlack (rare behind the first steps), which a warp votes on once.
       uint32_t pb[NQ][KT][2];
 #pragma unroll
       for (int u = 0; u < NQ; ++u) {
@@ -880,7 +884,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
           my.y = tc::max3f(my.y, ys[t][0].y, ys[t][1].y);
         }
         const bool grow = mx.x > m[u].x + kSlack || mx.y > m[u].y + kSlack ||
-                          my.x > M[u].x + kSlack || my.y > M[u].y + kSlack;
+                          my.x > M[u].x + (kLift + kSlack) || my.y > M[u].y + (kLift + kSlack);
         if (__any_sync(kFull, grow)) {
           // the row sum's reference is this lane's own
           const float2 mn = make_float2(fmaxf(m[u].x, mx.x), fmaxf(m[u].y, mx.y));
@@ -893,7 +897,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
             my.x = fmaxf(my.x, __shfl_xor_sync(kFull, my.x, d));
             my.y = fmaxf(my.y, __shfl_xor_sync(kFull, my.y, d));
           }
-          const float2 Mn = make_float2(fmaxf(M[u].x, my.x), fmaxf(M[u].y, my.y));
+          const float2 Mn =
+              make_float2(fmaxf(M[u].x, my.x - kLift), fmaxf(M[u].y, my.y - kLift));
           const float2 f = make_float2(ex2(M[u].x - Mn.x), ex2(M[u].y - Mn.y));
           M[u] = Mn;
 #pragma unroll

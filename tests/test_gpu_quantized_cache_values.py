@@ -123,3 +123,36 @@ def test_zero_rows_beside_rows_of_the_same_scale_byte(fmt, dtype):
     assert torch.isnan(bad[2, 4:]).all() and torch.equal(bad_lse, lse)
     bad[2, 4:] = o[2, 4:]
     assert torch.equal(bad, o)
+
+
+@pytest.mark.parametrize("fmt,dtype", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_a_row_large_in_one_column_does_not_coarsen_the_others(form, fmt, dtype):
+    """The first row holds 2^10 in one column, zeros in the others, and a score 14 powers of two above
+    the rest: the other columns come from the other rows alone.
+
+    Bound: the kernel's reference M of the weighted values lies at least 11 powers of two below
+    the largest weight times scale, so a weight that falls below fp16's normal range is off by at most
+    2^-25 2^M <= 2^-36 max_i(w_i 2^e_i) for each code of the column."""
+    g = gen(44)
+    B, D = 36, 128
+    c, H, n, G, prefix = cache_of(form, B, D, dtype, fmt)
+    k, q = keys_and_queries(g, B, H, G, n, D, dtype)
+    v = 1 + 0.5 * torch.randn(B, H, n, D, generator=g, device=DEV)
+    v[:, :, 0], k[:, :, 0, 0] = 0.0, 14 / 4
+    v[:, :, 0, 17] = 2.0 ** 10
+    c.append(k.to(dtype), v.to(dtype))
+    o = c.attend(q, LOG2, prefix=prefix)
+    u = ref.half_step(dtype)
+    u_p = ref.U16 if prefix is None else max(u, ref.U16)
+    for b in range(B):
+        for h in range(H):
+            kk, vv = ref.values(c, b, h)
+            scale = torch.exp2(c.scales[b, h, :, 1].double() - 127)
+            if prefix is not None:
+                kk, vv = torch.cat((prefix.k[h].double(), kk)), torch.cat((prefix.v[h].double(), vv))
+            hs = slice(h * G, (h + 1) * G)
+            eo, _, A, ds = ref.attention(q[b, hs, 0], kk, vv, LOG2)
+            w = torch.softmax(q[b, hs, 0].double() @ kk.T * LOG2, -1)[:, -n:]
+            extra = (w * scale).amax(-1)[:, None] * c.v[b, h].double().abs().sum(0) * 2.0 ** -36
+            ref.check(o[b, hs, 0], eo, A, ds, u, u_p, extra, f"b{b} h{h}")
