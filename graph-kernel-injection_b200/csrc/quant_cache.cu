@@ -449,12 +449,12 @@ __device__ __forceinline__ void att_join(int parts, S&& stat, V&& vec, float& Mx
   }
 }
 
-// O (rounded, or fp32 to o32) and LSE of four columns of row `out`.
+// O (rounded, or fp32 to o32) and LSE of four columns of row `out`; `some`: whether its sequence has
+// rows.  Where all their scores are minus infinity L is 0 and the result NaN, with that LSE.
 template <typename T>
 __device__ __forceinline__ void att_write(T* o, float* o32, float* lse, int64_t out, int d, int col,
-                                          float Mx, float mx, float L, float4 a) {
-  const bool some = !(L == 0.f);
-  const float f = some ? 1.f / L : 0.f;
+                                          bool some, float Mx, float mx, float L, float4 a) {
+  const float f = 1.f / L;
   const float back = ex2((Mx == -INFINITY ? 0.f : Mx) - (mx == -INFINITY ? 0.f : mx));
   a.x = some ? a.x * f * back : 0.f;
   a.y = some ? a.y * f * back : 0.f;
@@ -988,7 +988,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (AttCfg<DP, NQ>::kCtas))
     float* cm = cM + C::kRowsQ;
     float* cl = cm + C::kRowsQ;
     auto write = [&](int row, int col, float Mx, float mx, float L, float4 a) {
-      att_write<T>(o, o32, lse, qrow0 + row, c.d, col, Mx, mx, L, a);
+      att_write<T>(o, o32, lse, qrow0 + row, c.d, col, n > 0, Mx, mx, L, a);
     };
     for (int idx = threadIdx.x; idx < nq * (DP / 4); idx += kAttWarps * 32) {
       const int row = idx / (DP / 4), col = idx % (DP / 4) * 4;
@@ -1134,13 +1134,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   for (int i = 0; i < VEC; i += 4) {
     const int col = lane * VEC + i;
     if constexpr (VEC >= 4) {
-      att_write<T>(o, o32, lse, r.row + row, d, col, Mx, mx, L,
+      att_write<T>(o, o32, lse, r.row + row, d, col, true, Mx, mx, L,
                    make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]));
     } else {   // two columns a lane: even lanes write their neighbour's as well
       const float2 up = make_float2(__shfl_down_sync(kFull, a[0], 1),
                                     __shfl_down_sync(kFull, a[1], 1));
       if (lane % 2 == 0)
-        att_write<T>(o, o32, lse, r.row + row, d, col, Mx, mx, L,
+        att_write<T>(o, o32, lse, r.row + row, d, col, true, Mx, mx, L,
                      make_float4(a[0], a[1], up.x, up.y));
     }
   }

@@ -1,6 +1,7 @@
 """Attention over the 8-bit ring where one value row must not decide how finely the others are
 weighed: rows of zeros (an attention sink, a padding token) and rows that are large in one column.
-In every form of the kernel: a cluster per unit, equal runs, behind a prefix."""
+In every form of the kernel: a cluster per unit, equal runs, behind a prefix.  And scores that are
+all minus infinity."""
 
 from __future__ import annotations
 
@@ -13,7 +14,7 @@ import sbfa_native as native
 from shared_prefix import SharedPrefix
 from streaming_kv_cache import QuantizedStreamingKVCache as Cache
 from tests import serving_reference as ref
-from tests.test_gpu_quantized_cache import gen
+from tests.test_gpu_quantized_cache import gen, rows
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -156,3 +157,29 @@ def test_a_row_large_in_one_column_does_not_coarsen_the_others(form, fmt, dtype)
             w = torch.softmax(q[b, hs, 0].double() @ kk.T * LOG2, -1)[:, -n:]
             extra = (w * scale).amax(-1)[:, None] * c.v[b, h].double().abs().sum(0) * 2.0 ** -36
             ref.check(o[b, hs, 0], eo, A, ds, u, u_p, extra, f"b{b} h{h}")
+
+
+@pytest.mark.parametrize("H,n,G,ws", [(1, 40, 3, 0), (4, 6000, 2, 1)])
+def test_scores_of_minus_infinity_only(H, n, G, ws):
+    """A sequence whose every score overflows to minus infinity has tokens: it gives the NaN and the
+    LSE of minus infinity that the formula gives, not an empty sequence's zeros, and behind a
+    prefix what the prefix gives alone."""
+    D, B, dt = 128, 36, torch.bfloat16
+    c = Cache(B, H, D, 4, n - 4, dtype=dt, device=DEV)
+    assert (native.lib().sbfa_qcache_attend_workspace_bytes(c._handle, H * G) > 0) == bool(ws)
+    k, v = torch.zeros(B, H, n, D, dtype=dt, device=DEV), rows(gen(45), (B, H, n, D), dt)
+    q = torch.zeros(B, H * G, 1, D, dtype=dt, device=DEV)
+    q[..., 0], k[..., 0] = 3e38, -3e38
+    counts = torch.full((B,), n, device=DEV)
+    counts[::3] = 0
+    counts[1::3] = torch.arange(1, n, n // 12, device=DEV)[:12]
+    c.append(k, v, counts)
+    o, lse = c.attend(q, return_lse=True)
+    some = counts > 0
+    assert not o[~some].any() and not lse[~some].any()
+    assert torch.isnan(o[some]).all() and (lse[some] == -math.inf).all()
+    pre = SharedPrefix(torch.zeros(H, 70, D, dtype=dt, device=DEV), rows(gen(46), (H, 70, D), dt))
+    o, lse = c.attend(q, return_lse=True, prefix=pre)
+    c.reset()
+    alone = c.attend(q, return_lse=True, prefix=pre)
+    assert torch.equal(o, alone[0]) and torch.equal(lse, alone[1])
