@@ -400,6 +400,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int seq = row / per;
       const int hg = (row - seq * per) / geo.n_q;
       const int iq = row - seq * per - hg * geo.n_q;   // the row's query of its sequence
+      // columns [lo, hi) of own key tile t that this row sees, off the column of its sequence's
+      // token 0; none in a tile of other sequences
+      auto own_keys = [&](int t, int* lo, int* hi, int* off) {
+        int b, kt;
+        own.at(t - geo.n_tiles, &b, &kt);
+        const int seqs = kTN / geo.box;
+        const int s = seq - b * seqs;                  // this row's sequence in the tile
+        *off = s * geo.box - kt * kTN;
+        *lo = *off + max(iq - geo.window + 1, 0);
+        *hi = live && s >= 0 && s < seqs ? *off + iq + 1 : 0;
+      };
       {  // gather this warp's query rows, D / 8 lanes a row; columns behind d and rows behind
          // R are zero.  (A row per lane would touch 32 lines with every load: 1.5 us more.)
         const T* mine = live ? q + seq * geo.sb + ((int64_t)kvh * geo.group + hg) * geo.sh +
@@ -438,18 +449,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
         bool all_vis = t < geo.n_tiles - 1;   // all but the prefix's last tile are full
         if (!all_vis) {
-          int lo = 0, hi;
-          if (t < geo.n_tiles) {
+          int lo = 0, hi, off;
+          if (t < geo.n_tiles)
             hi = geo.P - t * kTN;
-          } else {
-            int b, kt;
-            own.at(t - geo.n_tiles, &b, &kt);
-            const int seqs = kTN / geo.box;
-            const int s = seq - b * seqs;                  // this row's sequence in the tile
-            const int off = s * geo.box - kt * kTN;
-            lo = off + max(iq - geo.window + 1, 0);
-            hi = live && s >= 0 && s < seqs ? off + iq + 1 : 0;
-          }
+          else
+            own_keys(t, &lo, &hi, &off);
           vis[0] = range_bits(lo, hi, kHalf * h);
           vis[1] = range_bits(lo, hi, kHalf * h + 32);
           all_vis = __all_sync(0xffffffffu, (vis[0] & vis[1]) == 0xffffffffu);
@@ -577,18 +581,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         };
-        // columns [c0, c0 + 32) of what the fourth warp took out of the value rows that this
-        // row sees
+        // columns [c0, c0 + 32) of what the fourth warp took out of the value rows that this row
+        // sees in this CTA's own tiles (another slice adds its own: here such a row may have no key
+        // at all, and then a weight of 0 in the merge, which an infinity must not meet)
         const bool patch = live && *bad_flag != 0;
         auto put_back = [&](float* f, int c0) {
           const T* v = (const T*)out.own_v + seq * out.sv.b + (int64_t)kvh * out.sv.h + c0;
-          for (int k = max(iq - geo.window + 1, 0); k <= iq; ++k)
+          for (int j = j_own; j < n; ++j) {
+            int lo, hi, off;
+            own_keys(t0 + j, &lo, &hi, &off);
+            for (int c = max(lo, 0); c < min(hi, kTN); ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c0 + i < geo.d) {
-                const float y = Elem<T>::to(v[k * out.sv.n + i]);
-                if (!(fabsf(y) < INFINITY)) f[i] += y;
-              }
+              for (int i = 0; i < 32; ++i)
+                if (c0 + i < geo.d) {
+                  const float y = Elem<T>::to(v[(c - off) * out.sv.n + i]);
+                  if (!(fabsf(y) < INFINITY)) f[i] += y;
+                }
+          }
         };
         if (sliced) {
           const int64_t all = (int64_t)geo.n_tail * (kPair * kTM);
