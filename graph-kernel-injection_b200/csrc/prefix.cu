@@ -16,10 +16,10 @@
 // key), many by the tensor cores and the exponentials (4 D operations and one exponential per
 // row and key).
 //
-// The batch's own prompts (n_q tokens each, causal window) follow as more key tiles of
-// the same pass: a tile of 128 keys of one sequence, or of 128 / 2^k short
+// The batch's own prompts (n_q tokens each, causal window and own sinks) follow as more key
+// tiles of the same pass: a tile of 128 keys of one sequence, or of 128 / 2^k short
 // sequences with 2^k >= n_q rows each, in which each query row sees one interval
-// of columns.  So a prompt takes one launch, and its two parts share one softmax and
+// of columns, or two where a tile holds sinks.  So a prompt takes one launch, and its two parts share one softmax and
 // one rounding.  A value row in a tile belongs to some of the tile's query rows only, and a
 // weight of zero does not keep a NaN or an infinity out of the others' sums: a fourth
 // warp looks over every own V tile as it arrives, replaces such elements by zeros and
@@ -72,6 +72,7 @@ struct PrefixGeom {
   int n_tiles;         // 128-key tiles of the prefix
   int own;             // whether own tokens follow the prefix
   int window, box;     // their window; rows of a TMA box of own keys (128 / box sequences a tile)
+  int sink;            // first own tokens that every later one sees
 };
 
 // How a row's attention to its own tokens comes from a cache's kernel: O of the output type (every
@@ -99,13 +100,14 @@ __device__ __forceinline__ int64_t out_row(const PrefixGeom& g, int kvh, int row
 }
 
 // The own-key tiles that rows [row0, row1) need, in order: sequence by sequence (box == 128;
-// the first one's from its window's oldest key), or blocks of 128 / box sequences.
+// the first one's with its sinks and from its window's oldest key), or blocks of 128 / box sequences.
 struct OwnTiles {
-  int b0, kt0, c0;   // first sequence (or block), its first tile and tiles
+  int b0, kt0, c0;   // first sequence (or block), its window's first tile, its tiles in all
+  int sinks;         // of them ahead of the window's
   int full;          // tiles of a whole sequence
   int count;
   __device__ __forceinline__ OwnTiles(const PrefixGeom& g, int row0, int row1) {
-    b0 = kt0 = c0 = count = 0;
+    b0 = kt0 = c0 = sinks = count = 0;
     full = 1;
     if (!g.own) return;
     const int per = g.group * g.n_q;
@@ -124,7 +126,8 @@ struct OwnTiles {
     const bool one = lo / g.n_q == hi / g.n_q;
     const int q_lo = one ? lo % g.n_q : 0, q_hi = one ? hi % g.n_q : g.n_q - 1;
     kt0 = max(0, q_lo - g.window + 1) / kTN;
-    c0 = q_hi / kTN - kt0 + 1;
+    sinks = min(kt0, (g.sink + kTN - 1) / kTN);
+    c0 = sinks + q_hi / kTN - kt0 + 1;
     count = c0;
     if (b1 > b0) {
       const int last = row1 - 1 - b1 * per;
@@ -135,7 +138,7 @@ struct OwnTiles {
   __device__ __forceinline__ void at(int u, int* b, int* kt) const {
     if (u < c0) {
       *b = b0;
-      *kt = kt0 + u;
+      *kt = u < sinks ? u : kt0 + u - sinks;
     } else {
       *b = b0 + 1 + (u - c0) / full;
       *kt = (u - c0) % full;
@@ -400,8 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int seq = row / per;
       const int hg = (row - seq * per) / geo.n_q;
       const int iq = row - seq * per - hg * geo.n_q;   // the row's query of its sequence
-      // columns [lo, hi) of own key tile t that this row sees, off the column of its sequence's
-      // token 0; none in a tile of other sequences
+      // Columns of own key tile t that this row sees: [lo, hi), and from off, its sequence's token
+      // 0, to off + sink as far as they lie ahead of hi.  None in a tile of other sequences.
       auto own_keys = [&](int t, int* lo, int* hi, int* off) {
         int b, kt;
         own.at(t - geo.n_tiles, &b, &kt);
@@ -456,6 +459,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             own_keys(t, &lo, &hi, &off);
           vis[0] = range_bits(lo, hi, kHalf * h);
           vis[1] = range_bits(lo, hi, kHalf * h + 32);
+          if (t >= geo.n_tiles && geo.sink > 0) {
+            const int end = min(off + geo.sink, hi);
+            vis[0] |= range_bits(off, end, kHalf * h);
+            vis[1] |= range_bits(off, end, kHalf * h + 32);
+          }
           all_vis = __all_sync(0xffffffffu, (vis[0] & vis[1]) == 0xffffffffu);
         }
         ok = wait_bar_w(bar(L::kSFull + 2 * x + h), (uint32_t)((u >> 1) & 1), abort_flag, status);
@@ -590,13 +598,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = j_own; j < n; ++j) {
             int lo, hi, off;
             own_keys(t0 + j, &lo, &hi, &off);
-            for (int c = max(lo, 0); c < min(hi, kTN); ++c)
+            for (int c = max(off, 0); c < min(hi, kTN); ++c) {
+              if (c >= off + geo.sink && c < lo) continue;
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (c0 + i < geo.d) {
                   const float y = Elem<T>::to(v[(c - off) * out.sv.n + i]);
                   if (!(fabsf(y) < INFINITY)) f[i] += y;
                 }
+            }
           }
         };
         if (sliced) {
@@ -808,6 +818,7 @@ bool prefix_geometry(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_
   geo->n_tiles = ceil_div_i(P, kTN);
   geo->own = window > 0;
   geo->window = (int)std::min<int64_t>(window, n_q);
+  geo->sink = 0;
   // a box of own keys holds one sequence's rows: the least power of two, at least the 8 rows
   // of a swizzle atom; more than 64 rows take whole tiles of one sequence
   int box = 8;
@@ -1047,10 +1058,23 @@ extern "C" int sbfa_prefix_prompt(const void* q, const void* k, const void* v,
                                   int64_t kv_heads, int64_t n_q, int64_t P, int64_t head_dim,
                                   int dtype, double softmax_scale, int64_t window, void* ws,
                                   int64_t ws_bytes, void* stream) {
+  return sbfa_prefix_prompt_sinks(q, k, v, strides, k_prefix, v_prefix, o, lse, B, H, kv_heads, n_q,
+                                  P, head_dim, dtype, softmax_scale, 0, window, ws, ws_bytes, stream);
+}
+
+extern "C" int sbfa_prefix_prompt_sinks(const void* q, const void* k, const void* v,
+                                        const int64_t* strides, const void* k_prefix,
+                                        const void* v_prefix, void* o, float* lse, int64_t B,
+                                        int64_t H, int64_t kv_heads, int64_t n_q, int64_t P,
+                                        int64_t head_dim, int dtype, double softmax_scale,
+                                        int64_t sink, int64_t window, void* ws, int64_t ws_bytes,
+                                        void* stream) {
   PrefixGeom geo;
   if (int rc = check_prefix(B, H, kv_heads, n_q, P, head_dim, dtype, window, &geo)) return rc;
   if (window < 1)
     return fail(SBFA_ERR_INVALID, "sbfa_prefix_prompt: window must be at least 1");
+  if (sink < 0) return fail(SBFA_ERR_INVALID, "sbfa_prefix_prompt: sink must not be negative");
+  geo.sink = (int)std::min(sink, n_q);
   if (!k || !v) return fail(SBFA_ERR_INVALID, "sbfa_prefix_prompt: NULL tensor pointer");
   PrefixCall c = {};
   c.q = q;

@@ -82,6 +82,8 @@ _SIGNATURES = {
                             _i64, _i32, _f64, _vp, _i64, _vp], _i32),
     "sbfa_prefix_prompt": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                             _i64, _i32, _f64, _i64, _vp, _i64, _vp], _i32),
+    "sbfa_prefix_prompt_sinks": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                  _i64, _i64, _i32, _f64, _i64, _i64, _vp, _i64, _vp], _i32),
     "sbfa_prefix_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "sbfa_decode_noalloc": ([_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _f64, _i32,
                              _i64, _i64, _vp, _i64, _i64, _vp], _i32),

@@ -153,11 +153,14 @@ class SharedPrefix:
         return (o, lse) if return_lse else o
 
     def attend_prompt(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window_size: int,
-                      softmax_scale: Optional[float] = None, return_lse: bool = False):
+                      softmax_scale: Optional[float] = None, return_lse: bool = False,
+                      sink_size: int = 0):
         """Attention of the batch's own prompts behind the prefix: query ``i`` of a sequence
         ([B, H, N, D]) sees the whole prefix and the sequence's tokens ``(i - window_size, i]``
-        of ``k``, ``v`` ([B, H_kv, N, D]); views welcome.  Right-padded prompts need no
-        lengths: no query sees a token behind it.  One pass over both parts."""
+        and, of the first ``sink_size``, those up to ``i``, of ``k``, ``v`` ([B, H_kv, N, D]; views
+        welcome).  Give the two sizes of the cache that goes on from the prompt: behind a prefix it
+        shows its sinks to every later token.  Right-padded prompts need no lengths: no query sees
+        a token behind it.  One pass over both parts."""
         self._check(q)
         B, H, N, D = q.shape
         if tuple(k.shape) != (B, self.heads, N, D) or k.shape != v.shape:
@@ -168,6 +171,8 @@ class SharedPrefix:
                 raise ValueError(f"k and v must be {self.dtype} on {self.device}")
         if window_size < 1:
             raise ValueError("window_size must be at least 1: a query sees its own token")
+        if sink_size < 0:
+            raise ValueError("sink_size must not be negative")
         no_gradients(k, v)
         scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
         q, k, v = vector_readable(q), tma_readable(k), tma_readable(v)
@@ -176,9 +181,9 @@ class SharedPrefix:
         lse = torch.empty(B, H, N, dtype=torch.float32, device=dev) if return_lse else None
         ws, ws_bytes = self._workspace(B, H, N, window_size)
         strides = stride_array((*q.stride()[:3], *stk._strides3(k), *stk._strides3(v)))
-        native.launch("sbfa_prefix_prompt", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides,
+        native.launch("sbfa_prefix_prompt_sinks", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides,
                       self.k.data_ptr(), self.v.data_ptr(), o.data_ptr(), native.ptr(lse), B, H,
-                      self.heads, N, self.length, D, self._code, scale, window_size,
+                      self.heads, N, self.length, D, self._code, scale, sink_size, window_size,
                       native.ptr(ws), ws_bytes)
         return (o, lse) if return_lse else o
 

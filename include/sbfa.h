@@ -397,7 +397,15 @@ int sbfa_prefix_prompt(const void* q, const void* k, const void* v, const int64_
                        int64_t head_dim, int dtype, double softmax_scale, int64_t window,
                        void* ws, int64_t ws_bytes, void* stream);
 
-/* Scratch bytes sbfa_prefix_attend (window = 0) or sbfa_prefix_prompt needs for this shape
+/* The same with `sink` (>= 0) own sinks: query i also sees its sequence's tokens [0, min(sink,
+ * i + 1)), as a cache with that sink_size behind the prefix shows them to every later token. */
+int sbfa_prefix_prompt_sinks(const void* q, const void* k, const void* v, const int64_t* strides,
+                             const void* k_prefix, const void* v_prefix, void* o, float* lse,
+                             int64_t B, int64_t H, int64_t kv_heads, int64_t n_q, int64_t P,
+                             int64_t head_dim, int dtype, double softmax_scale, int64_t sink,
+                             int64_t window, void* ws, int64_t ws_bytes, void* stream);
+
+/* Scratch bytes sbfa_prefix_attend (window = 0) or sbfa_prefix_prompt[_sinks] needs for this shape
  * on the current device (may be 0; ws may then be NULL), -1 for a bad shape. */
 int64_t sbfa_prefix_workspace_bytes(int64_t B, int64_t H, int64_t kv_heads, int64_t n_q,
                                     int64_t P, int64_t head_dim, int64_t window);
