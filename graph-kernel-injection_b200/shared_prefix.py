@@ -22,14 +22,24 @@ import math
 from typing import Dict, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 import sbfa_native as native
 import sparse_triton_kernel as stk
+
 
 def no_gradients(*tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("this serving operator has no gradients: call it under torch.no_grad() "
                            "or with detached tensors")
+    if in_dual_level() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("this serving operator has no forward-mode gradients: call it with the "
+                           "primals")
+
+
+def in_dual_level() -> bool:
+    """Whether tensors may carry tangents at all."""
+    return forward_ad._current_level >= 0
 
 
 def vector_readable(t: torch.Tensor) -> torch.Tensor:

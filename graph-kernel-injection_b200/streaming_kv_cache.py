@@ -25,7 +25,8 @@ from typing import Optional, Tuple
 import torch
 
 import sbfa_native as native
-from shared_prefix import SharedPrefix, no_gradients, stride_array, vector_readable
+from shared_prefix import (SharedPrefix, in_dual_level, no_gradients, stride_array,
+                           vector_readable)
 
 
 class StreamingKVCache:
@@ -191,7 +192,7 @@ class QuantizedStreamingKVCache:
             raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
         if t.dtype != self.dtype or t.device != self.device:
             raise ValueError(f"{name} must be {self.dtype} on {self.device}")
-        if t.requires_grad:
+        if t.requires_grad or in_dual_level():
             no_gradients(t)
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor,
