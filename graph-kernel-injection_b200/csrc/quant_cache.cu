@@ -1277,15 +1277,7 @@ template <typename T, int FMT, int DP, int NQ, bool FLAT>
 int launch_attend(const QAttend& a, const QCache& c, const AttPlan& p) {
   using C = AttCfg<DP, NQ>;
   auto kern = qcache_attend_kernel<T, FMT, DP, NQ, FLAT>;
-  static std::atomic<uint64_t> ready{0};
-  if (C::kBytes > 48 * 1024)
-    if (int rc = once_per_device(ready, [&] {
-          return check_cuda(
-              cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)C::kBytes),
-              "cudaFuncSetAttribute(qcache_attend)");
-        }))
-      return rc;
+  static_assert(C::kBytes <= 48 * 1024, "more shared memory than a launch gets unasked");
   FlatWs ws = {};
   ws.rec = (FlatRecord*)a.ws;
   ws.stats = (float*)(ws.rec + p.grid);
