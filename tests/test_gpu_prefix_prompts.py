@@ -144,3 +144,22 @@ def test_sink_size_must_not_be_negative():
     x = torch.zeros(1, 1, 3, 64, dtype=torch.float16, device=DEV)
     with pytest.raises(ValueError, match="sink_size"):
         pre.attend_prompt(x, x, x, window_size=2, sink_size=-1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,n,P,W", [(64, 17, 200, 40), (300, 129, 77, 50), (700, 1, 3000, 256)])
+def test_padding_reaches_no_query_of_the_prompt(dtype, N, n, P, W):
+    """A padded prompt and the prompt alone both hold the bound of the 64-bit result."""
+    g = gen(51)
+    B, Hkv, G, D = 3, 2, 4, 128
+    u = ref.half_step(dtype)
+    pre = make(g, Hkv, P, D, dtype)
+    q, k, v = (rows(g, (B, h, N, D), dtype, 0.2) for h in (Hkv * G, Hkv, Hkv))
+    padded = pre.attend_prompt(q, k, v, window_size=W, return_lse=True)
+    alone = pre.attend_prompt(q[1:2, :, :n], k[1:2, :, :n], v[1:2, :, :n], window_size=W,
+                              return_lse=True)
+    for h in range(Hkv * G):
+        eo, el, A, ds = expected(pre, q, k, v, 1, h, G, W, n=n)
+        for (o, lse), b in ((padded, 1), (alone, 0)):
+            ref.check(o[b, h, :n], eo, A, ds, u, u, label=f"h{h} b{b}")
+            ref.check_lse(lse[b, h, :n], el, ds, f"h{h} b{b}")
