@@ -9,7 +9,9 @@ every plan index and tile coordinate the kernels read is range-checked on
 the device, and a value out of range is recorded in the status word
 (``sbfa_device_status`` code 3) and clamped, so the access stays in bounds.
 It is the stand-in for a memory checker (none can run on the target pool):
-the odd-shape GPU tests run through it as well.
+the odd-shape GPU tests run through it as well.  The serving kernels
+(``quant_cache.cu``, ``prefix.cu``) read no plan: what they take from the
+device, lengths and counts, is clamped in every build.
 
     python graph-kernel-injection_b200/build_native.py [--verbose-ptxas] [--force] [--debug]
 """

@@ -125,7 +125,8 @@ class QuantizedStreamingKVCache:
     ``k``, ``v`` (codes [B, H, rows, D]), ``scales`` (uint8 [B, H, rows, 2]: ``e + 127``
     of K's and of V's ``2 ** e``; 255 marks a row with a NaN or an infinity, which
     reads as NaN) and ``lengths`` are the state: save them, and hand them to :meth:`load`.
-    No gradients.  Calls on one cache follow each other on one stream.
+    No gradients.  Calls that write a cache (``append``, ``load``, ``reset``) and those around them
+    follow each other on one stream; ``attend`` and ``read`` may overlap with each other.
     """
 
     def __init__(self, batch: int, heads: int, head_dim: int, sink_size: int, window_size: int,
@@ -198,7 +199,7 @@ class QuantizedStreamingKVCache:
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor,
                counts: Optional[torch.Tensor] = None) -> None:
         """Quantise and append the next ``t`` tokens of every sequence ([B, H, t, D],
-        views welcome).  ``counts`` (int64 [B] on the device, clamped to [0, t]) says how many
+        views welcome).  ``counts`` (int64, or int32, [B] on the device, clamped to [0, t]) says how many
         of them each sequence takes: the rest of a right-padded batch is not read."""
         shape = k_new.shape
         if len(shape) != 4:
@@ -210,7 +211,7 @@ class QuantizedStreamingKVCache:
         if counts is not None:
             if (tuple(counts.shape) != (self.batch,) or counts.device != self.device
                     or counts.dtype not in (torch.int64, torch.int32)):
-                raise ValueError(f"counts must be int64 [{self.batch}] on {self.device}")
+                raise ValueError(f"counts must be int64 or int32 [{self.batch}] on {self.device}")
             counts = counts.to(torch.int64).contiguous()
         if n == 0:
             return
